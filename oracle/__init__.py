@@ -66,8 +66,9 @@ _oracle = None
 
 
 def build(ref: bool = False) -> None:
-    """Run oracle/Makefile (the C oracle; with ``ref`` also oracle/_ref)."""
-    target = "all" if ref else "oracle"
+    """Run oracle/Makefile (the C oracle; with ``ref`` also oracle/_ref, where
+    the reference directory holds the sources)."""
+    target = "all" if ref and (REFERENCE_DIR / "examples" / "attention_reference.h").exists() else "oracle"
     subprocess.run(["make", "-s", "-C", str(HERE), target, f"REF={REFERENCE_DIR}"], check=True)
 
 
