@@ -147,6 +147,75 @@ typedef struct kvb_append_input {
 const char* kvb_append_shape_error(const kvb_append_shape* s);
 int kvb_append_kv(const kvb_append_shape* s, const kvb_append_input* in, void* stream);
 
+/* ---- 4-bit cache (kvbridge/attention_kv4.h has the formats and rules) ---- */
+/* Element types of dense rows, queries and outputs. */
+#define KVB_F32 0
+#define KVB_F16 1
+#define KVB_BF16 2
+
+typedef struct kvb_kv4_pool {
+  uint32_t kv_heads, dim, page_tokens, pages;
+  uint8_t* k;
+  uint8_t* v;
+  float* k_params;
+  float* v_params;
+  int32_t* positions; /* optional */
+} kvb_kv4_pool;
+
+typedef struct kvb_kv4_rows {
+  uint32_t tokens;
+  int32_t type;
+  void* k;
+  void* v;
+  int64_t k_stride, v_stride; /* elements between tokens */
+  const int64_t* slots;
+  const int32_t* positions; /* append: required iff the pool has positions */
+} kvb_kv4_rows;
+
+typedef struct kvb_kv4_query {
+  uint32_t batch, rows, q_heads, table_stride, max_tokens;
+  int32_t type;
+  float scale, softcap;
+  uint32_t window;
+  const void* q;
+  int64_t batch_stride, row_stride; /* elements */
+  const uint32_t* seq_lens;
+  const uint32_t* block_table;
+  const int32_t* q_positions;  /* optional; required iff the pool has positions */
+  const float* slopes;         /* optional */
+  const uint32_t* prefix_lens; /* optional */
+} kvb_kv4_query;
+
+typedef struct kvb_kv4_eviction {
+  uint32_t batch, kv_heads, max_tokens, budget, sinks, recent;
+  const uint32_t* seq_lens;
+  const float* weights;
+  int64_t weight_stride;
+} kvb_kv4_eviction;
+
+/* NULL when valid, else a static message. */
+const char* kvb_kv4_pool_error(const kvb_kv4_pool* pool);
+const char* kvb_kv4_query_error(const kvb_kv4_pool* pool, const kvb_kv4_query* query);
+const char* kvb_kv4_eviction_error(const kvb_kv4_eviction* eviction);
+/* quantise rows into the pool, and read slots back as dense rows */
+int kvb_append_kv4(const kvb_kv4_pool* pool, const kvb_kv4_rows* rows, void* stream);
+int kvb_load_kv4(const kvb_kv4_pool* pool, const kvb_kv4_rows* rows, void* stream);
+int kvb_attention_kv4_workspace_bytes(const kvb_kv4_pool* pool, const kvb_kv4_query* query,
+                                      size_t* bytes);
+/* out in the query's type; lse may be NULL */
+int kvb_launch_attention_kv4(const kvb_kv4_pool* pool, const kvb_kv4_query* query, void* workspace,
+                             size_t workspace_bytes, void* out, float* lse, void* stream);
+int kvb_accumulate_weights_kv4(const kvb_kv4_pool* pool, const kvb_kv4_query* query,
+                               const float* lse, float* weights, int64_t weight_stride,
+                               void* stream);
+int kvb_select_tokens(const kvb_kv4_eviction* eviction, int32_t* keep, uint32_t* kept_lens,
+                      void* stream);
+/* new_weights may be NULL */
+int kvb_compact_kv4(const kvb_kv4_pool* pool, const kvb_kv4_eviction* eviction,
+                    const uint32_t* block_table, uint32_t table_stride, const int32_t* keep,
+                    const uint32_t* new_table, uint32_t new_stride, float* new_weights,
+                    int64_t new_weight_stride, void* stream);
+
 int kvb_merge_attention_shards(unsigned shards, unsigned row_heads, unsigned dim,
                                const float* m_parts, const float* l_parts,
                                const float* n_parts, float* m, float* l, float* n,

@@ -64,3 +64,32 @@ from .api import (  # noqa: F401
     validate_shape,
 )
 from ._lib import LIB_PATH, LibraryMissing  # noqa: F401
+
+# The 4-bit cache (kv4.py) takes torch tensors; torch is imported with it.
+_KV4 = (
+    "EvictPlan",
+    "Kv4Pool",
+    "Kv4Query",
+    "Kv4Rows",
+    "accumulate_weights_kv4",
+    "append_kv4",
+    "attention_kv4_workspace_bytes",
+    "compact_kv4",
+    "launch_attention_kv4",
+    "load_kv4",
+    "select_tokens",
+)
+
+
+def __getattr__(name):
+    if name not in _KV4:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import kv4
+
+    for known in _KV4:
+        globals()[known] = getattr(kv4, known)
+    return globals()[name]
+
+
+def __dir__():
+    return sorted({*globals(), *_KV4})

@@ -7,7 +7,7 @@ implementation of the kernels to fall back to.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_bool, c_char_p, c_float, c_int, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_bool, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libkvbridge_b200.so"
@@ -83,6 +83,50 @@ class KvbAppendInput(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("k_new", "v_new", "slots", "k", "v", "k_scales", "v_scales")]
 
 
+class KvbKv4Pool(ctypes.Structure):
+    _fields_ = [(n, c_uint32) for n in ("kv_heads", "dim", "page_tokens", "pages")] + [
+        (n, c_void_p) for n in ("k", "v", "k_params", "v_params", "positions")
+    ]
+
+
+class KvbKv4Rows(ctypes.Structure):
+    _fields_ = [
+        ("tokens", c_uint32),
+        ("type", c_int32),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_stride", c_int64),
+        ("v_stride", c_int64),
+        ("slots", c_void_p),
+        ("positions", c_void_p),
+    ]
+
+
+class KvbKv4Query(ctypes.Structure):
+    _fields_ = [(n, c_uint32) for n in ("batch", "rows", "q_heads", "table_stride", "max_tokens")] + [
+        ("type", c_int32),
+        ("scale", c_float),
+        ("softcap", c_float),
+        ("window", c_uint32),
+        ("q", c_void_p),
+        ("batch_stride", c_int64),
+        ("row_stride", c_int64),
+        ("seq_lens", c_void_p),
+        ("block_table", c_void_p),
+        ("q_positions", c_void_p),
+        ("slopes", c_void_p),
+        ("prefix_lens", c_void_p),
+    ]
+
+
+class KvbKv4Eviction(ctypes.Structure):
+    _fields_ = [(n, c_uint32) for n in ("batch", "kv_heads", "max_tokens", "budget", "sinks", "recent")] + [
+        ("seq_lens", c_void_p),
+        ("weights", c_void_p),
+        ("weight_stride", c_int64),
+    ]
+
+
 # name -> (restype, argtypes); mirrors include/kvbridge_c.h
 SIGNATURES = {
     "kvb_last_error": (c_char_p, []),
@@ -151,6 +195,26 @@ SIGNATURES = {
     ),
     "kvb_append_shape_error": (c_char_p, [POINTER(KvbAppendShape)]),
     "kvb_append_kv": (c_int, [POINTER(KvbAppendShape), POINTER(KvbAppendInput), c_void_p]),
+    "kvb_kv4_pool_error": (c_char_p, [POINTER(KvbKv4Pool)]),
+    "kvb_kv4_query_error": (c_char_p, [POINTER(KvbKv4Pool), POINTER(KvbKv4Query)]),
+    "kvb_kv4_eviction_error": (c_char_p, [POINTER(KvbKv4Eviction)]),
+    "kvb_append_kv4": (c_int, [POINTER(KvbKv4Pool), POINTER(KvbKv4Rows), c_void_p]),
+    "kvb_load_kv4": (c_int, [POINTER(KvbKv4Pool), POINTER(KvbKv4Rows), c_void_p]),
+    "kvb_attention_kv4_workspace_bytes": (c_int, [POINTER(KvbKv4Pool), POINTER(KvbKv4Query), POINTER(c_size_t)]),
+    "kvb_launch_attention_kv4": (
+        c_int,
+        [POINTER(KvbKv4Pool), POINTER(KvbKv4Query), c_void_p, c_size_t, c_void_p, c_void_p, c_void_p],
+    ),
+    "kvb_accumulate_weights_kv4": (
+        c_int,
+        [POINTER(KvbKv4Pool), POINTER(KvbKv4Query), c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "kvb_select_tokens": (c_int, [POINTER(KvbKv4Eviction), c_void_p, c_void_p, c_void_p]),
+    "kvb_compact_kv4": (
+        c_int,
+        [POINTER(KvbKv4Pool), POINTER(KvbKv4Eviction), c_void_p, c_uint32, c_void_p, c_void_p, c_uint32, c_void_p,
+         c_int64, c_void_p],
+    ),
     "kvb_merge_attention_shards": (
         c_int,
         [

@@ -11,6 +11,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -22,7 +23,7 @@ BUILD_DIR = PKG / "_build"
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-SOURCES = ["attention_shape.cpp", "attention.cu", "c_api.cpp"]
+SOURCES = ["attention_shape.cpp", "attention.cu", "kv4.cu", "c_api.cpp"]
 HEADERS = [
     "kvb_device.cuh",
     "kvb_schedule.h",
@@ -33,7 +34,12 @@ HEADERS = [
     "merge.cuh",
     "peer_merge.cuh",
     "append_kv.cuh",
+    "kv4_common.cuh",
+    "kv4_store.cuh",
+    "kv4_attend.cuh",
+    "kv4_evict.cuh",
     "launch_checks.h",
+    "launch_internal.h",
 ]
 
 
@@ -73,7 +79,7 @@ def build(force: bool = False, verbose_ptxas: bool = False, trace: bool = False)
     common = ["-std=c++17", "-O3", f"-I{INCLUDE}", f"-I{CSRC}", "-Xcompiler", "-fPIC"]
     if trace:
         common.append("-DKVB_TC_TRACE")
-    objects = []
+    objects, cmds = [], []
     for src in SOURCES:
         obj = build_dir / (Path(src).stem + ".o")
         cmd = [NVCC, *common, "-c", str(CSRC / src), "-o", str(obj)]
@@ -81,8 +87,10 @@ def build(force: bool = False, verbose_ptxas: bool = False, trace: bool = False)
             cmd[1:1] = [*ARCH, "-lineinfo", "--expt-relaxed-constexpr"]
             if verbose_ptxas:
                 cmd.insert(1, "-Xptxas=-v")
-        _run(cmd)
+        cmds.append(cmd)
         objects.append(str(obj))
+    with ThreadPoolExecutor() as pool:  # the sources compile side by side
+        list(pool.map(_run, cmds))
     tmp = lib.with_suffix(".so.tmp")
     _run([NVCC, *ARCH, "-shared", "-o", str(tmp), *objects, "-Xlinker", "-Bsymbolic"])
     os.replace(tmp, lib)

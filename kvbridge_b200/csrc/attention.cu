@@ -18,7 +18,9 @@
 
 #include "kvbridge/attention_b200.h"
 #include "kvbridge/attention_common.h"
+#include "kvbridge/attention_kv4.h"
 #include "launch_checks.h"
+#include "launch_internal.h"
 #include "decode_simt.cuh"
 #include "decode_tma.cuh"
 #include "decode_tc.cuh"
@@ -1095,7 +1097,10 @@ cudaError_t read_device_status(int* status) {
   if (code != cudaSuccess) return code;
   const int zero = 0;
   code = cudaMemcpyToSymbol(kvb::g_kvb_status, &zero, sizeof(int));
-  *status = value;
+  if (code != cudaSuccess) return code;
+  int kv4 = 0;
+  code = detail::read_kv4_status(&kv4);
+  *status = std::max(value, kv4);
   return code;
 }
 
@@ -1104,7 +1109,12 @@ cudaError_t read_wait_failure(long long* record6) {
   cudaError_t code = cudaMemcpyFromSymbol(record6, kvb::g_kvb_first_failure, 6 * sizeof(long long));
   if (code != cudaSuccess) return code;
   const long long zeros[6] = {0, 0, 0, 0, 0, 0};
-  return cudaMemcpyToSymbol(kvb::g_kvb_first_failure, zeros, sizeof(zeros));
+  code = cudaMemcpyToSymbol(kvb::g_kvb_first_failure, zeros, sizeof(zeros));
+  if (code != cudaSuccess) return code;
+  long long kv4[6] = {};
+  code = detail::read_kv4_wait_failure(kv4);
+  if (record6[0] == 0) std::copy(kv4, kv4 + 6, record6);
+  return code;
 }
 
 void set_wait_limit_ns(unsigned long long ns) noexcept {
@@ -1114,6 +1124,13 @@ void set_wait_limit_ns(unsigned long long ns) noexcept {
 unsigned long long wait_limit_ns() noexcept { return g_wait_limit_ns.load(); }
 
 namespace detail {
+
+void launch_kernel_pdl(const void* fn, dim3 grid, dim3 block, uint32_t smem, cudaStream_t stream,
+                       void** args, const char* what) {
+  launch_pdl(fn, grid, block, smem, stream, args, what);
+}
+
+int device_sms() { return current_device_facts().sms; }
 
 cudaError_t read_tc_trace(unsigned long long* out, size_t count, bool* available) noexcept {
 #ifdef KVB_TC_TRACE

@@ -7,9 +7,11 @@
 #include <exception>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "kvbridge/attention_b200.h"
 #include "kvbridge/attention_common.h"
+#include "kvbridge/attention_kv4.h"
 #include "kvbridge_c.h"
 #include "kvb_schedule.h"
 
@@ -64,6 +66,36 @@ kvbridge::BatchInput to_batch_input(const kvb_batch_input* in) {
   if (in == nullptr) throw std::invalid_argument("input pointer is null");
   return kvbridge::BatchInput{in->q, in->seq_lens, in->block_table, in->k,
                               in->v, in->k_scales, in->v_scales};
+}
+
+// The kv4 structs have the fields of their kvbridge:: counterparts in the
+// same order; they are read through this copy.
+template <class To, class From>
+To kv4_struct(const From* from, const char* null_message) {
+  static_assert(sizeof(To) == sizeof(From) && alignof(To) == alignof(From));
+  static_assert(std::is_trivially_copyable_v<To> && std::is_trivially_copyable_v<From>);
+  if (from == nullptr) throw std::invalid_argument(null_message);
+  To to;
+  std::memcpy(&to, from, sizeof(to));
+  return to;
+}
+static_assert(offsetof(kvb_kv4_pool, positions) == offsetof(kvbridge::Kv4Pool, positions));
+static_assert(offsetof(kvb_kv4_rows, positions) == offsetof(kvbridge::Kv4Rows, positions));
+static_assert(offsetof(kvb_kv4_query, q) == offsetof(kvbridge::Kv4Query, q));
+static_assert(offsetof(kvb_kv4_query, prefix_lens) == offsetof(kvbridge::Kv4Query, prefix_lens));
+static_assert(offsetof(kvb_kv4_eviction, weights) == offsetof(kvbridge::Kv4Eviction, weights));
+
+kvbridge::Kv4Pool to_kv4_pool(const kvb_kv4_pool* p) {
+  return kv4_struct<kvbridge::Kv4Pool>(p, "pool pointer is null");
+}
+kvbridge::Kv4Rows to_kv4_rows(const kvb_kv4_rows* r) {
+  return kv4_struct<kvbridge::Kv4Rows>(r, "rows pointer is null");
+}
+kvbridge::Kv4Query to_kv4_query(const kvb_kv4_query* q) {
+  return kv4_struct<kvbridge::Kv4Query>(q, "query pointer is null");
+}
+kvbridge::Kv4Eviction to_kv4_eviction(const kvb_kv4_eviction* e) {
+  return kv4_struct<kvbridge::Kv4Eviction>(e, "eviction pointer is null");
 }
 
 template <class F>
@@ -344,6 +376,72 @@ int kvb_debug_copy_to_device(void* dst, const void* src, size_t bytes) {
     if (dst == nullptr || src == nullptr) throw std::invalid_argument("null pointer");
     const cudaError_t code = cudaMemcpy(dst, src, bytes, cudaMemcpyHostToDevice);
     if (code != cudaSuccess) throw std::runtime_error(std::string("copy: ") + cudaGetErrorString(code));
+  });
+}
+
+const char* kvb_kv4_pool_error(const kvb_kv4_pool* pool) {
+  return pool == nullptr ? "pool pointer is null" : kvbridge::kv4_pool_error(to_kv4_pool(pool));
+}
+
+const char* kvb_kv4_query_error(const kvb_kv4_pool* pool, const kvb_kv4_query* query) {
+  if (pool == nullptr) return "pool pointer is null";
+  if (query == nullptr) return "query pointer is null";
+  return kvbridge::kv4_query_error(to_kv4_pool(pool), to_kv4_query(query));
+}
+
+const char* kvb_kv4_eviction_error(const kvb_kv4_eviction* eviction) {
+  return eviction == nullptr ? "eviction pointer is null"
+                             : kvbridge::kv4_eviction_error(to_kv4_eviction(eviction));
+}
+
+int kvb_append_kv4(const kvb_kv4_pool* pool, const kvb_kv4_rows* rows, void* stream) {
+  return guarded([&] { kvbridge::append_kv4(to_kv4_pool(pool), to_kv4_rows(rows), as_stream(stream)); });
+}
+
+int kvb_load_kv4(const kvb_kv4_pool* pool, const kvb_kv4_rows* rows, void* stream) {
+  return guarded([&] { kvbridge::load_kv4(to_kv4_pool(pool), to_kv4_rows(rows), as_stream(stream)); });
+}
+
+int kvb_attention_kv4_workspace_bytes(const kvb_kv4_pool* pool, const kvb_kv4_query* query,
+                                      size_t* bytes) {
+  return guarded([&] {
+    const size_t v = kvbridge::attention_kv4_workspace_bytes(to_kv4_pool(pool), to_kv4_query(query));
+    if (bytes == nullptr) throw std::invalid_argument("output pointer is null");
+    *bytes = v;
+  });
+}
+
+int kvb_launch_attention_kv4(const kvb_kv4_pool* pool, const kvb_kv4_query* query, void* workspace,
+                             size_t workspace_bytes, void* out, float* lse, void* stream) {
+  return guarded([&] {
+    kvbridge::launch_attention_kv4(to_kv4_pool(pool), to_kv4_query(query), workspace,
+                                   workspace_bytes, out, lse, as_stream(stream));
+  });
+}
+
+int kvb_accumulate_weights_kv4(const kvb_kv4_pool* pool, const kvb_kv4_query* query,
+                               const float* lse, float* weights, int64_t weight_stride,
+                               void* stream) {
+  return guarded([&] {
+    kvbridge::accumulate_weights_kv4(to_kv4_pool(pool), to_kv4_query(query), lse, weights,
+                                     weight_stride, as_stream(stream));
+  });
+}
+
+int kvb_select_tokens(const kvb_kv4_eviction* eviction, int32_t* keep, uint32_t* kept_lens,
+                      void* stream) {
+  return guarded(
+      [&] { kvbridge::select_tokens(to_kv4_eviction(eviction), keep, kept_lens, as_stream(stream)); });
+}
+
+int kvb_compact_kv4(const kvb_kv4_pool* pool, const kvb_kv4_eviction* eviction,
+                    const uint32_t* block_table, uint32_t table_stride, const int32_t* keep,
+                    const uint32_t* new_table, uint32_t new_stride, float* new_weights,
+                    int64_t new_weight_stride, void* stream) {
+  return guarded([&] {
+    kvbridge::compact_kv4(to_kv4_pool(pool), to_kv4_eviction(eviction), block_table, table_stride,
+                          keep, new_table, new_stride, new_weights, new_weight_stride,
+                          as_stream(stream));
   });
 }
 

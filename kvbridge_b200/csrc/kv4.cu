@@ -1,0 +1,325 @@
+// Launchers of the 4-bit cache operators (include/kvbridge/attention_kv4.h).
+#include <algorithm>
+#include <cmath>
+#include <limits>
+#include <stdexcept>
+#include <string>
+#include <type_traits>
+
+#include "kvbridge/attention_b200.h"
+#include "kvbridge/attention_kv4.h"
+#include "kv4_attend.cuh"
+#include "kv4_evict.cuh"
+#include "kv4_store.cuh"
+#include "launch_checks.h"
+#include "launch_internal.h"
+
+namespace kvbridge {
+namespace {
+
+using detail::aligned_to;
+using detail::cuda_ok;
+using detail::launch_kernel_pdl;
+
+constexpr uint32_t kMaxColumns = 128;  // query rows x heads of a KV head
+
+void require(const char* error) {
+  if (error != nullptr) throw std::invalid_argument(error);
+}
+
+uintptr_t type_bytes(Kv4Type t) { return t == Kv4Type::f32 ? 4 : 2; }
+
+bool type_ok(Kv4Type t) { return t == Kv4Type::f32 || t == Kv4Type::f16 || t == Kv4Type::bf16; }
+
+void check_pool(const Kv4Pool& p) {
+  require(kv4_pool_error(p));
+  if (!p.k || !p.v || !p.k_params || !p.v_params)
+    throw std::invalid_argument("kv4 pool buffers must be non-null");
+  if (!aligned_to(p.k, 16) || !aligned_to(p.v, 16) || !aligned_to(p.k_params, 16) ||
+      !aligned_to(p.v_params, 16) || !aligned_to(p.positions, 16))
+    throw std::invalid_argument("kv4 pool buffers must be 16-byte aligned");
+}
+
+kvb::Kv4View view(const Kv4Pool& p) {
+  return kvb::Kv4View{p.k, p.v, reinterpret_cast<float2*>(p.k_params),
+                      reinterpret_cast<float2*>(p.v_params), p.positions, p.kv_heads, p.pages};
+}
+
+// Calls f(integral_constant<int, D>) with the pool's head dim.
+template <class F>
+auto by_dim(uint32_t dim, F&& f) {
+  if (dim == 64) return f(std::integral_constant<int, 64>{});
+  if (dim == 128) return f(std::integral_constant<int, 128>{});
+  return f(std::integral_constant<int, 256>{});
+}
+
+// Calls f(T{}) with the C++ type of a Kv4Type.
+template <class F>
+auto by_type(Kv4Type type, F&& f) {
+  if (type == Kv4Type::f32) return f(float{});
+  if (type == Kv4Type::f16) return f(__half{});
+  return f(__nv_bfloat16{});
+}
+
+template <class P>
+void launch(const void* fn, dim3 grid, uint32_t threads, uint32_t smem, cudaStream_t stream, P prm,
+            uint32_t page_tokens, const char* what) {
+  void* args[] = {&prm, &page_tokens};
+  launch_kernel_pdl(fn, grid, dim3(threads), smem, stream, args, what);
+}
+
+}  // namespace
+
+const char* kv4_pool_error(const Kv4Pool& p) noexcept {
+  if (p.kv_heads == 0 || p.kv_heads > 65535) return "kv_heads must be in [1, 65535]";
+  if (p.dim != 64 && p.dim != 128 && p.dim != 256) return "kv4 needs dim 64, 128 or 256";
+  if (p.page_tokens != 16 && p.page_tokens != 32 && p.page_tokens != 64)
+    return "kv4 needs page_tokens 16, 32 or 64";
+  if (p.pages == 0) return "pages must be positive";
+  if (uint64_t(p.pages) * p.kv_heads >= (uint64_t(1) << 34)) return "kv4 pool extent too large";
+  return nullptr;
+}
+
+namespace {
+
+// Shared checks of append_kv4 and load_kv4; false if there is nothing to do.
+bool check_rows(const Kv4Pool& pool, const Kv4Rows& rows) {
+  require(kv4_pool_error(pool));
+  if (!type_ok(rows.type)) throw std::invalid_argument("unknown element type");
+  if (rows.tokens == 0) return false;
+  check_pool(pool);
+  if (!rows.k || !rows.v || !rows.slots)
+    throw std::invalid_argument("kv4 rows and slots must be non-null device buffers");
+  const uintptr_t bytes = type_bytes(rows.type);
+  if (!aligned_to(rows.k, bytes) || !aligned_to(rows.v, bytes) || !aligned_to(rows.slots, 8) ||
+      !aligned_to(rows.positions, 4))
+    throw std::invalid_argument("kv4 rows, slots and positions must be aligned to their elements");
+  const int64_t width = int64_t(pool.kv_heads) * pool.dim;
+  if (rows.tokens > 1 && (rows.k_stride < width || rows.v_stride < width))
+    throw std::invalid_argument("kv4 row strides must be at least kv_heads * dim");
+  return true;
+}
+
+kvb::Kv4RowsParams rows_params(const Kv4Pool& pool, const Kv4Rows& rows) {
+  return kvb::Kv4RowsParams{view(pool),     rows.k,     rows.v,         rows.k_stride,
+                            rows.v_stride,  rows.slots, rows.positions, rows.tokens,
+                            uint64_t(pool.pages) * pool.page_tokens};
+}
+
+uint32_t row_blocks(const Kv4Pool& pool, const Kv4Rows& rows) {
+  const uint64_t warps = uint64_t(rows.tokens) * pool.kv_heads * 2;
+  const uint64_t blocks = (warps + kvb::kKv4RowWarps - 1) / kvb::kKv4RowWarps;
+  if (blocks > 0x7fffffffull) throw std::invalid_argument("kv4 rows call too large for one grid");
+  return uint32_t(blocks);
+}
+
+}  // namespace
+
+void append_kv4(const Kv4Pool& pool, const Kv4Rows& rows, cudaStream_t stream) {
+  if (!check_rows(pool, rows)) return;
+  if (pool.positions != nullptr && rows.positions == nullptr)
+    throw std::invalid_argument("the pool keeps positions: append_kv4 needs the rows' positions");
+  const void* fn = by_dim(pool.dim, [&](auto d) {
+    return by_type(rows.type, [&](auto t) {
+      return reinterpret_cast<const void*>(&kvb::append_kv4_rows_kernel<decltype(t), decltype(d)::value>);
+    });
+  });
+  launch(fn, dim3(row_blocks(pool, rows)), 32 * kvb::kKv4RowWarps, 0, stream, rows_params(pool, rows),
+         pool.page_tokens, "kv4 append launch");
+}
+
+void load_kv4(const Kv4Pool& pool, const Kv4Rows& rows, cudaStream_t stream) {
+  if (!check_rows(pool, rows)) return;
+  const void* fn = by_dim(pool.dim, [&](auto d) {
+    return by_type(rows.type, [&](auto t) {
+      return reinterpret_cast<const void*>(&kvb::load_kv4_rows_kernel<decltype(t), decltype(d)::value>);
+    });
+  });
+  launch(fn, dim3(row_blocks(pool, rows)), 32 * kvb::kKv4RowWarps, 0, stream, rows_params(pool, rows),
+         pool.page_tokens, "kv4 load launch");
+}
+
+// ---------------------------------------------------------------------------
+// Attention and weights.
+
+const char* kv4_query_error(const Kv4Pool& pool, const Kv4Query& q) noexcept {
+  if (const char* e = kv4_pool_error(pool)) return e;
+  if (q.batch == 0 || q.rows == 0 || q.q_heads == 0) return "batch, rows and q_heads must be positive";
+  if (q.q_heads % pool.kv_heads) return "q_heads must be divisible by kv_heads";
+  if (uint64_t(q.rows) * (q.q_heads / pool.kv_heads) > kMaxColumns)
+    return "rows * (q_heads / kv_heads) must be at most 128";
+  if (!type_ok(q.type)) return "unknown element type";
+  if (q.batch > 65535) return "batch must be at most 65535";
+  if (q.table_stride == 0) return "table_stride must be positive";
+  if (q.max_tokens > 0x7fffffffu - 65536u) return "max_tokens must be below 2^31 - 65536";
+  if (!std::isfinite(q.scale)) return "score scale must be finite";
+  if (!std::isfinite(q.softcap) || q.softcap < 0.f) return "softcap must be finite and not negative";
+  if (uint64_t(q.batch) * q.rows * q.q_heads > 0x7fffffffull) return "batch/row/head product too large";
+  if (q.batch_stride < 0 || q.row_stride < 0) return "query strides must not be negative";
+  return nullptr;
+}
+
+namespace {
+
+kvb::Kv4AttendParams check_query(const Kv4Pool& pool, const Kv4Query& q) {
+  require(kv4_query_error(pool, q));
+  check_pool(pool);
+  if (!q.q || !q.seq_lens || !q.block_table)
+    throw std::invalid_argument("kv4 query, seq_lens and block_table must be non-null");
+  if (!aligned_to(q.q, type_bytes(q.type)) || !aligned_to(q.seq_lens, 4) ||
+      !aligned_to(q.block_table, 4) || !aligned_to(q.q_positions, 4) || !aligned_to(q.slopes, 4) ||
+      !aligned_to(q.prefix_lens, 4))
+    throw std::invalid_argument("kv4 query buffers must be aligned to their elements");
+  if (pool.positions != nullptr && q.q_positions == nullptr)
+    throw std::invalid_argument("the pool keeps positions: the query needs q_positions");
+  kvb::Kv4AttendParams prm{};
+  prm.pool = view(pool);
+  prm.rule = kvb::Kv4Rule{q.scale, q.softcap, q.window, q.slopes, q.prefix_lens, q.q_positions};
+  prm.q = q.q;
+  prm.batch_stride = q.batch_stride;
+  prm.row_stride = q.row_stride;
+  prm.seq_lens = q.seq_lens;
+  prm.table = q.block_table;
+  prm.batch = q.batch;
+  prm.rows = q.rows;
+  prm.q_heads = q.q_heads;
+  prm.group = q.q_heads / pool.kv_heads;
+  prm.table_stride = q.table_stride;
+  prm.max_tokens = uint32_t(std::min<uint64_t>(q.max_tokens, uint64_t(q.table_stride) * pool.page_tokens));
+  return prm;
+}
+
+}  // namespace
+
+size_t attention_kv4_workspace_bytes(const Kv4Pool& pool, const Kv4Query& q) {
+  require(kv4_query_error(pool, q));
+  return 16;
+}
+
+void launch_attention_kv4(const Kv4Pool& pool, const Kv4Query& q, void* workspace,
+                          size_t workspace_bytes, void* out, float* lse, cudaStream_t stream) {
+  kvb::Kv4AttendParams prm = check_query(pool, q);
+  if (!workspace || !out) throw std::invalid_argument("kv4 workspace and output must be non-null");
+  if (!aligned_to(workspace, 16) || !aligned_to(out, type_bytes(q.type)) || !aligned_to(lse, 4))
+    throw std::invalid_argument("kv4 workspace must be 16-byte aligned, outputs to their elements");
+  if (workspace_bytes < attention_kv4_workspace_bytes(pool, q))
+    throw std::invalid_argument("workspace smaller than attention_kv4_workspace_bytes(pool, query)");
+  prm.out = out;
+  prm.lse = lse;
+  by_dim(pool.dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    const void* fn = by_type(q.type, [&](auto t) {
+      return reinterpret_cast<const void*>(&kvb::attend_kv4_rows_kernel<decltype(t), D>);
+    });
+    launch(fn, dim3(q.batch * q.rows * q.q_heads), D, 0, stream, prm, pool.page_tokens, "kv4 attention launch");
+  });
+}
+
+void accumulate_weights_kv4(const Kv4Pool& pool, const Kv4Query& q, const float* lse, float* weights,
+                            int64_t weight_stride, cudaStream_t stream) {
+  kvb::Kv4AttendParams prm = check_query(pool, q);
+  if (!lse || !weights) throw std::invalid_argument("kv4 lse and weights must be non-null");
+  if (!aligned_to(lse, 4) || !aligned_to(weights, 4))
+    throw std::invalid_argument("kv4 lse and weights must be 4-byte aligned");
+  if (weight_stride < int64_t(prm.max_tokens))
+    throw std::invalid_argument("weight_stride must be at least max_tokens");
+  if (prm.max_tokens == 0) return;
+  prm.lse_in = lse;
+  prm.weights = weights;
+  prm.weight_stride = weight_stride;
+  by_dim(pool.dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    const void* fn = by_type(q.type, [&](auto t) {
+      return reinterpret_cast<const void*>(&kvb::weigh_kv4_rows_kernel<decltype(t), D>);
+    });
+    launch(fn, dim3((prm.max_tokens + 7) / 8, pool.kv_heads, q.batch), 256, 0, stream, prm, pool.page_tokens,
+           "kv4 weights launch");
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Eviction.
+
+const char* kv4_eviction_error(const Kv4Eviction& e) noexcept {
+  if (e.batch == 0 || e.batch > 65535) return "batch must be in [1, 65535]";
+  if (e.kv_heads == 0 || e.kv_heads > 65535) return "kv_heads must be in [1, 65535]";
+  if (uint64_t(e.batch) * e.kv_heads > 0x7fffffffull) return "batch/head product too large";
+  if (e.max_tokens > 0x7fffffffu - 65536u) return "max_tokens must be below 2^31 - 65536";
+  if (e.budget == 0 || e.budget > 0x7fffffffu - 65536u) return "budget must be positive and below 2^31 - 65536";
+  if (uint64_t(e.sinks) + e.recent > e.budget) return "sinks + recent must not exceed budget";
+  if (e.weight_stride < int64_t(e.max_tokens)) return "weight_stride must be at least max_tokens";
+  return nullptr;
+}
+
+namespace {
+
+void check_eviction(const Kv4Eviction& e) {
+  require(kv4_eviction_error(e));
+  if (!e.seq_lens || !e.weights) throw std::invalid_argument("eviction seq_lens and weights must be non-null");
+  if (!aligned_to(e.seq_lens, 4) || !aligned_to(e.weights, 4))
+    throw std::invalid_argument("eviction seq_lens and weights must be 4-byte aligned");
+}
+
+}  // namespace
+
+void select_tokens(const Kv4Eviction& e, int32_t* keep, uint32_t* kept_lens, cudaStream_t stream) {
+  check_eviction(e);
+  if (!keep || !kept_lens) throw std::invalid_argument("keep and kept_lens must be non-null");
+  if (!aligned_to(keep, 4) || !aligned_to(kept_lens, 4))
+    throw std::invalid_argument("keep and kept_lens must be 4-byte aligned");
+  kvb::SelectParams prm{e.seq_lens, e.weights,    e.weight_stride, keep,    kept_lens, e.batch,
+                        e.kv_heads, e.max_tokens, e.budget,        e.sinks, e.recent};
+  void* args[] = {&prm};
+  launch_kernel_pdl(reinterpret_cast<const void*>(&kvb::select_tokens_kernel), dim3(e.batch * e.kv_heads),
+                    dim3(kvb::kSelectThreads), 0, stream, args, "token selection launch");
+}
+
+void compact_kv4(const Kv4Pool& pool, const Kv4Eviction& e, const uint32_t* block_table,
+                 uint32_t table_stride, const int32_t* keep, const uint32_t* new_table,
+                 uint32_t new_stride, float* new_weights, int64_t new_weight_stride,
+                 cudaStream_t stream) {
+  check_pool(pool);
+  check_eviction(e);
+  if (e.kv_heads != pool.kv_heads) throw std::invalid_argument("eviction kv_heads differ from the pool's");
+  if (!block_table || !keep || !new_table)
+    throw std::invalid_argument("block_table, keep and new_table must be non-null");
+  if (!aligned_to(block_table, 4) || !aligned_to(keep, 4) || !aligned_to(new_table, 4) ||
+      !aligned_to(new_weights, 4))
+    throw std::invalid_argument("eviction buffers must be 4-byte aligned");
+  if (table_stride == 0 || new_stride == 0)
+    throw std::invalid_argument("block-table strides must be positive");
+  if (uint64_t(std::min(e.budget, e.max_tokens)) > uint64_t(new_stride) * pool.page_tokens)
+    throw std::invalid_argument("budget exceeds the new block-table row capacity");
+  if (new_weights != nullptr && new_weight_stride < int64_t(e.budget))
+    throw std::invalid_argument("new_weight_stride must be at least budget");
+  const uint32_t pages = (e.budget + pool.page_tokens - 1) / pool.page_tokens;
+  kvb::CompactParams prm{view(pool), e.seq_lens, e.weights,   e.weight_stride,   block_table,
+                         keep,       new_table,  new_weights, new_weight_stride, e.batch,
+                         e.max_tokens, e.budget, table_stride, new_stride};
+  const void* fn = by_dim(pool.dim, [&](auto d) {
+    return reinterpret_cast<const void*>(&kvb::compact_kv4_kernel<decltype(d)::value>);
+  });
+  launch(fn, dim3(pages, e.kv_heads, e.batch), 128, 0, stream, prm, pool.page_tokens, "kv4 compaction launch");
+}
+
+// ---------------------------------------------------------------------------
+
+namespace detail {
+
+cudaError_t read_kv4_status(int* status) noexcept {
+  cudaError_t code = cudaMemcpyFromSymbol(status, kvb::g_kvb_status, sizeof(int));
+  if (code != cudaSuccess) return code;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(kvb::g_kvb_status, &zero, sizeof(int));
+}
+
+cudaError_t read_kv4_wait_failure(long long* record6) noexcept {
+  cudaError_t code = cudaMemcpyFromSymbol(record6, kvb::g_kvb_first_failure, 6 * sizeof(long long));
+  if (code != cudaSuccess) return code;
+  const long long zeros[6] = {0, 0, 0, 0, 0, 0};
+  return cudaMemcpyToSymbol(kvb::g_kvb_first_failure, zeros, sizeof(zeros));
+}
+
+}  // namespace detail
+
+}  // namespace kvbridge
