@@ -2,8 +2,11 @@
 #include <algorithm>
 #include <cmath>
 #include <limits>
+#include <map>
+#include <mutex>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <type_traits>
 
 #include "kvbridge/attention_b200.h"
@@ -76,7 +79,7 @@ const char* kv4_pool_error(const Kv4Pool& p) noexcept {
   if (p.page_tokens != 16 && p.page_tokens != 32 && p.page_tokens != 64)
     return "kv4 needs page_tokens 16, 32 or 64";
   if (p.pages == 0) return "pages must be positive";
-  if (uint64_t(p.pages) * p.kv_heads >= (uint64_t(1) << 34)) return "kv4 pool extent too large";
+  if (uint64_t(p.pages) * p.kv_heads >= 0xffffffffull) return "kv4 pool extent too large: pages * kv_heads";
   return nullptr;
 }
 
@@ -185,15 +188,161 @@ kvb::Kv4AttendParams check_query(const Kv4Pool& pool, const Kv4Query& q) {
   prm.q_heads = q.q_heads;
   prm.group = q.q_heads / pool.kv_heads;
   prm.table_stride = q.table_stride;
+  prm.page_tokens = pool.page_tokens;
+  prm.log2_page = pool.page_tokens == 64 ? 6 : pool.page_tokens == 32 ? 5 : 4;
+  prm.type = int32_t(q.type);
+  const int64_t per = int64_t(16 / type_bytes(q.type));  // elements of a vector load
+  prm.vector_q = aligned_to(q.q, 16) && q.batch_stride % per == 0 && q.row_stride % per == 0;
+  prm.wait_limit_ns = wait_limit_ns();
   prm.max_tokens = uint32_t(std::min<uint64_t>(q.max_tokens, uint64_t(q.table_stride) * pool.page_tokens));
   return prm;
 }
 
 }  // namespace
 
+namespace {
+
+// One attention or weights kernel: its entry point and its shared memory.
+struct Kv4Kernel {
+  const void* fn;
+  uint32_t smem;
+};
+
+// K and V slots a warp and CTAs an SM. Four warps of 64-token stages a CTA;
+// dim 128: 12 warps an SM with two K slots and one V slot each (75 KB a CTA),
+// at most 168 registers.
+template <int D>
+struct Kv4Shape;
+template <>
+struct Kv4Shape<64> {
+  static constexpr int kK = 2, kV = 2, kCtas = 4, kWeighK = 4, kWeighCtas = 4;
+};
+template <>
+struct Kv4Shape<128> {
+  static constexpr int kK = 2, kV = 1, kCtas = 3, kWeighK = 3, kWeighCtas = 3;
+};
+template <>
+struct Kv4Shape<256> {
+  static constexpr int kK = 1, kV = 1, kCtas = 2, kWeighK = 2, kWeighCtas = 2;
+};
+
+template <int D, int L, bool RULES>
+Kv4Kernel attend_kernel() {
+  using T = Kv4Shape<D>;
+  return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, L, T::kK, T::kV, T::kCtas, RULES>),
+          kvb::Kv4Smem<D, T::kK, T::kV>::kBytes};
+}
+
+template <int D, int L, bool RULES>
+Kv4Kernel weigh_kernel(uint32_t groups) {
+  using T = Kv4Shape<D>;
+  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, L, T::kWeighK, T::kWeighCtas, RULES>),
+          kvb::Kv4Smem<D, T::kWeighK, 0>::kBytes + groups * 32 * uint32_t(sizeof(kvb::Kv4WeighFrag<D, L>))};
+}
+
+bool has_rules(const Kv4Pool& pool, const Kv4Query& q) {
+  return q.softcap > 0.f || q.window != 0 || q.slopes || q.prefix_lens || q.q_positions || pool.positions;
+}
+
+// Column layout: three digits where four columns are enough (they cost
+// nothing there) or fp32 outputs need them, else two.
+int attend_layout(const Kv4Pool& pool, const Kv4Query& q) {
+  if (q.rows * (q.q_heads / pool.kv_heads) <= 4) return kvb::kCols4;
+  return q.type == Kv4Type::f32 ? kvb::kCols8x3 : kvb::kCols8x2;
+}
+
+template <bool RULES>
+Kv4Kernel attend_kernel(uint32_t dim, int layout) {
+  return by_dim(dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return layout == kvb::kCols4     ? attend_kernel<D, kvb::kCols4, RULES>()
+           : layout == kvb::kCols8x2 ? attend_kernel<D, kvb::kCols8x2, RULES>()
+                                     : attend_kernel<D, kvb::kCols8x3, RULES>();
+  });
+}
+
+// Weights are fp32 whatever the queries: three digits.
+template <bool RULES>
+Kv4Kernel weigh_kernel(uint32_t dim, bool four, uint32_t groups) {
+  return by_dim(dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return four ? weigh_kernel<D, kvb::kCols4, RULES>(groups) : weigh_kernel<D, kvb::kCols8x3, RULES>(groups);
+  });
+}
+
+// CTAs of a kernel that the current device holds at once. The first use on a
+// device also raises the kernel's shared-memory limit.
+uint32_t resident_ctas(const Kv4Kernel& k) {
+  static std::mutex mu;
+  static std::map<std::tuple<int, const void*, uint32_t>, uint32_t> cache;
+  int dev = 0;
+  cuda_ok(cudaGetDevice(&dev), "cudaGetDevice");
+  std::lock_guard<std::mutex> lock(mu);
+  const auto key = std::make_tuple(dev, k.fn, k.smem);
+  const auto it = cache.find(key);
+  if (it != cache.end()) return it->second;
+  // The limit may only grow: the weights kernels' shared memory varies with the query.
+  cudaFuncAttributes attr{};
+  cuda_ok(cudaFuncGetAttributes(&attr, k.fn), "kv4 kernel attributes");
+  if (uint32_t(attr.maxDynamicSharedSizeBytes) < k.smem)
+    cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(k.smem)),
+            "kv4 kernel shared-memory opt-in");
+  cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributePreferredSharedMemoryCarveout,
+                               int(cudaSharedmemCarveoutMaxShared)),
+          "kv4 kernel carveout");
+  int blocks = 0;
+  cuda_ok(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k.fn, kvb::kKv4Threads, k.smem), "occupancy query");
+  const uint32_t ctas = uint32_t(std::max(blocks, 1) * detail::device_sms());
+  cache.emplace(key, ctas);
+  return ctas;
+}
+
+// CTAs of a call whose segments have at most max_tokens tokens: a full wave,
+// or fewer so that each has a stage for every warp.
+uint32_t split_ctas(const Kv4Kernel& k, uint64_t segments, uint32_t max_tokens) {
+  const uint64_t stages = segments * ((uint64_t(max_tokens) + kvb::kStageTokens - 1) / kvb::kStageTokens);
+  const uint64_t most = (stages + kvb::kKv4Warps - 1) / kvb::kKv4Warps;
+  return uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(resident_ctas(k), most)));
+}
+
+struct AttendPlan {
+  Kv4Kernel kernel;
+  int layout;
+  bool rules, direct;
+  uint32_t col_groups, segments, ctas;
+  size_t ml_offset, ctas_offset, bytes;  // of the workspace
+};
+
+// Short sequences: one CTA per segment writes the result, nothing is merged.
+constexpr uint32_t kDirectTokens = 512;
+
+AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
+  AttendPlan a{};
+  a.rules = has_rules(pool, q);
+  a.layout = attend_layout(pool, q);
+  a.kernel = a.rules ? attend_kernel<true>(pool.dim, a.layout) : attend_kernel<false>(pool.dim, a.layout);
+  const uint32_t cols = uint32_t(kvb::kv4_cols(a.layout)), all = q.rows * (q.q_heads / pool.kv_heads);
+  a.col_groups = (all + cols - 1) / cols;
+  a.segments = q.batch * pool.kv_heads * a.col_groups;
+  a.direct = q.max_tokens <= kDirectTokens;
+  a.ctas = a.direct ? a.segments : split_ctas(a.kernel, a.segments, q.max_tokens);
+  if (a.direct) {
+    resident_ctas(a.kernel);
+    a.bytes = 16;
+    return a;
+  }
+  const size_t slots = size_t(a.ctas) + a.segments;
+  a.ml_offset = slots * cols * pool.dim * sizeof(float);
+  a.ctas_offset = a.ml_offset + slots * cols * sizeof(float2);
+  a.bytes = a.ctas_offset + size_t(a.segments) * sizeof(uint2);
+  return a;
+}
+
+}  // namespace
+
 size_t attention_kv4_workspace_bytes(const Kv4Pool& pool, const Kv4Query& q) {
   require(kv4_query_error(pool, q));
-  return 16;
+  return plan_attention(pool, q).bytes;
 }
 
 void launch_attention_kv4(const Kv4Pool& pool, const Kv4Query& q, void* workspace,
@@ -202,17 +351,30 @@ void launch_attention_kv4(const Kv4Pool& pool, const Kv4Query& q, void* workspac
   if (!workspace || !out) throw std::invalid_argument("kv4 workspace and output must be non-null");
   if (!aligned_to(workspace, 16) || !aligned_to(out, type_bytes(q.type)) || !aligned_to(lse, 4))
     throw std::invalid_argument("kv4 workspace must be 16-byte aligned, outputs to their elements");
-  if (workspace_bytes < attention_kv4_workspace_bytes(pool, q))
+  const AttendPlan a = plan_attention(pool, q);
+  if (workspace_bytes < a.bytes)
     throw std::invalid_argument("workspace smaller than attention_kv4_workspace_bytes(pool, query)");
+  prm.col_groups = a.col_groups;
+  prm.ctas = a.ctas;
+  prm.direct = a.direct;
+  prm.part = static_cast<float*>(workspace);
+  prm.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + a.ml_offset);
+  prm.seg_ctas = reinterpret_cast<uint2*>(static_cast<uint8_t*>(workspace) + a.ctas_offset);
   prm.out = out;
   prm.lse = lse;
-  by_dim(pool.dim, [&](auto d) {
+  void* args[] = {&prm};
+  launch_kernel_pdl(a.kernel.fn, dim3(a.ctas), dim3(kvb::kKv4Threads), a.kernel.smem, stream, args,
+                    "kv4 attention launch");
+  if (a.direct) return;
+  uint32_t cols = uint32_t(kvb::kv4_cols(a.layout));
+  void* merge_args[] = {&prm, &cols};
+  const void* merge = by_dim(pool.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    const void* fn = by_type(q.type, [&](auto t) {
-      return reinterpret_cast<const void*>(&kvb::attend_kv4_rows_kernel<decltype(t), D>);
-    });
-    launch(fn, dim3(q.batch * q.rows * q.q_heads), D, 0, stream, prm, pool.page_tokens, "kv4 attention launch");
+    return a.rules ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, true>)
+                   : reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, false>);
   });
+  launch_kernel_pdl(merge, dim3(q.batch * q.rows * q.q_heads), dim3(32 * kvb::kKv4MergeWarps), 0, stream, merge_args,
+                    "kv4 merge launch");
 }
 
 void accumulate_weights_kv4(const Kv4Pool& pool, const Kv4Query& q, const float* lse, float* weights,
@@ -224,17 +386,18 @@ void accumulate_weights_kv4(const Kv4Pool& pool, const Kv4Query& q, const float*
   if (weight_stride < int64_t(prm.max_tokens))
     throw std::invalid_argument("weight_stride must be at least max_tokens");
   if (prm.max_tokens == 0) return;
+  const uint32_t all = q.rows * prm.group;
+  const bool four = all <= 4;
+  uint32_t groups = four ? 1 : (all + 7) / 8;
+  const Kv4Kernel k = has_rules(pool, q) ? weigh_kernel<true>(pool.dim, four, groups)
+                                         : weigh_kernel<false>(pool.dim, four, groups);
+  prm.col_groups = 1;
+  prm.ctas = split_ctas(k, uint64_t(q.batch) * pool.kv_heads, prm.max_tokens);
   prm.lse_in = lse;
   prm.weights = weights;
   prm.weight_stride = weight_stride;
-  by_dim(pool.dim, [&](auto d) {
-    constexpr int D = decltype(d)::value;
-    const void* fn = by_type(q.type, [&](auto t) {
-      return reinterpret_cast<const void*>(&kvb::weigh_kv4_rows_kernel<decltype(t), D>);
-    });
-    launch(fn, dim3((prm.max_tokens + 7) / 8, pool.kv_heads, q.batch), 256, 0, stream, prm, pool.page_tokens,
-           "kv4 weights launch");
-  });
+  void* args[] = {&prm, &groups};
+  launch_kernel_pdl(k.fn, dim3(prm.ctas), dim3(kvb::kKv4Threads), k.smem, stream, args, "kv4 weights launch");
 }
 
 // ---------------------------------------------------------------------------

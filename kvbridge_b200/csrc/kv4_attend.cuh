@@ -1,9 +1,53 @@
 #pragma once
 // Attention over the 4-bit pool, and the attention weight that each cached
-// token gets.
+// token gets (include/kvbridge/attention_kv4.h).
+//
+// Schedule. The attended tokens of a sequence are runs of 64-token stages;
+// one segment per (sequence, KV head, group of query columns). The segments'
+// stages, concatenated, are cut into equal contiguous ranges, one per CTA
+// (kvb_schedule.h); a CTA's part of a segment is a piece. Stage g of a CTA
+// belongs to warp g % 4. A windowed call leaves the stages between the
+// prefix and the window out of the list, so they are never read.
+//
+// A warp feeds itself: lane 0 arms the mbarrier of the next free slot and a
+// few lanes start bulk copies of the stage's pages (codes, params), K when
+// the previous K has been multiplied, V when the previous V has been. No
+// producer warp and no empty barriers: the warp that reads a slot is the one
+// that refills it.
+//
+// Arithmetic (int8 tensor cores, exact s32 sums; codes 0..15 are int8
+// operands after a mask or a shift and a mask, two values a byte):
+//   scores   The query side is the A operand: each query value as three
+//            signed base-256 digits of a fixed-point number, one A row per
+//            (column, digit). x = scale_t * (A . (codes - 8)) + (lo_t + 8
+//            scale_t) * sum(q) in fp32: the sums start at -8 * sum(digits),
+//            so that little cancels between the two parts.
+//   output   P = exp(x - m) * v_scale as unsigned fixed point against the
+//            tile's largest, in base-256 digits that are the mantissa bytes
+//            of P * 2^e + 2^23. These sums count codes from -8 too; the part
+//            that carries lo, sum exp(x - m) * (lo + 8 v_scale), is in fp32.
+//
+// Column layouts (template L):
+//   kCols4    up to 4 query columns a segment, three digits on both sides.
+//             One m16 tile holds digits 0 and 1 of column c in rows c and
+//             c + 8, digit 2 in row c + 4; lanes c and c + 4 share a column.
+//   kCols8x2  up to 8 columns, three digits of q in two m16 tiles (the lse is
+//             fp32 whatever the outputs are), two digits of P: 2^-16 of the
+//             tile's largest, below the rounding of 16-bit outputs.
+//   kCols8x3  up to 8 columns, three digits on both sides: fp32 outputs.
 #include "kv4_common.cuh"
+#include "kvb_schedule.h"
 
 namespace kvb {
+
+enum : int { kCols4 = 0, kCols8x2 = 1, kCols8x3 = 2 };
+constexpr int kv4_cols(int layout) { return layout == kCols4 ? 4 : 8; }
+constexpr int kv4_q_tiles(int layout) { return layout == kCols4 ? 1 : 2; }    // m16 tiles of the scores
+constexpr int kv4_p_tiles(int layout) { return layout == kCols8x3 ? 2 : 1; }  // and of the output
+
+constexpr int kKv4Warps = 4;
+constexpr int kKv4Threads = 32 * kKv4Warps;
+constexpr uint32_t kNoUnit = 0xffffffffu;
 
 struct Kv4AttendParams {
   Kv4View pool;
@@ -13,6 +57,18 @@ struct Kv4AttendParams {
   const uint32_t* seq_lens;
   const uint32_t* table;
   uint32_t batch, rows, q_heads, group, table_stride, max_tokens;
+  uint32_t page_tokens, log2_page;
+  uint32_t col_groups;  // groups of query columns (rows * group) of a KV head
+  uint32_t ctas;
+  int32_t type;   // of q and out: 0 f32, 1 f16, 2 bf16
+  bool vector_q;  // 16-byte aligned query rows
+  bool direct;    // one CTA per segment, which writes the outputs itself
+  unsigned long long wait_limit_ns;
+  // Partials of piece (CTA c, segment i) in slot c + i: per column D sums and
+  // {max, sum}; the first and last CTA of every segment.
+  float* part;
+  float2* part_ml;
+  uint2* seg_ctas;
   void* out;
   float* lse;
   // accumulate_weights_kv4
@@ -21,126 +77,1066 @@ struct Kv4AttendParams {
   int64_t weight_stride;
 };
 
-// Score of one token for one query row held in shared memory, or -inf.
-template <int D>
-__device__ float kv4_score(const Kv4AttendParams& p, const float* q, uint32_t P, uint64_t unit,
-                           uint32_t s, int32_t pk, int32_t pq, float slope, uint32_t prefix) {
-  if (!kv4_visible(pk, pq, p.rule.window, prefix)) return -INFINITY;
-  const uint8_t* row = p.pool.k + (unit * P + s) * (D / 2);
-  float dot = 0.f, sum = 0.f;
-  for (int i = 0; i < D / 2; ++i) {
-    const uint32_t b = row[i];
-    dot = fmaf(q[2 * i], float(b & 15u), dot);
-    dot = fmaf(q[2 * i + 1], float(b >> 4), dot);
-    sum += q[2 * i] + q[2 * i + 1];
+// ---------------------------------------------------------------------------
+// The stage list.
+
+// A segment being walked; positions are relative to the CTA's first stage.
+struct Kv4Cursor {
+  uint32_t b, seg;
+  uint32_t len;     // tokens of sequence b
+  uint32_t stages;  // of the segment
+  uint32_t head, skip;  // stage j of the segment is j (j < head) or j + skip
+  int32_t base;     // where the segment's stage 0 lies
+};
+
+template <bool RULES>
+__device__ __forceinline__ void kv4_stages(const Kv4AttendParams& p, uint32_t b, uint32_t& len,
+                                           uint32_t& stages, uint32_t& head, uint32_t& skip) {
+  len = kv4_len(p.seq_lens, b, p.max_tokens);
+  stages = (len + kStageTokens - 1) / kStageTokens;
+  head = stages;
+  skip = 0;
+  if (RULES && p.rule.window != 0 && p.pool.pos == nullptr && p.rule.q_pos == nullptr) {
+    // The first row's window starts at len - rows - window + 1.
+    const uint64_t reach = uint64_t(p.rows) + p.rule.window - 1;
+    const uint32_t from = reach < len ? uint32_t(len - reach) / kStageTokens : 0u;
+    const uint32_t fix = p.rule.prefix != nullptr ? min(__ldg(p.rule.prefix + b), len) : 0u;
+    head = (fix + kStageTokens - 1) / kStageTokens;
+    if (head < from) {
+      skip = from - head;
+      stages -= skip;
+    }
   }
-  const float2 par = p.pool.kp[unit * P + s];
-  float x = p.rule.scale * fmaf(par.x, dot, par.y * sum);
-  if (p.rule.softcap > 0.f) x = p.rule.softcap * tanhf(x / p.rule.softcap);
-  return x - slope * fabsf(float(pq - pk));
 }
 
-// One CTA of D threads per (sequence, query row, query head): tiles of D
-// tokens, one score a thread, then one output dim a thread.
-template <class T, int D>
-__global__ void __launch_bounds__(D) attend_kv4_rows_kernel(Kv4AttendParams p, uint32_t P) {
-  __shared__ float q[D], ps[D], pl[D], red[D / 32];
-  __shared__ const uint8_t* vat[D];
-  grid_dependency_wait();
-  const uint32_t tid = threadIdx.x;
-  const uint32_t head = blockIdx.x % p.q_heads, br = blockIdx.x / p.q_heads;
-  const uint32_t r = br % p.rows, b = br / p.rows, h = head / p.group;
-  const uint32_t len = kv4_len(p.seq_lens, b, p.max_tokens);
-  if (tid == 0 && __ldg(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
-  q[tid] = to_f32(static_cast<const T*>(p.q)[int64_t(b) * p.batch_stride + int64_t(r) * p.row_stride + head * D + tid]);
-  const int32_t pq = kv4_query_position(p.rule, b, r, p.rows, len);
-  const float slope = p.rule.slopes != nullptr ? p.rule.slopes[head] : 0.f;
-  const uint32_t prefix = p.rule.prefix != nullptr ? p.rule.prefix[b] : 0u;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (uint32_t base = 0; base < len; base += D) {
-    const uint32_t t = base + tid;
-    float x = -INFINITY;
-    uint64_t unit = 0;
-    uint32_t s = 0;
-    __syncthreads();
-    if (t < len) {
-      const uint32_t page = p.table[size_t(b) * p.table_stride + t / P];
-      s = t % P;
-      if (page < p.pool.pages) {
-        unit = uint64_t(page) * p.pool.kv_heads + h;
-        const int32_t pk = p.pool.pos != nullptr ? p.pool.pos[unit * P + s] : int32_t(t);
-        x = kv4_score<D>(p, q, P, unit, s, pk, pq, slope, prefix);
-      } else {
-        atomicMax(&g_kvb_status, kKv4BadPage);
+template <bool RULES>
+__device__ __forceinline__ uint32_t kv4_stage_count(const Kv4AttendParams& p, uint32_t b) {
+  uint32_t len, stages, head, skip;
+  kv4_stages<RULES>(p, b, len, stages, head, skip);
+  return stages;
+}
+
+template <bool RULES>
+__device__ __forceinline__ void kv4_load_sequence(const Kv4AttendParams& p, Kv4Cursor& c) {
+  kv4_stages<RULES>(p, c.b, c.len, c.stages, c.head, c.skip);
+}
+
+// The next segment that has stages (b = batch at the end).
+template <bool RULES>
+__device__ __forceinline__ void kv4_next_segment(const Kv4AttendParams& p, uint32_t segs, Kv4Cursor& c) {
+  c.base += int32_t(c.stages);
+  if (++c.seg < segs) return;
+  c.seg = 0;
+  while (++c.b < p.batch) {
+    kv4_load_sequence<RULES>(p, c);
+    if (c.stages != 0) return;
+  }
+}
+
+// Warp-cooperative: the CTA's range and the cursor at its first stage.
+// Returns the number of stages of the range.
+template <bool RULES>
+__device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t segs, Kv4Cursor& c) {
+  const uint32_t lane = threadIdx.x & 31;
+  if (p.direct) {
+    c.b = blockIdx.x / segs;
+    c.seg = blockIdx.x % segs;
+    c.base = 0;
+    kv4_load_sequence<RULES>(p, c);
+    return c.stages;
+  }
+  uint64_t total = 0;
+  for (uint32_t b = lane; b < p.batch; b += 32) total += kv4_stage_count<RULES>(p, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  total *= segs;
+  // No more CTAs than have a stage for every warp; the others leave.
+  const uint32_t ctas = uint32_t(min(uint64_t(p.ctas), (total + kKv4Warps - 1) / kKv4Warps));
+  if (blockIdx.x >= ctas) return 0;
+  const uint64_t x0 = cta_stage_begin(blockIdx.x, total, ctas);
+  const uint64_t x1 = cta_stage_begin(blockIdx.x + 1, total, ctas);
+  uint64_t before = 0;
+  for (uint32_t from = 0; from < p.batch; from += 32) {
+    const uint64_t n = from + lane < p.batch ? kv4_stage_count<RULES>(p, from + lane) : 0u;
+    uint64_t upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= uint32_t(o)) upto += y;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, (before + upto) * segs > x0);
+    if (hit != 0) {
+      const int at = __ffs(hit) - 1;
+      before = (before + __shfl_sync(0xffffffffu, upto - n, at)) * segs;
+      c.b = from + at;
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  kv4_load_sequence<RULES>(p, c);
+  c.seg = uint32_t((x0 - before) / c.stages);
+  c.base = -int32_t(x0 - before - uint64_t(c.seg) * c.stages);
+  return uint32_t(x1 - x0);
+}
+
+// ---------------------------------------------------------------------------
+// Shared memory of one warp.
+
+template <int D, int KR, int VR>
+struct Kv4Smem {
+  // K slot: codes, params, positions. V slot: codes (pages of 16 and 32
+  // tokens 32 and 64 bytes further apart, so that a quarter-warp's reads of
+  // several pages hit different banks), params.
+  static constexpr uint32_t kCodes = kStageTokens * D / 2;
+  static constexpr uint32_t kParams = kStageTokens * 8;
+  static constexpr uint32_t kKSlot = kCodes + kParams + kStageTokens * 4;
+  static constexpr uint32_t kVCodes = VR > 0 ? kCodes + 128 : 0;
+  static constexpr uint32_t kVSlot = VR > 0 ? kVCodes + kParams : 0;
+  static constexpr uint32_t kWarp = KR * kKSlot + VR * kVSlot;
+  static constexpr uint32_t kBars = 8 * (KR + VR);
+  // Combine buffer of the four warps: 8 columns (or column shares) of D.
+  static constexpr uint32_t kPitch = D + 4;
+  static constexpr uint32_t kCombine = VR > 0 ? kKv4Warps * 8 * kPitch * 4 : 0;
+  static constexpr uint32_t kStats = VR > 0 ? kKv4Warps * 8 * 12 : 0;  // max, sum, lo part
+  static constexpr uint32_t kOffCombine = kKv4Warps * kWarp;
+  static constexpr uint32_t kOffStats = kOffCombine + kCombine;
+  static constexpr uint32_t kOffBars = kOffStats + kStats;
+  static constexpr uint32_t kOffAbort = kOffBars + kKv4Warps * kBars;
+  static constexpr uint32_t kOffFrags = kOffAbort + 16;  // accumulate_weights_kv4
+  static constexpr uint32_t kBytes = kOffFrags;
+};
+
+__device__ __forceinline__ uint32_t kv4_v_pitch(uint32_t page_bytes, uint32_t P) {
+  return P == 64 ? page_bytes : page_bytes + 2 * P;
+}
+
+// ---------------------------------------------------------------------------
+// Feeding: the pages of the warp's stages, looked up one stage ahead of the
+// K copies, kept until the V copies.
+
+template <int D, int KR, int VR, bool RULES>
+struct Kv4Feeder {
+  uint8_t* ring;    // the warp's slots: K slots, then V slots
+  uint64_t* bars;   // KR full barriers for K, then VR for V
+  Kv4Cursor cur;    // the segment of the next stage to look up
+  uint32_t next;    // that stage, relative to the CTA's first
+  uint32_t count;   // stages of the CTA
+  uint32_t segs;
+  uint64_t policy;
+  uint32_t k_used, v_used;  // slots filled so far
+  uint32_t unit[KR + 1];  // (page, KV head) of this lane's page: stages i .. i + KR
+
+  // The pool unit of page lane % 4 of stage `next`; advances by one stage of the warp.
+  __device__ uint32_t lookup(const Kv4AttendParams& p) {
+    uint32_t found = kNoUnit;
+    if (next < count) {
+      while (int32_t(next) >= cur.base + int32_t(cur.stages)) kv4_next_segment<RULES>(p, segs, cur);
+      const uint32_t j = uint32_t(int32_t(next) - cur.base);
+      const uint32_t stage = RULES && j >= cur.head ? j + cur.skip : j;
+      const uint32_t q = threadIdx.x & 3, pps = kStageTokens >> p.log2_page;
+      const uint32_t page = stage * pps + q;
+      if (q < pps && (page << p.log2_page) < cur.len) {
+        const uint32_t phys = __ldg(p.table + size_t(cur.b) * p.table_stride + page);
+        const uint32_t h = cur.seg / p.col_groups;
+        if (phys < p.pool.pages)
+          found = phys * p.pool.kv_heads + h;
+        else
+          atomicMax(&g_kvb_status, kKv4BadPage);
       }
     }
-    float mx = warp_max(x);
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    for (int i = 0; i < D / 32; ++i) mx = fmaxf(mx, red[i]);
-    const float mnew = fmaxf(m, mx);
-    const float base_m = mnew == -INFINITY ? 0.f : mnew;
-    const float alpha = m == -INFINITY ? 0.f : expf(m - base_m);
-    const bool on = x != -INFINITY;
-    const float e = on ? expf(x - base_m) : 0.f;
-    const float2 par = on ? p.pool.vp[unit * P + s] : make_float2(0.f, 0.f);
-    ps[tid] = on ? e * par.x : 0.f;
-    pl[tid] = on ? e * par.y : 0.f;
-    vat[tid] = on ? p.pool.v + unit * (D / 2) * P + s : nullptr;
-    const float sum = warp_sum(e);
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = sum;
-    __syncthreads();
-    float lsum = 0.f;
-    for (int i = 0; i < D / 32; ++i) lsum += red[i];
-    l = l * alpha + lsum;
-    acc *= alpha;
-    for (int i = 0; i < D; ++i)
-      if (vat[i] != nullptr) {
-        const uint32_t byte = vat[i][size_t(tid / 2) * P];
-        acc += fmaf(ps[i], float((byte >> (4 * (tid & 1))) & 15u), pl[i]);
-      }
-    m = mnew;
+    next += kKv4Warps;
+    return found;
   }
-  static_cast<T*>(p.out)[size_t(blockIdx.x) * D + tid] = from_f32<T>(m == -INFINITY ? 0.f : acc / l);
-  if (tid == 0 && p.lse != nullptr) p.lse[blockIdx.x] = m == -INFINITY ? -INFINITY : m + logf(l);
+
+  // The pages u of the warp's next stage into the next K or V slot. All lanes.
+  __device__ void copy_k(const Kv4AttendParams& p, uint32_t u) {
+    const uint32_t lane = threadIdx.x & 31, q = lane & 3, part = lane >> 2, use = k_used++;
+    const uint32_t P = p.page_tokens, bytes = P * (D / 2);
+    uint8_t* slot = ring + (use % KR) * Kv4Smem<D, KR, VR>::kKSlot;
+    uint64_t* bar = bars + use % KR;
+    const bool pos = RULES && p.pool.pos != nullptr;
+    const uint32_t ok = __popc(__ballot_sync(0xffffffffu, u != kNoUnit && part == 0));
+    if (lane == 0) mbar_arrive_expect_tx(bar, ok * (bytes + P * (pos ? 12u : 8u)));
+    __syncwarp();
+    if (u == kNoUnit) return;
+    constexpr uint32_t kCodes = Kv4Smem<D, KR, VR>::kCodes;
+    if (part == 0)
+      bulk_copy_g2s(slot + q * bytes, p.pool.k + size_t(u) * bytes, bytes, bar, policy);
+    else if (part == 1)
+      bulk_copy_g2s(slot + kCodes + q * P * 8, p.pool.kp + size_t(u) * P, P * 8, bar, policy);
+    else if (part == 2 && pos)
+      bulk_copy_g2s(slot + kCodes + Kv4Smem<D, KR, VR>::kParams + q * P * 4, p.pool.pos + size_t(u) * P,
+                    P * 4, bar, policy);
+  }
+
+  __device__ void copy_v(const Kv4AttendParams& p, uint32_t u) {
+    const uint32_t lane = threadIdx.x & 31, q = lane & 3, part = lane >> 2, use = v_used++;
+    const uint32_t P = p.page_tokens, bytes = P * (D / 2);
+    uint8_t* slot = ring + KR * Kv4Smem<D, KR, VR>::kKSlot + (use % VR) * Kv4Smem<D, KR, VR>::kVSlot;
+    uint64_t* bar = bars + KR + use % VR;
+    const uint32_t ok = __popc(__ballot_sync(0xffffffffu, u != kNoUnit && part == 0));
+    if (lane == 0) mbar_arrive_expect_tx(bar, ok * (bytes + P * 8));
+    __syncwarp();
+    if (u == kNoUnit) return;
+    if (part == 0)
+      bulk_copy_g2s(slot + q * kv4_v_pitch(bytes, P), p.pool.v + size_t(u) * bytes, bytes, bar, policy);
+    else if (part == 1)
+      bulk_copy_g2s(slot + Kv4Smem<D, KR, VR>::kVCodes + q * P * 8, p.pool.vp + size_t(u) * P, P * 8,
+                    bar, policy);
+  }
+};
+
+// After a wait that gave up: lets the copies in flight (the last `ring` of
+// `used` fills of the slots) land, each for at most limit_ns.
+__device__ __forceinline__ void kv4_drain(uint64_t* bars, uint32_t ring, uint32_t used, unsigned long long limit_ns) {
+  for (uint32_t use = used > ring ? used - ring : 0; use < used; ++use) {
+    const unsigned long long start = global_ns();
+    while (!mbar_try_wait(bars + use % ring, (use / ring) & 1) && global_ns() - start < limit_ns) {
+    }
+  }
 }
 
-// One warp per (sequence, KV head, token).
-template <class T, int D>
-__global__ void __launch_bounds__(256) weigh_kv4_rows_kernel(Kv4AttendParams p, uint32_t P) {
-  __shared__ float qs[8][D];
-  grid_dependency_wait();
-  const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const uint32_t b = blockIdx.z, h = blockIdx.y;
-  const uint32_t t = blockIdx.x * 8 + w;
-  const uint32_t len = kv4_len(p.seq_lens, b, p.max_tokens);
-  if (t == 0 && lane == 0 && __ldg(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
-  if (t >= len) return;
-  const uint32_t page = p.table[size_t(b) * p.table_stride + t / P], s = t % P;
-  if (page >= p.pool.pages) {
-    if (lane == 0) atomicMax(&g_kvb_status, kKv4BadPage);
+// ---------------------------------------------------------------------------
+// Queries.
+
+// Eight consecutive query values from element `at`.
+__device__ __forceinline__ void kv4_load8(const void* q, int64_t at, int32_t type, bool vector, float (&v)[8]) {
+  if (type == 0) {
+    const float* s = static_cast<const float*>(q) + at;
+    if (vector) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(s)), b = __ldg(reinterpret_cast<const float4*>(s) + 1);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __ldg(s + i);
+    }
     return;
   }
-  const uint64_t unit = uint64_t(page) * p.pool.kv_heads + h;
-  const int32_t pk = p.pool.pos != nullptr ? p.pool.pos[unit * P + s] : int32_t(t);
-  const uint32_t prefix = p.rule.prefix != nullptr ? p.rule.prefix[b] : 0u;
-  float total = 0.f;
-  for (uint32_t r = 0; r < p.rows; ++r)
-    for (uint32_t g = 0; g < p.group; ++g) {
-      const uint32_t head = h * p.group + g;
-      for (int i = lane; i < D; i += 32)
-        qs[w][i] = to_f32(static_cast<const T*>(p.q)[int64_t(b) * p.batch_stride + int64_t(r) * p.row_stride + head * D + i]);
-      __syncwarp();
-      if (lane == 0) {
-        const int32_t pq = kv4_query_position(p.rule, b, r, p.rows, len);
-        const float slope = p.rule.slopes != nullptr ? p.rule.slopes[head] : 0.f;
-        const float x = kv4_score<D>(p, qs[w], P, unit, s, pk, pq, slope, prefix);
-        if (x != -INFINITY) total += expf(x - p.lse_in[(size_t(b) * p.rows + r) * p.q_heads + head]);
+  const uint16_t* s = static_cast<const uint16_t*>(q) + at;
+  uint32_t w[4];
+  if (vector) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(s));
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __ldg(s + 2 * i) | (uint32_t(__ldg(s + 2 * i + 1)) << 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (type == 1) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    } else {
+      v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+// The A operand of the scores for one group of columns. Lane (grp, tig) =
+// (lane / 4, lane % 4) holds column grp (kCols4: grp % 4) at the dims of its
+// quarter of each K row: word i of the lane's packed row covers 8 dims, the
+// even ones in the low halves (a[.][0], a[.][1]), the odd ones in the high
+// halves (a[.][2], a[.][3]).
+template <int D, int L>
+struct Kv4Query {
+  uint32_t a[kv4_q_tiles(L)][D / 32][4];
+  int start[kv4_q_tiles(L)][2];  // -8 * digit sums of rows grp and grp + 8
+  float dot, sum;  // score = scale_t * dot * (A . (codes - 8)) + (lo_t + 8 scale_t) * sum
+  float slope;
+  int32_t pos;     // query position
+};
+
+// First dim of word i of the lane's part of a packed row.
+template <int D>
+__device__ __forceinline__ uint32_t kv4_word_dim(uint32_t tig, uint32_t i) {
+  if constexpr (D == 256) return 128 * (i / 4) + 32 * tig + 8 * (i % 4);
+  return (D / 4) * tig + 8 * i;
+}
+
+template <int D, int L, bool RULES>
+__device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h, uint32_t col_group,
+                               uint32_t len, Kv4Query<D, L>& qf) {
+  const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
+  const uint32_t col = col_group * kv4_cols(L) + (L == kCols4 ? grp & 3 : grp);
+  const bool valid = col < p.rows * p.group;
+  const uint32_t r = valid ? col / p.group : 0, head = h * p.group + (valid ? col % p.group : 0);
+  const int64_t at = int64_t(b) * p.batch_stride + int64_t(r) * p.row_stride + int64_t(head) * D;
+  float v[D / 32][8];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) kv4_load8(p.q, at + kv4_word_dim<D>(tig, i), p.type, p.vector_q, v[i]);
+  float amax = 0.f;
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      finite = finite && fabsf(v[i][e]) <= 3.402823466e38f;
+      amax = fmaxf(amax, fabsf(v[i][e]));
+    }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  finite = __reduce_and_sync(0xfu << (4 * grp), finite ? 1u : 0u) != 0;
+  // Fixed point n = rint(q * up), |n| <= 2^22: n = d0 + 256 d1 + 65536 d2
+  // with signed digits; up is a power of two.
+  int e = int((__float_as_uint(amax) >> 23) & 0xffu) - 126;  // amax < 2^e
+  e = max(-100, min(128, e));
+  const float up = __uint_as_float(uint32_t(127 + 22 - e) << 23);
+  const float down = __uint_as_float(uint32_t(127 + e - 22) << 23);
+  // fma(q, up, 1.5 * 2^23) rounds to the integer in the low mantissa bits;
+  // removing the sum's bias and adding 0x808080 leaves n + 0x808080, whose
+  // bytes are the digits + 128.
+  constexpr float kRoundInt = 12582912.0f;
+  constexpr uint32_t kBias = 0x808080u - 0x4B400000u;
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      uint32_t w[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        w[x] = valid ? __float_as_uint(fmaf(v[i][2 * x + odd], up, kRoundInt)) + kBias : 0x808080u;
+        total += int(w[x]) - 0x808080;
+      }
+      const uint32_t x = __byte_perm(w[0], w[1], 0x5140), y = __byte_perm(w[2], w[3], 0x5140);
+      const uint32_t d0 = __byte_perm(x, y, 0x5410) ^ 0x80808080u, d1 = __byte_perm(x, y, 0x7632) ^ 0x80808080u;
+      const uint32_t x2 = __byte_perm(w[0], w[1], 0x0062), y2 = __byte_perm(w[2], w[3], 0x0062);
+      const uint32_t d2 = __byte_perm(x2, y2, 0x5410) ^ 0x80808080u;
+      if constexpr (L == kCols4) {
+        qf.a[0][i][2 * odd] = grp >= 4 ? d2 : d0;
+        qf.a[0][i][2 * odd + 1] = grp >= 4 ? 0u : d1;
+      } else {
+        qf.a[0][i][2 * odd] = d0;
+        qf.a[0][i][2 * odd + 1] = d1;
+        qf.a[1][i][2 * odd] = d2;
+        qf.a[1][i][2 * odd + 1] = 0u;
+      }
+    }
+#pragma unroll
+  for (int m = 0; m < kv4_q_tiles(L); ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      int s = 0;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        s = __dp4a(int(qf.a[m][i][r]), 0x01010101, s);
+        s = __dp4a(int(qf.a[m][i][2 + r]), 0x01010101, s);
+      }
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      qf.start[m][r] = -8 * s;
+    }
+  total += __shfl_xor_sync(0xffffffffu, total, 1);
+  total += __shfl_xor_sync(0xffffffffu, total, 2);
+  // Scores in log2 units, or in natural ones where rules come after.
+  const float unit = RULES ? p.rule.scale : p.rule.scale * kLog2e;
+  qf.dot = finite ? down * unit : __int_as_float(0x7fffffff);
+  qf.sum = float(total) * qf.dot;
+  qf.slope = RULES && p.rule.slopes != nullptr ? __ldg(p.rule.slopes + head) : 0.f;
+  qf.pos = valid ? kv4_query_position(p.rule, b, r, p.rows, len) : -1;
+}
+
+// ---------------------------------------------------------------------------
+// Scores of one stage: thread (grp, tig) gets those of its column for the
+// tokens 16 tig + [0, 16). N-tile j takes tokens 16 (n / 2) + 2 j + n % 2, so
+// that the thread's C fragments (n = 2 tig, 2 tig + 1) are its tokens 2 j and
+// 2 j + 1, and a quarter-warp reads two neighbouring K rows.
+template <int D, int L>
+__device__ __forceinline__ void kv4_dots(const uint8_t* codes, const uint32_t (&a)[kv4_q_tiles(L)][D / 32][4],
+                                         const int (&start)[kv4_q_tiles(L)][2], float (&sc)[16]) {
+  const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
+  constexpr int kWords = D / 32;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint8_t* row = codes + (16 * (grp >> 1) + 2 * j + (grp & 1)) * (D / 2);
+    uint32_t w[kWords];
+    if constexpr (D == 64) {
+      const uint2 x = *reinterpret_cast<const uint2*>(row + 8 * tig);
+      w[0] = x.x, w[1] = x.y;
+    } else {
+#pragma unroll
+      for (int c = 0; c < D / 128; ++c) {
+        const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * c + 16 * tig);
+        w[4 * c] = x.x, w[4 * c + 1] = x.y, w[4 * c + 2] = x.z, w[4 * c + 3] = x.w;
+      }
+    }
+    int acc[kv4_q_tiles(L)][4];
+#pragma unroll
+    for (int m = 0; m < kv4_q_tiles(L); ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][e] = start[m][e / 2];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      const uint32_t lo = w[i] & 0x0f0f0f0fu, hi = (w[i] >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+      for (int m = 0; m < kv4_q_tiles(L); ++m)
+        imma_16832(acc[m], a[m][i][0], a[m][i][1], a[m][i][2], a[m][i][3], lo, hi);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      // |digit dot| <= 128 * 8 * 256: exact in s32 with its neighbour
+      float x = float(acc[0][e] + 256 * acc[0][2 + e]);
+      if constexpr (L != kCols4) x = fmaf(float(acc[1][e]), 65536.f, x);
+      if constexpr (L == kCols4) {
+        if (grp >= 4) x *= 65536.f;
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+      }
+      sc[2 * j + e] = x;
+    }
+  }
+}
+
+// softcap * tanh(x / softcap).
+__device__ __forceinline__ float kv4_cap(float x, float cap, float inv_cap) {
+  const float y = x * inv_cap;
+  // tanh y = 1 - 2 / (e^2y + 1); near 0, where that cancels, its series.
+  const float u = fast_exp2(y * (2.0f * kLog2e));
+  const float far = 1.0f - __fdividef(2.0f, u + 1.0f);
+  const float y2 = y * y;
+  float s = fmaf(y2, 62.0f / 2835.0f, -17.0f / 315.0f);
+  s = fmaf(s, y2, 2.0f / 15.0f);
+  s = fmaf(s, y2, -1.0f / 3.0f);
+  const float near = fmaf(s * y2, y, y);
+  return cap * (y2 < 0.09f ? near : far);
+}
+
+// exp(x - y) of scores x and y: log2 units without rules, natural units with
+// them (differences are small where the result is not).
+template <bool RULES>
+__device__ __forceinline__ float kv4_exp(float x, float y) {
+  return fast_exp2(RULES ? (x - y) * kLog2e : x - y);
+}
+
+// Scores from the digit dots; invisible ones -inf. Returns the thread's
+// visible tokens as a bit mask (all ones where MASK is false).
+template <int D, bool RULES, bool MASK>
+__device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const uint8_t* params, uint32_t tb,
+                                               uint32_t len, uint32_t prefix, float dot, float sum, float slope,
+                                               int32_t pq, bool positions, float (&sc)[16]) {
+  const uint32_t tig = threadIdx.x & 3;
+  const float4* par = reinterpret_cast<const float4*>(params + 128 * tig);
+  if constexpr (!RULES) {
+    uint32_t seen = 0xffffu;
+    if (MASK) {
+      // tokens t <= pq < len
+      const int32_t n = pq + 1 - int32_t(tb + 16 * tig);
+      seen = n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 f = par[i];
+      sc[2 * i] = fmaf(sc[2 * i] * dot, f.x, fmaf(8.f, f.x, f.y) * sum);
+      sc[2 * i + 1] = fmaf(sc[2 * i + 1] * dot, f.z, fmaf(8.f, f.z, f.w) * sum);
+    }
+    if (MASK) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t)
+        if (!(seen >> t & 1u)) sc[t] = -INFINITY;
+    }
+    return seen;
+  } else {
+    uint32_t seen = 0;
+    const float cap = p.rule.softcap, inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
+    const int4* pos = reinterpret_cast<const int4*>(params + kStageTokens * 8 + 64 * tig);
+    const int32_t t0 = int32_t(tb + 16 * tig);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int32_t pk[4];
+      if (positions) {
+        const int4 x = pos[i];
+        pk[0] = x.x, pk[1] = x.y, pk[2] = x.z, pk[3] = x.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pk[e] = t0 + 4 * i + e;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = 4 * i + e;
+        const float4 f = par[2 * i + e / 2];
+        const float scale = e % 2 ? f.z : f.x, lo = e % 2 ? f.w : f.y;
+        float x = fmaf(sc[t] * dot, scale, fmaf(8.f, scale, lo) * sum);
+        if (cap > 0.f) x = kv4_cap(x, cap, inv_cap);
+        // exact below 2^24; |pq - pk| as the larger minus the smaller
+        const uint32_t away = pq >= pk[e] ? uint32_t(pq) - uint32_t(pk[e]) : uint32_t(pk[e]) - uint32_t(pq);
+        x = fmaf(-slope, float(away), x);
+        const bool on = uint32_t(t0 + t) < len && kv4_visible(pk[e], pq, p.rule.window, prefix);
+        sc[t] = on ? x : -INFINITY;
+        seen |= on ? 1u << t : 0u;
+      }
+    }
+    return seen;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention.
+
+template <int D>
+struct Kv4State {
+  float o[D / 16][4];  // dims 16 j + 4 tig + [0, 4) of the thread's column (kCols4: its digits' share)
+  float m;             // running max, the same in a column's four lanes
+  float l, lo;         // the thread's part of sum p and of sum p * (lo + 8 scale)
+};
+
+template <int D, int L, bool RULES, bool MASK>
+__device__ __forceinline__ void kv4_softmax(const uint8_t* vparams, uint32_t seen, float (&sc)[16],
+                                            Kv4State<D>& st, uint32_t (&digit)[kv4_p_tiles(L)][2][4],
+                                            float& out_scale) {
+  const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
+  float top = sc[0];
+#pragma unroll
+  for (int t = 1; t < 16; ++t) top = fmaxf(top, sc[t]);
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const float m = fmaxf(st.m, top);
+  const float sub = m == -INFINITY ? 0.f : m;
+  const float alpha = m == st.m ? 1.f : kv4_exp<RULES>(st.m, sub);
+  st.m = m;
+  if (__any_sync(0xffffffffu, alpha != 1.f)) {
+    st.l *= alpha;
+    st.lo *= alpha;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.o[j][e] *= alpha;
+  }
+  const float4* par = reinterpret_cast<const float4*>(vparams + 128 * tig);
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 f = par[i];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int t = 2 * i + e;
+      const float scale = e ? f.z : f.x, lo = e ? f.w : f.y;
+      const float pr = kv4_exp<RULES>(sc[t], sub);
+      st.l += pr;
+      float w = pr * scale;
+      float mid = fmaf(8.f, scale, lo) * pr;
+      if (MASK && !(seen >> t & 1u)) w = 0.f, mid = 0.f;  // whatever the slot holds
+      st.lo += mid;
+      sc[t] = w;
+      big = fmaxf(big, w);
+    }
+  }
+  big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+  big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+  // Power of two (a little less, so that nothing rounds up to the next one)
+  // that puts the tile's largest below 2^16 or 2^23: the fixed-point values
+  // are the low bytes of sc * up + 2^23.
+  constexpr uint32_t kTop = L == kCols8x2 ? 269 : 276;
+  constexpr float kLess = 1.0f - 1.0f / 16384.0f;
+  const uint32_t ex = max(__float_as_uint(big) >> 23, kTop - 253u);
+  const float up = kLess * __uint_as_float((kTop - ex) << 23);
+  out_scale = (1.0f / kLess) * __uint_as_float((ex - (kTop - 254u)) << 23);
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    uint32_t f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = __float_as_uint(fmaf(sc[4 * h + e], up, 8388608.0f));
+    const uint32_t x = __byte_perm(f[0], f[1], 0x5140), y = __byte_perm(f[2], f[3], 0x5140);
+    const uint32_t d0 = __byte_perm(x, y, 0x5410), d1 = __byte_perm(x, y, 0x7632);
+    // tokens 8 i .. 8 i + 3 feed a[0] and a[1], the next four a[2] and a[3]
+    uint32_t* a = digit[0][h / 2] + 2 * (h % 2);
+    if constexpr (L == kCols8x2) {
+      a[0] = d0;
+      a[1] = d1;
+    } else {
+      const uint32_t x2 = __byte_perm(f[0], f[1], 0x0062), y2 = __byte_perm(f[2], f[3], 0x0062);
+      const uint32_t d2 = __byte_perm(x2, y2, 0x5410);
+      if constexpr (L == kCols4) {
+        a[0] = grp >= 4 ? d2 : d0;
+        a[1] = grp >= 4 ? 0u : d1;
+      } else {
+        a[0] = d0;
+        a[1] = d1;
+        digit[1][h / 2][2 * (h % 2)] = d2;
+        digit[1][h / 2][2 * (h % 2) + 1] = 0u;
+      }
+    }
+  }
+  if constexpr (L == kCols4) out_scale *= grp >= 4 ? 65536.f : 1.f;
+}
+
+// O += P . V for one stage. Thread (grp, tig) reads, for the dim pair 8 j +
+// grp, the codes of its 16 tokens; low halves are the even dims' tile, high
+// halves the odd dims'.
+template <int D, int L>
+__device__ __forceinline__ void kv4_output(const uint8_t* codes, uint32_t P, uint32_t pitch,
+                                           const uint32_t (&digit)[kv4_p_tiles(L)][2][4], float out_scale,
+                                           Kv4State<D>& st) {
+  const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
+  const uint8_t* base = codes + (16 * tig / P) * pitch + (16 * tig % P) + grp * P;
+  // -8 * (sum of the row's digits): rows grp and grp + 8 of every tile.
+  int start[kv4_p_tiles(L)][2];
+#pragma unroll
+  for (int m = 0; m < kv4_p_tiles(L); ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      uint32_t s = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s = __dp4a(digit[m][i][r], 0x01010101u, s);
+        s = __dp4a(digit[m][i][2 + r], 0x01010101u, s);
+      }
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      start[m][r] = -8 * int(s);
+    }
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) {
+    const uint4 w = *reinterpret_cast<const uint4*>(base + 8 * j * P);
+    const uint32_t lo[4] = {w.x & 0x0f0f0f0fu, w.y & 0x0f0f0f0fu, w.z & 0x0f0f0f0fu, w.w & 0x0f0f0f0fu};
+    const uint32_t hi[4] = {(w.x >> 4) & 0x0f0f0f0fu, (w.y >> 4) & 0x0f0f0f0fu, (w.z >> 4) & 0x0f0f0f0fu,
+                            (w.w >> 4) & 0x0f0f0f0fu};
+    int even[kv4_p_tiles(L)][4], odd[kv4_p_tiles(L)][4];
+#pragma unroll
+    for (int m = 0; m < kv4_p_tiles(L); ++m) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) even[m][e] = odd[m][e] = start[m][e / 2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t* a = digit[m][i];
+        imma_u8_16832(even[m], a[0], a[1], a[2], a[3], lo[2 * i], lo[2 * i + 1]);
+        imma_u8_16832(odd[m], a[0], a[1], a[2], a[3], hi[2 * i], hi[2 * i + 1]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      // exact: |sum| <= 255 * 8 * 64 a digit
+      float x = float(even[0][e] + 256 * even[0][2 + e]), y = float(odd[0][e] + 256 * odd[0][2 + e]);
+      if constexpr (L == kCols8x3) {
+        x = fmaf(float(even[1][e]), 65536.f, x);
+        y = fmaf(float(odd[1][e]), 65536.f, y);
+      }
+      st.o[j][2 * e] = fmaf(x, out_scale, st.o[j][2 * e]);
+      st.o[j][2 * e + 1] = fmaf(y, out_scale, st.o[j][2 * e + 1]);
+    }
+  }
+}
+
+__device__ __forceinline__ void kv4_store_out(void* out, size_t at, int32_t type, float x) {
+  if (type == 0) static_cast<float*>(out)[at] = x;
+  else if (type == 1) static_cast<__half*>(out)[at] = __float2half_rn(x);
+  else static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(x);
+}
+
+// o / l; zero for a row that saw nothing, NaN where l is.
+__device__ __forceinline__ float kv4_normalised(float o, float l) { return l == 0.f ? 0.f : o / l; }
+__device__ __forceinline__ float kv4_lse(float m, float l, bool rules) {
+  return l == 0.f ? -INFINITY : rules ? m + logf(l) : (m + log2f(l)) * kLn2;
+}
+
+// Index of (sequence b, row r, head) of a segment's column; false if unused.
+__device__ __forceinline__ bool kv4_column(const Kv4AttendParams& p, uint32_t b, uint32_t seg, uint32_t c,
+                                           uint32_t cols, size_t& index) {
+  const uint32_t col = (seg % p.col_groups) * cols + c;
+  if (col >= p.rows * p.group) return false;
+  index = (size_t(b) * p.rows + col / p.group) * p.q_heads + (seg / p.col_groups) * p.group + col % p.group;
+  return true;
+}
+
+template <int D, int L, int KR, int VR, int MINB, bool RULES>
+__global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4AttendParams p) {
+  using S = Kv4Smem<D, KR, VR>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = lane >> 2, tig = lane & 3;
+  int* abort_flag = reinterpret_cast<int*>(smem + S::kOffAbort);
+  Kv4Feeder<D, KR, VR, RULES> feed;
+  feed.ring = smem + warp * S::kWarp;
+  feed.bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars) + warp * (KR + VR);
+  feed.policy = l2_evict_first_policy();
+  if (lane == 0) {
+    for (int i = 0; i < KR + VR; ++i) mbar_init(feed.bars + i, 1);
+    fence_barrier_init();
+  }
+  if (tid == 0) *abort_flag = 0;
+  __syncthreads();
+  grid_launch_dependents();
+  grid_dependency_wait();
+
+  const uint32_t segs = p.pool.kv_heads * p.col_groups;
+  Kv4Cursor cur;
+  const uint32_t count = kv4_locate<RULES>(p, segs, cur);
+  if (p.direct ? blockIdx.x % segs == 0 && tid == 0 && __ldg(p.seq_lens + cur.b) > p.max_tokens
+               : blockIdx.x == 0 && warp == 0) {
+    bool over = p.direct;
+    if (!p.direct)
+      for (uint32_t b = lane; b < p.batch; b += 32) over = over || __ldg(p.seq_lens + b) > p.max_tokens;
+    if (over) atomicMax(&g_kvb_status, kKv4LenClamped);
+  }
+  if (count == 0 && !p.direct) return;
+
+  // The warp's first stages.
+  feed.cur = cur;
+  feed.next = warp;
+  feed.count = count;
+  feed.segs = segs;
+  feed.k_used = feed.v_used = 0;
+  const uint32_t mine = count > warp ? (count - warp + kKv4Warps - 1) / kKv4Warps : 0;  // stages of this warp
+#pragma unroll
+  for (int i = 0; i <= KR; ++i) feed.unit[i] = feed.lookup(p);
+#pragma unroll
+  for (int i = 0; i < KR; ++i) {
+    if (uint32_t(i) < mine) feed.copy_k(p, feed.unit[i]);
+    if (i < VR && uint32_t(i) < mine) feed.copy_v(p, feed.unit[i]);
+  }
+  uint32_t done = 0;  // the warp's stages consumed
+  bool failed = false;
+
+  float* combine = reinterpret_cast<float*>(smem + S::kOffCombine);
+  float* stat = reinterpret_cast<float*>(smem + S::kOffStats);  // [warp][8] max, then sums, then lo parts
+  const uint32_t vpitch = kv4_v_pitch(p.page_tokens * (D / 2), p.page_tokens);
+  const bool positions = RULES && p.pool.pos != nullptr;
+  constexpr uint32_t kCols = kv4_cols(L);
+
+  for (uint32_t rel = 0; rel < count || p.direct;) {
+    const uint32_t end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
+    const uint32_t h = cur.seg / p.col_groups;
+    Kv4Query<D, L> qf;
+    kv4_load_query<D, L, RULES>(p, cur.b, h, cur.seg % p.col_groups, cur.len, qf);
+    const uint32_t prefix = RULES && p.rule.prefix != nullptr ? __ldg(p.rule.prefix + cur.b) : 0u;
+    // Tokens below this are visible to every row (no rules).
+    const int32_t clear = int32_t(cur.len) - int32_t(p.rows) + 1;
+    Kv4State<D> st;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.o[j][e] = 0.f;
+    st.m = -INFINITY;
+    st.l = st.lo = 0.f;
+    for (; done < mine && warp + done * kKv4Warps < end; ++done) {
+      const uint32_t j = uint32_t(int32_t(warp + done * kKv4Warps) - cur.base);
+      const uint32_t tb = (RULES && j >= cur.head ? j + cur.skip : j) * kStageTokens;
+      const uint8_t* ks = feed.ring + (done % KR) * S::kKSlot;
+      const uint8_t* vs = feed.ring + KR * S::kKSlot + (done % VR) * S::kVSlot;
+      float sc[16];
+      uint32_t digit[kv4_p_tiles(L)][2][4], seen;
+      float out_scale;
+      if (!failed)
+        failed = mbar_wait_bounded(feed.bars + done % KR, (done / KR) & 1, abort_flag, kStatusFullWaitTimeout,
+                                   int(done), p.wait_limit_ns) != kWaitOk;
+      failed = __any_sync(0xffffffffu, failed);
+      if (failed) continue;
+      kv4_dots<D, L>(ks, qf.a, qf.start, sc);
+      const bool clean = !RULES && int32_t(tb + kStageTokens) <= clear;
+      if (clean)
+        seen = kv4_scores<D, RULES, false>(p, ks + S::kCodes, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope,
+                                           qf.pos, positions, sc);
+      else
+        seen = kv4_scores<D, RULES, true>(p, ks + S::kCodes, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope,
+                                          qf.pos, positions, sc);
+      __syncwarp();  // every lane has read the K slot
+      if (done + KR < mine) feed.copy_k(p, feed.unit[KR]);
+      failed = mbar_wait_bounded(feed.bars + KR + done % VR, (done / VR) & 1, abort_flag, kStatusFullWaitTimeout,
+                                 int(done), p.wait_limit_ns) != kWaitOk;
+      failed = __any_sync(0xffffffffu, failed);
+      if (failed) continue;
+      if (clean)
+        kv4_softmax<D, L, RULES, false>(vs + S::kVCodes, seen, sc, st, digit, out_scale);
+      else
+        kv4_softmax<D, L, RULES, true>(vs + S::kVCodes, seen, sc, st, digit, out_scale);
+      kv4_output<D, L>(vs, p.page_tokens, vpitch, digit, out_scale, st);
+      __syncwarp();  // every lane has read the V slot
+      if (done + VR < mine) feed.copy_v(p, feed.unit[VR]);
+#pragma unroll
+      for (int i = 0; i < KR; ++i) feed.unit[i] = feed.unit[i + 1];
+      feed.unit[KR] = feed.lookup(p);
+    }
+
+    // The four warps' states to one: publish the maxima, scale, add.
+    st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
+    st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
+    st.lo += __shfl_xor_sync(0xffffffffu, st.lo, 1);
+    st.lo += __shfl_xor_sync(0xffffffffu, st.lo, 2);
+    if (tig == 0) {
+      stat[warp * 8 + grp] = st.m;
+      stat[32 + warp * 8 + grp] = st.l;
+      stat[64 + warp * 8 + grp] = st.lo;
+    }
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kKv4Warps; ++w) top = fmaxf(top, stat[w * 8 + grp]);
+    const float f = kv4_exp<RULES>(st.m, top == -INFINITY ? 0.f : top);
+    float* mine_o = combine + (warp * 8 + grp) * S::kPitch + 4 * tig;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+      *reinterpret_cast<float4*>(mine_o + 16 * j) =
+          make_float4(st.o[j][0] * f, st.o[j][1] * f, st.o[j][2] * f, st.o[j][3] * f);
+    __syncthreads();
+    const uint32_t segment = cur.b * segs + cur.seg;
+    const uint32_t slot = blockIdx.x + segment;
+    for (uint32_t i = tid; i < kCols * (D / 4); i += kKv4Threads) {
+      const uint32_t c = i / (D / 4), d = 4 * (i % (D / 4));
+      size_t index;
+      if (!kv4_column(p, cur.b, cur.seg, c, kCols, index)) continue;
+      float cm = -INFINITY, l = 0.f, lo = 0.f;
+#pragma unroll
+      for (int w = 0; w < kKv4Warps; ++w) cm = fmaxf(cm, stat[w * 8 + c]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kKv4Warps; ++w) {
+        const float g = kv4_exp<RULES>(stat[w * 8 + c], cm == -INFINITY ? 0.f : cm);
+        l = fmaf(stat[32 + w * 8 + c], g, l);
+        lo = fmaf(stat[64 + w * 8 + c], g, lo);
+        const float4 x = *reinterpret_cast<const float4*>(combine + (w * 8 + c) * S::kPitch + d);
+        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+        if constexpr (L == kCols4) {
+          const float4 y = *reinterpret_cast<const float4*>(combine + (w * 8 + c + 4) * S::kPitch + d);
+          o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+        }
+      }
+      o.x += lo, o.y += lo, o.z += lo, o.w += lo;
+      if (p.direct) {
+        const size_t at = index * D + d;
+        kv4_store_out(p.out, at, p.type, kv4_normalised(o.x, l));
+        kv4_store_out(p.out, at + 1, p.type, kv4_normalised(o.y, l));
+        kv4_store_out(p.out, at + 2, p.type, kv4_normalised(o.z, l));
+        kv4_store_out(p.out, at + 3, p.type, kv4_normalised(o.w, l));
+        if (d == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(cm, l, RULES);
+      } else {
+        *reinterpret_cast<float4*>(p.part + (size_t(slot) * kCols + c) * D + d) = o;
+        if (d == 0) p.part_ml[size_t(slot) * kCols + c] = make_float2(cm, l);
+      }
+    }
+    if (p.direct) break;
+    if (tid == 0) {
+      if (int32_t(rel) == cur.base) p.seg_ctas[segment].x = blockIdx.x;
+      if (int32_t(end) == cur.base + int32_t(cur.stages)) p.seg_ctas[segment].y = blockIdx.x;
+    }
+    rel = end;
+    if (rel < count) kv4_next_segment<RULES>(p, segs, cur);
+  }
+
+  if (failed) {
+    kv4_drain(feed.bars, KR, feed.k_used, p.wait_limit_ns);
+    kv4_drain(feed.bars + KR, VR, feed.v_used, p.wait_limit_ns);
+  }
+}
+
+// One CTA per (sequence, row, head): the partials of its segment's CTAs.
+constexpr int kKv4MergeWarps = 8;
+
+template <int D, bool RULES>
+__global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv4AttendParams p, uint32_t cols) {
+  __shared__ float sum[kKv4MergeWarps][D];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t index = blockIdx.x, head = index % p.q_heads, br = index / p.q_heads;
+  const uint32_t r = br % p.rows, b = br / p.rows, h = head / p.group;
+  const uint32_t col = r * p.group + head % p.group, seg = h * p.col_groups + col / cols, c = col % cols;
+  const uint32_t segment = b * p.pool.kv_heads * p.col_groups + seg;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const uint32_t stages = kv4_stage_count<RULES>(p, b);
+  uint32_t first = 0, n = 0;
+  if (stages != 0) {
+    const uint2 range = __ldcg(p.seg_ctas + segment);
+    first = range.x + segment;
+    n = range.y - range.x + 1;
+  }
+  float top = -INFINITY;
+  for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(p.part_ml + size_t(first + i) * cols + c).x);
+  top = warp_max(top);
+  const float sub = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  for (uint32_t i = lane; i < n; i += 32) {
+    const float2 ml = __ldcg(p.part_ml + size_t(first + i) * cols + c);
+    l = fmaf(ml.y, kv4_exp<RULES>(ml.x, sub), l);
+  }
+  l = warp_sum(l);
+  constexpr int kPer = D / 32;  // consecutive dims of a lane
+  float o[kPer] = {};
+#pragma unroll 4
+  for (uint32_t i = warp; i < n; i += kKv4MergeWarps) {
+    const size_t at = size_t(first + i) * cols + c;
+    const float f = kv4_exp<RULES>(__ldcg(&p.part_ml[at].x), sub);
+    const float* src = p.part + at * D + lane * kPer;
+    if constexpr (kPer == 2) {
+      const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+      o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPer / 4; ++k) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(src) + k);
+        o[4 * k] = fmaf(x.x, f, o[4 * k]), o[4 * k + 1] = fmaf(x.y, f, o[4 * k + 1]);
+        o[4 * k + 2] = fmaf(x.z, f, o[4 * k + 2]), o[4 * k + 3] = fmaf(x.w, f, o[4 * k + 3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) sum[warp][lane * kPer + k] = o[k];
+  __syncthreads();
+  for (uint32_t d = tid; d < D; d += 32 * kKv4MergeWarps) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kKv4MergeWarps; ++w) x += sum[w][d];
+    kv4_store_out(p.out, size_t(index) * D + d, p.type, kv4_normalised(x, l));
+  }
+  if (tid == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(top, l, RULES);
+}
+
+// ---------------------------------------------------------------------------
+// Accumulated weights: the scores again, against the given log-sum-exp. The
+// segments are (sequence, KV head); a stage's K codes are multiplied with
+// every column group's queries, whose A fragments the CTA keeps in shared
+// memory, so that one thread adds up each token's weight in a fixed order.
+
+template <int D, int L>
+struct alignas(16) Kv4WeighFrag {
+  uint32_t a[kv4_q_tiles(L)][D / 32][4];
+  int start[kv4_q_tiles(L)][2];
+  float dot, sum, slope, lse;
+  int32_t pos;
+};
+
+template <int D, int L, int KR, int MINB, bool RULES>
+__global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4AttendParams p,
+                                                                      uint32_t query_groups) {
+  using S = Kv4Smem<D, KR, 0>;
+  using F = Kv4WeighFrag<D, L>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = lane >> 2, tig = lane & 3;
+  int* abort_flag = reinterpret_cast<int*>(smem + S::kOffAbort);
+  F* frags = reinterpret_cast<F*>(smem + S::kOffFrags);  // [group][lane]
+  Kv4Feeder<D, KR, 0, RULES> feed;
+  feed.ring = smem + warp * S::kWarp;
+  feed.bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars) + warp * KR;
+  feed.policy = l2_evict_first_policy();
+  if (lane == 0) {
+    for (int i = 0; i < KR; ++i) mbar_init(feed.bars + i, 1);
+    fence_barrier_init();
+  }
+  if (tid == 0) *abort_flag = 0;
+  __syncthreads();
+  grid_launch_dependents();
+  grid_dependency_wait();
+
+  const uint32_t segs = p.pool.kv_heads;  // p.col_groups is 1 here
+  Kv4Cursor cur;
+  const uint32_t count = kv4_locate<RULES>(p, segs, cur);
+  if (blockIdx.x == 0 && warp == 0) {
+    bool over = false;
+    for (uint32_t b = lane; b < p.batch; b += 32) over = over || __ldg(p.seq_lens + b) > p.max_tokens;
+    if (over) atomicMax(&g_kvb_status, kKv4LenClamped);
+  }
+  if (count == 0) return;
+  feed.cur = cur;
+  feed.next = warp;
+  feed.count = count;
+  feed.segs = segs;
+  feed.k_used = feed.v_used = 0;
+  const uint32_t mine = count > warp ? (count - warp + kKv4Warps - 1) / kKv4Warps : 0;
+#pragma unroll
+  for (int i = 0; i <= KR; ++i) feed.unit[i] = feed.lookup(p);
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (uint32_t(i) < mine) feed.copy_k(p, feed.unit[i]);
+  uint32_t done = 0;
+  bool failed = false;
+  const bool positions = RULES && p.pool.pos != nullptr;
+
+  for (uint32_t rel = 0; rel < count;) {
+    const uint32_t end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
+    __syncthreads();  // the last segment's fragments are read
+    for (uint32_t g = warp; g < query_groups; g += kKv4Warps) {
+      Kv4Query<D, L> qf;
+      kv4_load_query<D, L, RULES>(p, cur.b, cur.seg, g, cur.len, qf);
+      F& out = frags[g * 32 + lane];
+#pragma unroll
+      for (int m = 0; m < kv4_q_tiles(L); ++m) {
+        out.start[m][0] = qf.start[m][0];
+        out.start[m][1] = qf.start[m][1];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+          *reinterpret_cast<uint4*>(out.a[m][i]) =
+              make_uint4(qf.a[m][i][0], qf.a[m][i][1], qf.a[m][i][2], qf.a[m][i][3]);
+      }
+      out.dot = qf.dot;
+      out.sum = qf.sum;
+      out.slope = qf.slope;
+      out.pos = qf.pos;
+      const uint32_t col = g * kv4_cols(L) + (L == kCols4 ? grp & 3 : grp);
+      const bool valid = col < p.rows * p.group && (L != kCols4 || grp < 4);
+      // infinite: a column that is not there, or a row that saw nothing
+      out.lse = INFINITY;
+      if (valid) {
+        const float lse = __ldg(p.lse_in + (size_t(cur.b) * p.rows + col / p.group) * p.q_heads +
+                                cur.seg * p.group + col % p.group);
+        if (lse != -INFINITY) out.lse = RULES ? lse : lse * kLog2e;
+      }
+    }
+    __syncthreads();
+    const uint32_t prefix = RULES && p.rule.prefix != nullptr ? __ldg(p.rule.prefix + cur.b) : 0u;
+    const int32_t clear = int32_t(cur.len) - int32_t(p.rows) + 1;
+    float* weights = p.weights + (int64_t(cur.b) * p.pool.kv_heads + cur.seg) * p.weight_stride;
+    for (; done < mine && warp + done * kKv4Warps < end; ++done) {
+      const uint32_t j = uint32_t(int32_t(warp + done * kKv4Warps) - cur.base);
+      const uint32_t tb = (RULES && j >= cur.head ? j + cur.skip : j) * kStageTokens;
+      const uint8_t* ks = feed.ring + (done % KR) * S::kKSlot;
+      // After the reduction below this lane holds tokens 16 tig + 2 grp, + 1.
+      const uint32_t t0 = tb + 16 * tig + 2 * grp;
+      const float old0 = t0 < cur.len ? weights[t0] : 0.f, old1 = t0 + 1 < cur.len ? weights[t0 + 1] : 0.f;
+      if (!failed)
+        failed = mbar_wait_bounded(feed.bars + done % KR, (done / KR) & 1, abort_flag, kStatusFullWaitTimeout,
+                                   int(done), p.wait_limit_ns) != kWaitOk;
+      failed = __any_sync(0xffffffffu, failed);
+      if (failed) continue;
+      float w[16] = {};
+      const bool clean = !RULES && int32_t(tb + kStageTokens) <= clear;
+      for (uint32_t g = 0; g < query_groups; ++g) {
+        const F& fr = frags[g * 32 + lane];
+        uint32_t a[kv4_q_tiles(L)][D / 32][4];
+        int start[kv4_q_tiles(L)][2];
+#pragma unroll
+        for (int m = 0; m < kv4_q_tiles(L); ++m) {
+          start[m][0] = fr.start[m][0];
+          start[m][1] = fr.start[m][1];
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(fr.a[m][i]);
+            a[m][i][0] = x.x, a[m][i][1] = x.y, a[m][i][2] = x.z, a[m][i][3] = x.w;
+          }
+        }
+        float sc[16];
+        kv4_dots<D, L>(ks, a, start, sc);
+        if (clean)
+          kv4_scores<D, RULES, false>(p, ks + S::kCodes, tb, cur.len, prefix, fr.dot, fr.sum, fr.slope, fr.pos,
+                                      positions, sc);
+        else
+          kv4_scores<D, RULES, true>(p, ks + S::kCodes, tb, cur.len, prefix, fr.dot, fr.sum, fr.slope, fr.pos,
+                                     positions, sc);
+        const float lse = fr.lse;
+        if (lse != INFINITY) {
+#pragma unroll
+          for (int t = 0; t < 16; ++t) w[t] += sc[t] == -INFINITY ? 0.f : kv4_exp<RULES>(sc[t], lse);
+        }
       }
       __syncwarp();
+      if (done + KR < mine) feed.copy_k(p, feed.unit[KR]);
+#pragma unroll
+      for (int i = 0; i < KR; ++i) feed.unit[i] = feed.unit[i + 1];
+      feed.unit[KR] = feed.lookup(p);
+      // Sum over the eight columns (lanes grp), halving the tokens held at
+      // each step: lane grp ends with tokens 2 grp and 2 grp + 1.
+#pragma unroll
+      for (int half = 8; half >= 2; half >>= 1) {
+        const uint32_t bit = 2 * half;  // lanes grp ^ (half / 2)
+        const bool upper = lane & bit;
+#pragma unroll
+        for (int t = 0; t < half; ++t) {
+          const float give = upper ? w[t] : w[t + half];
+          const float keep = upper ? w[t + half] : w[t];
+          w[t] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+        }
+      }
+      if (t0 < cur.len) weights[t0] = old0 + w[0];
+      if (t0 + 1 < cur.len) weights[t0 + 1] = old1 + w[1];
     }
-  if (lane == 0) p.weights[(int64_t(b) * p.pool.kv_heads + h) * p.weight_stride + t] += total;
+    rel = end;
+    if (rel < count) kv4_next_segment<RULES>(p, segs, cur);
+  }
+  if (failed) kv4_drain(feed.bars, KR, feed.k_used, p.wait_limit_ns);
 }
 
 }  // namespace kvb
