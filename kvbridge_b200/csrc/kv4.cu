@@ -6,7 +6,7 @@
 #include <mutex>
 #include <stdexcept>
 #include <string>
-#include <tuple>
+#include <utility>
 #include <type_traits>
 
 #include "kvbridge/attention_b200.h"
@@ -208,36 +208,35 @@ struct Kv4Kernel {
   uint32_t smem;
 };
 
-// K and V slots a warp and CTAs an SM. Four warps of 64-token stages a CTA;
-// dim 128: 12 warps an SM with two K slots and one V slot each (75 KB a CTA),
-// at most 168 registers.
+// Stage slots a warp and CTAs an SM. Dim 128: 12 warps an SM with two 9.1 KB
+// slots each, at most 168 registers.
 template <int D>
 struct Kv4Shape;
 template <>
 struct Kv4Shape<64> {
-  static constexpr int kK = 2, kV = 2, kCtas = 4, kWeighK = 4, kWeighCtas = 4;
+  static constexpr int kSlots = 2, kCtas = 4, kWeighSlots = 4, kWeighCtas = 4;
 };
 template <>
 struct Kv4Shape<128> {
-  static constexpr int kK = 2, kV = 1, kCtas = 3, kWeighK = 3, kWeighCtas = 3;
+  static constexpr int kSlots = 2, kCtas = 3, kWeighSlots = 3, kWeighCtas = 3;
 };
 template <>
 struct Kv4Shape<256> {
-  static constexpr int kK = 1, kV = 1, kCtas = 2, kWeighK = 2, kWeighCtas = 2;
+  static constexpr int kSlots = 1, kCtas = 2, kWeighSlots = 2, kWeighCtas = 2;
 };
 
 template <int D, int L, bool RULES>
 Kv4Kernel attend_kernel() {
   using T = Kv4Shape<D>;
-  return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, L, T::kK, T::kV, T::kCtas, RULES>),
-          kvb::Kv4Smem<D, T::kK, T::kV>::kBytes};
+  return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, L, T::kSlots, T::kCtas, RULES>),
+          kvb::Kv4Smem<D, T::kSlots, true>::kBytes};
 }
 
 template <int D, int L, bool RULES>
-Kv4Kernel weigh_kernel(uint32_t groups) {
+Kv4Kernel weigh_kernel() {
   using T = Kv4Shape<D>;
-  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, L, T::kWeighK, T::kWeighCtas, RULES>),
-          kvb::Kv4Smem<D, T::kWeighK, 0>::kBytes + groups * 32 * uint32_t(sizeof(kvb::Kv4WeighFrag<D, L>))};
+  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, L, T::kWeighSlots, T::kWeighCtas, RULES>),
+          kvb::Kv4Smem<D, T::kWeighSlots, false>::kBytes};
 }
 
 bool has_rules(const Kv4Pool& pool, const Kv4Query& q) {
@@ -263,10 +262,10 @@ Kv4Kernel attend_kernel(uint32_t dim, int layout) {
 
 // Weights are fp32 whatever the queries: three digits.
 template <bool RULES>
-Kv4Kernel weigh_kernel(uint32_t dim, bool four, uint32_t groups) {
+Kv4Kernel weigh_kernel(uint32_t dim, bool four) {
   return by_dim(dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    return four ? weigh_kernel<D, kvb::kCols4, RULES>(groups) : weigh_kernel<D, kvb::kCols8x3, RULES>(groups);
+    return four ? weigh_kernel<D, kvb::kCols4, RULES>() : weigh_kernel<D, kvb::kCols8x3, RULES>();
   });
 }
 
@@ -274,19 +273,15 @@ Kv4Kernel weigh_kernel(uint32_t dim, bool four, uint32_t groups) {
 // device also raises the kernel's shared-memory limit.
 uint32_t resident_ctas(const Kv4Kernel& k) {
   static std::mutex mu;
-  static std::map<std::tuple<int, const void*, uint32_t>, uint32_t> cache;
+  static std::map<std::pair<int, const void*>, uint32_t> cache;
   int dev = 0;
   cuda_ok(cudaGetDevice(&dev), "cudaGetDevice");
   std::lock_guard<std::mutex> lock(mu);
-  const auto key = std::make_tuple(dev, k.fn, k.smem);
+  const auto key = std::make_pair(dev, k.fn);
   const auto it = cache.find(key);
   if (it != cache.end()) return it->second;
-  // The limit may only grow: the weights kernels' shared memory varies with the query.
-  cudaFuncAttributes attr{};
-  cuda_ok(cudaFuncGetAttributes(&attr, k.fn), "kv4 kernel attributes");
-  if (uint32_t(attr.maxDynamicSharedSizeBytes) < k.smem)
-    cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(k.smem)),
-            "kv4 kernel shared-memory opt-in");
+  cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(k.smem)),
+          "kv4 kernel shared-memory opt-in");
   cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributePreferredSharedMemoryCarveout,
                                int(cudaSharedmemCarveoutMaxShared)),
           "kv4 kernel carveout");
@@ -298,7 +293,7 @@ uint32_t resident_ctas(const Kv4Kernel& k) {
 }
 
 // CTAs of a call whose segments have at most max_tokens tokens: a full wave,
-// or fewer so that each has a stage for every warp.
+// or fewer where there are fewer stages than warps.
 uint32_t split_ctas(const Kv4Kernel& k, uint64_t segments, uint32_t max_tokens) {
   const uint64_t stages = segments * ((uint64_t(max_tokens) + kvb::kStageTokens - 1) / kvb::kStageTokens);
   const uint64_t most = (stages + kvb::kKv4Warps - 1) / kvb::kKv4Warps;
@@ -308,13 +303,13 @@ uint32_t split_ctas(const Kv4Kernel& k, uint64_t segments, uint32_t max_tokens) 
 struct AttendPlan {
   Kv4Kernel kernel;
   int layout;
-  bool rules, direct;
-  uint32_t col_groups, segments, ctas;
-  size_t ml_offset, ctas_offset, bytes;  // of the workspace
+  bool rules, direct, many;
+  uint32_t col_groups, segments, ctas, workers;
+  size_t ml_offset, warps_offset, bytes;  // of the workspace
 };
 
-// Short sequences: one CTA per segment writes the result, nothing is merged.
-constexpr uint32_t kDirectTokens = 512;
+// Short sequences: one warp per segment writes the result, nothing is merged.
+constexpr uint32_t kDirectTokens = 128;
 
 AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
   AttendPlan a{};
@@ -325,16 +320,20 @@ AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
   a.col_groups = (all + cols - 1) / cols;
   a.segments = q.batch * pool.kv_heads * a.col_groups;
   a.direct = q.max_tokens <= kDirectTokens;
-  a.ctas = a.direct ? a.segments : split_ctas(a.kernel, a.segments, q.max_tokens);
   if (a.direct) {
     resident_ctas(a.kernel);
+    a.workers = a.segments;
+    a.ctas = (a.segments + kvb::kKv4Warps - 1) / kvb::kKv4Warps;
     a.bytes = 16;
     return a;
   }
-  const size_t slots = size_t(a.ctas) + a.segments;
+  a.ctas = split_ctas(a.kernel, a.segments, q.max_tokens);
+  a.workers = a.ctas * kvb::kKv4Warps;
+  a.many = a.workers > 8 * a.segments;
+  const size_t slots = size_t(a.workers) + a.segments;
   a.ml_offset = slots * cols * pool.dim * sizeof(float);
-  a.ctas_offset = a.ml_offset + slots * cols * sizeof(float2);
-  a.bytes = a.ctas_offset + size_t(a.segments) * sizeof(uint2);
+  a.warps_offset = a.ml_offset + slots * cols * sizeof(float2);
+  a.bytes = a.warps_offset + size_t(a.segments) * sizeof(uint2);
   return a;
 }
 
@@ -355,11 +354,11 @@ void launch_attention_kv4(const Kv4Pool& pool, const Kv4Query& q, void* workspac
   if (workspace_bytes < a.bytes)
     throw std::invalid_argument("workspace smaller than attention_kv4_workspace_bytes(pool, query)");
   prm.col_groups = a.col_groups;
-  prm.ctas = a.ctas;
+  prm.workers = a.workers;
   prm.direct = a.direct;
   prm.part = static_cast<float*>(workspace);
   prm.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + a.ml_offset);
-  prm.seg_ctas = reinterpret_cast<uint2*>(static_cast<uint8_t*>(workspace) + a.ctas_offset);
+  prm.seg_warps = reinterpret_cast<uint2*>(static_cast<uint8_t*>(workspace) + a.warps_offset);
   prm.out = out;
   prm.lse = lse;
   void* args[] = {&prm};
@@ -370,11 +369,14 @@ void launch_attention_kv4(const Kv4Pool& pool, const Kv4Query& q, void* workspac
   void* merge_args[] = {&prm, &cols};
   const void* merge = by_dim(pool.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    return a.rules ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, true>)
-                   : reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, false>);
+    return a.rules ? a.many ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, true, true>)
+                            : reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, true, false>)
+           : a.many ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, false, true>)
+                    : reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, false, false>);
   });
-  launch_kernel_pdl(merge, dim3(q.batch * q.rows * q.q_heads), dim3(32 * kvb::kKv4MergeWarps), 0, stream, merge_args,
-                    "kv4 merge launch");
+  const uint32_t rows = q.batch * q.rows * q.q_heads;
+  launch_kernel_pdl(merge, dim3(a.many ? rows : (rows + kvb::kKv4MergeWarps - 1) / kvb::kKv4MergeWarps),
+                    dim3(32 * kvb::kKv4MergeWarps), 0, stream, merge_args, "kv4 merge launch");
 }
 
 void accumulate_weights_kv4(const Kv4Pool& pool, const Kv4Query& q, const float* lse, float* weights,
@@ -388,16 +390,18 @@ void accumulate_weights_kv4(const Kv4Pool& pool, const Kv4Query& q, const float*
   if (prm.max_tokens == 0) return;
   const uint32_t all = q.rows * prm.group;
   const bool four = all <= 4;
-  uint32_t groups = four ? 1 : (all + 7) / 8;
-  const Kv4Kernel k = has_rules(pool, q) ? weigh_kernel<true>(pool.dim, four, groups)
-                                         : weigh_kernel<false>(pool.dim, four, groups);
+  const uint32_t groups = four ? 1 : (all + 7) / 8;
+  const Kv4Kernel k = has_rules(pool, q) ? weigh_kernel<true>(pool.dim, four) : weigh_kernel<false>(pool.dim, four);
   prm.col_groups = 1;
-  prm.ctas = split_ctas(k, uint64_t(q.batch) * pool.kv_heads, prm.max_tokens);
+  const uint32_t ctas = split_ctas(k, uint64_t(q.batch) * pool.kv_heads, prm.max_tokens);
+  prm.workers = ctas * kvb::kKv4Warps;
   prm.lse_in = lse;
   prm.weights = weights;
   prm.weight_stride = weight_stride;
-  void* args[] = {&prm, &groups};
-  launch_kernel_pdl(k.fn, dim3(prm.ctas), dim3(kvb::kKv4Threads), k.smem, stream, args, "kv4 weights launch");
+  for (uint32_t group = 0; group < groups; ++group) {
+    void* args[] = {&prm, &group};
+    launch_kernel_pdl(k.fn, dim3(ctas), dim3(kvb::kKv4Threads), k.smem, stream, args, "kv4 weights launch");
+  }
 }
 
 // ---------------------------------------------------------------------------

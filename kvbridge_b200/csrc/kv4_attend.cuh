@@ -4,16 +4,16 @@
 //
 // Schedule. The attended tokens of a sequence are runs of 64-token stages;
 // one segment per (sequence, KV head, group of query columns). The segments'
-// stages, concatenated, are cut into equal contiguous ranges, one per CTA
-// (kvb_schedule.h); a CTA's part of a segment is a piece. Stage g of a CTA
-// belongs to warp g % 4. A windowed call leaves the stages between the
-// prefix and the window out of the list, so they are never read.
+// stages, concatenated, are cut into equal contiguous ranges, one per warp
+// (kvb_schedule.h); a warp's part of a segment is a piece and gives one
+// partial result, or the output itself where the piece is the whole segment.
+// A windowed call leaves the stages between the prefix and the window out of
+// the list, so they are never read.
 //
-// A warp feeds itself: lane 0 arms the mbarrier of the next free slot and a
-// few lanes start bulk copies of the stage's pages (codes, params), K when
-// the previous K has been multiplied, V when the previous V has been. No
-// producer warp and no empty barriers: the warp that reads a slot is the one
-// that refills it.
+// Warps share nothing: each has its own ring of stage slots and its own
+// mbarriers, and refills a slot (a few lanes start one bulk copy each: K and V
+// codes, K and V params of a page) as soon as it has read it. No producer
+// warp, no empty barriers and no CTA barriers.
 //
 // Arithmetic (int8 tensor cores, exact s32 sums; codes 0..15 are int8
 // operands after a mask or a shift and a mask, two values a byte):
@@ -59,16 +59,16 @@ struct Kv4AttendParams {
   uint32_t batch, rows, q_heads, group, table_stride, max_tokens;
   uint32_t page_tokens, log2_page;
   uint32_t col_groups;  // groups of query columns (rows * group) of a KV head
-  uint32_t ctas;
+  uint32_t workers;     // warps of the grid
   int32_t type;   // of q and out: 0 f32, 1 f16, 2 bf16
   bool vector_q;  // 16-byte aligned query rows
-  bool direct;    // one CTA per segment, which writes the outputs itself
+  bool direct;    // one warp per segment, nothing to merge
   unsigned long long wait_limit_ns;
-  // Partials of piece (CTA c, segment i) in slot c + i: per column D sums and
-  // {max, sum}; the first and last CTA of every segment.
+  // Partials of piece (warp w, segment i) in slot w + i: per column D sums and
+  // {max, sum}; the first and last warp of every segment.
   float* part;
   float2* part_ml;
-  uint2* seg_ctas;
+  uint2* seg_warps;
   void* out;
   float* lse;
   // accumulate_weights_kv4
@@ -80,7 +80,7 @@ struct Kv4AttendParams {
 // ---------------------------------------------------------------------------
 // The stage list.
 
-// A segment being walked; positions are relative to the CTA's first stage.
+// A segment being walked; positions are relative to the warp's first stage.
 struct Kv4Cursor {
   uint32_t b, seg;
   uint32_t len;     // tokens of sequence b
@@ -133,14 +133,15 @@ __device__ __forceinline__ void kv4_next_segment(const Kv4AttendParams& p, uint3
   }
 }
 
-// Warp-cooperative: the CTA's range and the cursor at its first stage.
-// Returns the number of stages of the range.
+// Warp-cooperative: the range of worker `w` and the cursor at its first
+// stage. Returns the number of stages of the range.
 template <bool RULES>
-__device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t segs, Kv4Cursor& c) {
+__device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t w, uint32_t segs, Kv4Cursor& c) {
   const uint32_t lane = threadIdx.x & 31;
   if (p.direct) {
-    c.b = blockIdx.x / segs;
-    c.seg = blockIdx.x % segs;
+    if (w >= p.workers) return 0;
+    c.b = w / segs;
+    c.seg = w % segs;
     c.base = 0;
     kv4_load_sequence<RULES>(p, c);
     return c.stages;
@@ -150,11 +151,10 @@ __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t segs, Kv4Curso
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   total *= segs;
-  // No more CTAs than have a stage for every warp; the others leave.
-  const uint32_t ctas = uint32_t(min(uint64_t(p.ctas), (total + kKv4Warps - 1) / kKv4Warps));
-  if (blockIdx.x >= ctas) return 0;
-  const uint64_t x0 = cta_stage_begin(blockIdx.x, total, ctas);
-  const uint64_t x1 = cta_stage_begin(blockIdx.x + 1, total, ctas);
+  const uint32_t workers = uint32_t(min(uint64_t(p.workers), total));
+  if (w >= workers) return 0;
+  const uint64_t x0 = cta_stage_begin(w, total, workers);
+  const uint64_t x1 = cta_stage_begin(w + 1, total, workers);
   uint64_t before = 0;
   for (uint32_t from = 0; from < p.batch; from += 32) {
     const uint64_t n = from + lane < p.batch ? kv4_stage_count<RULES>(p, from + lane) : 0u;
@@ -180,109 +180,99 @@ __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t segs, Kv4Curso
 }
 
 // ---------------------------------------------------------------------------
-// Shared memory of one warp.
+// One warp's ring.
 
-template <int D, int KR, int VR>
+// A slot: K codes, V codes (pages of 16 and 32 tokens 32 and 64 bytes further
+// apart, so that a quarter-warp's reads of several pages hit different
+// banks), K params, V params. V false: K alone.
+template <int D, int SLOTS, bool V>
 struct Kv4Smem {
-  // K slot: codes, params, positions. V slot: codes (pages of 16 and 32
-  // tokens 32 and 64 bytes further apart, so that a quarter-warp's reads of
-  // several pages hit different banks), params.
   static constexpr uint32_t kCodes = kStageTokens * D / 2;
   static constexpr uint32_t kParams = kStageTokens * 8;
-  static constexpr uint32_t kKSlot = kCodes + kParams + kStageTokens * 4;
-  static constexpr uint32_t kVCodes = VR > 0 ? kCodes + 128 : 0;
-  static constexpr uint32_t kVSlot = VR > 0 ? kVCodes + kParams : 0;
-  static constexpr uint32_t kWarp = KR * kKSlot + VR * kVSlot;
-  static constexpr uint32_t kBars = 8 * (KR + VR);
-  // Combine buffer of the four warps: 8 columns (or column shares) of D.
-  static constexpr uint32_t kPitch = D + 4;
-  static constexpr uint32_t kCombine = VR > 0 ? kKv4Warps * 8 * kPitch * 4 : 0;
-  static constexpr uint32_t kStats = VR > 0 ? kKv4Warps * 8 * 12 : 0;  // max, sum, lo part
-  static constexpr uint32_t kOffCombine = kKv4Warps * kWarp;
-  static constexpr uint32_t kOffStats = kOffCombine + kCombine;
-  static constexpr uint32_t kOffBars = kOffStats + kStats;
-  static constexpr uint32_t kOffAbort = kOffBars + kKv4Warps * kBars;
-  static constexpr uint32_t kOffFrags = kOffAbort + 16;  // accumulate_weights_kv4
-  static constexpr uint32_t kBytes = kOffFrags;
+  static constexpr uint32_t kOffV = kCodes;
+  static constexpr uint32_t kOffKp = kOffV + (V ? kCodes + 128 : 0);
+  static constexpr uint32_t kOffVp = kOffKp + kParams;
+  static constexpr uint32_t kSlot = kOffVp + (V ? kParams : 0);
+  static constexpr uint32_t kOffBars = kKv4Warps * SLOTS * kSlot;
+  static constexpr uint32_t kOffAbort = kOffBars + kKv4Warps * SLOTS * 8;
+  static constexpr uint32_t kBytes = kOffAbort + 16;
 };
 
 __device__ __forceinline__ uint32_t kv4_v_pitch(uint32_t page_bytes, uint32_t P) {
   return P == 64 ? page_bytes : page_bytes + 2 * P;
 }
 
-// ---------------------------------------------------------------------------
-// Feeding: the pages of the warp's stages, looked up one stage ahead of the
-// K copies, kept until the V copies.
-
-template <int D, int KR, int VR, bool RULES>
+template <int D, int SLOTS, bool V, bool RULES>
 struct Kv4Feeder {
-  uint8_t* ring;    // the warp's slots: K slots, then V slots
-  uint64_t* bars;   // KR full barriers for K, then VR for V
-  Kv4Cursor cur;    // the segment of the next stage to look up
-  uint32_t next;    // that stage, relative to the CTA's first
-  uint32_t count;   // stages of the CTA
-  uint32_t segs;
+  uint8_t* ring;
+  uint64_t* bars;
   uint64_t policy;
-  uint32_t k_used, v_used;  // slots filled so far
-  uint32_t unit[KR + 1];  // (page, KV head) of this lane's page: stages i .. i + KR
+  Kv4Cursor cur;   // the segment of the next stage to look up
+  uint32_t next;   // that stage, relative to the warp's first
+  uint32_t count;  // stages of the warp
+  uint32_t segs;
+  uint32_t used;   // slots filled so far
+  // This lane's copy of a stage: array lane / 4 (K codes, K params, V codes,
+  // V params) of page lane % 4.
+  const uint8_t* base;
+  uint32_t bytes, dst;
+  bool copies;
+  // The page looked up last: in flight until it is used.
+  uint32_t phys, head;
 
-  // The pool unit of page lane % 4 of stage `next`; advances by one stage of the warp.
-  __device__ uint32_t lookup(const Kv4AttendParams& p) {
-    uint32_t found = kNoUnit;
+  __device__ void init(const Kv4AttendParams& p, uint8_t* smem, uint32_t warp) {
+    using S = Kv4Smem<D, SLOTS, V>;
+    const uint32_t lane = threadIdx.x & 31, part = lane >> 2, q = lane & 3;
+    const uint32_t P = p.page_tokens, codes = P * (D / 2);
+    ring = smem + warp * SLOTS * S::kSlot;
+    bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars) + warp * SLOTS;
+    policy = l2_evict_first_policy();
+    copies = q < (kStageTokens >> p.log2_page) && part < (V ? 4u : 2u);
+    base = part == 0   ? p.pool.k
+           : part == 1 ? reinterpret_cast<const uint8_t*>(p.pool.kp)
+           : part == 2 ? p.pool.v
+                       : reinterpret_cast<const uint8_t*>(p.pool.vp);
+    bytes = part & 1 ? P * 8 : codes;
+    dst = part == 0 ? q * codes : part == 1 ? S::kOffKp + q * P * 8
+        : part == 2 ? S::kOffV + q * kv4_v_pitch(codes, P) : S::kOffVp + q * P * 8;
+    used = 0;
+    if (lane == 0) {
+      for (int i = 0; i < SLOTS; ++i) mbar_init(bars + i, 1);
+      fence_barrier_init();
+    }
+    __syncwarp();
+  }
+
+  // Starts the lookup of the page of stage `next`; kNoUnit where there is none.
+  __device__ __forceinline__ void lookup(const Kv4AttendParams& p) {
+    phys = kNoUnit;
     if (next < count) {
       while (int32_t(next) >= cur.base + int32_t(cur.stages)) kv4_next_segment<RULES>(p, segs, cur);
       const uint32_t j = uint32_t(int32_t(next) - cur.base);
       const uint32_t stage = RULES && j >= cur.head ? j + cur.skip : j;
-      const uint32_t q = threadIdx.x & 3, pps = kStageTokens >> p.log2_page;
-      const uint32_t page = stage * pps + q;
-      if (q < pps && (page << p.log2_page) < cur.len) {
-        const uint32_t phys = __ldg(p.table + size_t(cur.b) * p.table_stride + page);
-        const uint32_t h = cur.seg / p.col_groups;
-        if (phys < p.pool.pages)
-          found = phys * p.pool.kv_heads + h;
-        else
-          atomicMax(&g_kvb_status, kKv4BadPage);
-      }
+      const uint32_t page = (stage << (6 - p.log2_page)) + (threadIdx.x & 3);
+      head = p.col_groups == 1 ? cur.seg : cur.seg / p.col_groups;
+      if (copies && (page << p.log2_page) < cur.len) phys = __ldg(p.table + size_t(cur.b) * p.table_stride + page);
+      ++next;
     }
-    next += kKv4Warps;
-    return found;
   }
 
-  // The pages u of the warp's next stage into the next K or V slot. All lanes.
-  __device__ void copy_k(const Kv4AttendParams& p, uint32_t u) {
-    const uint32_t lane = threadIdx.x & 31, q = lane & 3, part = lane >> 2, use = k_used++;
-    const uint32_t P = p.page_tokens, bytes = P * (D / 2);
-    uint8_t* slot = ring + (use % KR) * Kv4Smem<D, KR, VR>::kKSlot;
-    uint64_t* bar = bars + use % KR;
-    const bool pos = RULES && p.pool.pos != nullptr;
-    const uint32_t ok = __popc(__ballot_sync(0xffffffffu, u != kNoUnit && part == 0));
-    if (lane == 0) mbar_arrive_expect_tx(bar, ok * (bytes + P * (pos ? 12u : 8u)));
+  // Starts the copies of the stage looked up last into the next slot.
+  __device__ __forceinline__ void copy(const Kv4AttendParams& p) {
+    using S = Kv4Smem<D, SLOTS, V>;
+    const uint32_t slot = used % SLOTS;
+    ++used;
+    uint64_t* bar = bars + slot;
+    const bool ok = phys < p.pool.pages;  // lanes without a copy hold kNoUnit
+    if (!ok && phys != kNoUnit) atomicMax(&g_kvb_status, kKv4BadPage);
+    // Lanes 0 to 3 stand for the stage's pages.
+    const uint32_t pages = __popc(__ballot_sync(0xffffffffu, ok) & 0xfu);
+    const uint32_t page_bytes = p.page_tokens * (V ? D + 16 : D / 2 + 8);
+    if ((threadIdx.x & 31) == 0) mbar_arrive_expect_tx(bar, pages * page_bytes);
     __syncwarp();
-    if (u == kNoUnit) return;
-    constexpr uint32_t kCodes = Kv4Smem<D, KR, VR>::kCodes;
-    if (part == 0)
-      bulk_copy_g2s(slot + q * bytes, p.pool.k + size_t(u) * bytes, bytes, bar, policy);
-    else if (part == 1)
-      bulk_copy_g2s(slot + kCodes + q * P * 8, p.pool.kp + size_t(u) * P, P * 8, bar, policy);
-    else if (part == 2 && pos)
-      bulk_copy_g2s(slot + kCodes + Kv4Smem<D, KR, VR>::kParams + q * P * 4, p.pool.pos + size_t(u) * P,
-                    P * 4, bar, policy);
-  }
-
-  __device__ void copy_v(const Kv4AttendParams& p, uint32_t u) {
-    const uint32_t lane = threadIdx.x & 31, q = lane & 3, part = lane >> 2, use = v_used++;
-    const uint32_t P = p.page_tokens, bytes = P * (D / 2);
-    uint8_t* slot = ring + KR * Kv4Smem<D, KR, VR>::kKSlot + (use % VR) * Kv4Smem<D, KR, VR>::kVSlot;
-    uint64_t* bar = bars + KR + use % VR;
-    const uint32_t ok = __popc(__ballot_sync(0xffffffffu, u != kNoUnit && part == 0));
-    if (lane == 0) mbar_arrive_expect_tx(bar, ok * (bytes + P * 8));
-    __syncwarp();
-    if (u == kNoUnit) return;
-    if (part == 0)
-      bulk_copy_g2s(slot + q * kv4_v_pitch(bytes, P), p.pool.v + size_t(u) * bytes, bytes, bar, policy);
-    else if (part == 1)
-      bulk_copy_g2s(slot + Kv4Smem<D, KR, VR>::kVCodes + q * P * 8, p.pool.vp + size_t(u) * P, P * 8,
-                    bar, policy);
+    if (ok)
+      bulk_copy_g2s(ring + slot * S::kSlot + dst, base + (size_t(phys) * p.pool.kv_heads + head) * bytes, bytes, bar,
+                    policy);
   }
 };
 
@@ -508,11 +498,12 @@ __device__ __forceinline__ float kv4_exp(float x, float y) {
 }
 
 // Scores from the digit dots; invisible ones -inf. Returns the thread's
-// visible tokens as a bit mask (all ones where MASK is false).
+// visible tokens as a bit mask (all ones where MASK is false). pos: the
+// positions of the thread's 16 tokens, or null for their indices.
 template <int D, bool RULES, bool MASK>
 __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const uint8_t* params, uint32_t tb,
                                                uint32_t len, uint32_t prefix, float dot, float sum, float slope,
-                                               int32_t pq, bool positions, float (&sc)[16]) {
+                                               int32_t pq, const int32_t* pos, float (&sc)[16]) {
   const uint32_t tig = threadIdx.x & 3;
   const float4* par = reinterpret_cast<const float4*>(params + 128 * tig);
   if constexpr (!RULES) {
@@ -537,13 +528,12 @@ __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const u
   } else {
     uint32_t seen = 0;
     const float cap = p.rule.softcap, inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
-    const int4* pos = reinterpret_cast<const int4*>(params + kStageTokens * 8 + 64 * tig);
     const int32_t t0 = int32_t(tb + 16 * tig);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       int32_t pk[4];
-      if (positions) {
-        const int4 x = pos[i];
+      if (pos != nullptr) {
+        const int4 x = __ldg(reinterpret_cast<const int4*>(pos) + i);
         pk[0] = x.x, pk[1] = x.y, pk[2] = x.z, pk[3] = x.w;
       } else {
 #pragma unroll
@@ -667,6 +657,7 @@ __device__ __forceinline__ void kv4_output(const uint8_t* codes, uint32_t P, uin
                                            Kv4State<D>& st) {
   const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
   const uint8_t* base = codes + (16 * tig / P) * pitch + (16 * tig % P) + grp * P;
+  const float odd_scale = out_scale * 0.0625f;
   // -8 * (sum of the row's digits): rows grp and grp + 8 of every tile.
   int start[kv4_p_tiles(L)][2];
 #pragma unroll
@@ -687,13 +678,13 @@ __device__ __forceinline__ void kv4_output(const uint8_t* codes, uint32_t P, uin
   for (int j = 0; j < D / 16; ++j) {
     const uint4 w = *reinterpret_cast<const uint4*>(base + 8 * j * P);
     const uint32_t lo[4] = {w.x & 0x0f0f0f0fu, w.y & 0x0f0f0f0fu, w.z & 0x0f0f0f0fu, w.w & 0x0f0f0f0fu};
-    const uint32_t hi[4] = {(w.x >> 4) & 0x0f0f0f0fu, (w.y >> 4) & 0x0f0f0f0fu, (w.z >> 4) & 0x0f0f0f0fu,
-                            (w.w >> 4) & 0x0f0f0f0fu};
+    // 16 times the odd dims' codes
+    const uint32_t hi[4] = {w.x & 0xf0f0f0f0u, w.y & 0xf0f0f0f0u, w.z & 0xf0f0f0f0u, w.w & 0xf0f0f0f0u};
     int even[kv4_p_tiles(L)][4], odd[kv4_p_tiles(L)][4];
 #pragma unroll
     for (int m = 0; m < kv4_p_tiles(L); ++m) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) even[m][e] = odd[m][e] = start[m][e / 2];
+      for (int e = 0; e < 4; ++e) even[m][e] = start[m][e / 2], odd[m][e] = 16 * start[m][e / 2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint32_t* a = digit[m][i];
@@ -703,14 +694,14 @@ __device__ __forceinline__ void kv4_output(const uint8_t* codes, uint32_t P, uin
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      // exact: |sum| <= 255 * 8 * 64 a digit
+      // exact: |sum| <= 255 * 128 * 64 a digit, times 257 below 2^30
       float x = float(even[0][e] + 256 * even[0][2 + e]), y = float(odd[0][e] + 256 * odd[0][2 + e]);
       if constexpr (L == kCols8x3) {
         x = fmaf(float(even[1][e]), 65536.f, x);
         y = fmaf(float(odd[1][e]), 65536.f, y);
       }
       st.o[j][2 * e] = fmaf(x, out_scale, st.o[j][2 * e]);
-      st.o[j][2 * e + 1] = fmaf(y, out_scale, st.o[j][2 * e + 1]);
+      st.o[j][2 * e + 1] = fmaf(y, odd_scale, st.o[j][2 * e + 1]);
     }
   }
 }
@@ -727,6 +718,32 @@ __device__ __forceinline__ float kv4_lse(float m, float l, bool rules) {
   return l == 0.f ? -INFINITY : rules ? m + logf(l) : (m + log2f(l)) * kLn2;
 }
 
+// Four neighbouring outputs; their alignment is only that of the buffer.
+__device__ __forceinline__ void kv4_store_out4(void* out, size_t at, int32_t type, const float (&o)[4], float l) {
+  float x[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = kv4_normalised(o[e], l);
+  if (type != 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+    uint32_t w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (type == 1) {
+        const __half2 y = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&y);
+      } else {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&y);
+      }
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(w[0], w[1]);
+  } else if (type == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) kv4_store_out(out, at + e, type, x[e]);
+  }
+}
+
 // Index of (sequence b, row r, head) of a segment's column; false if unused.
 __device__ __forceinline__ bool kv4_column(const Kv4AttendParams& p, uint32_t b, uint32_t seg, uint32_t c,
                                            uint32_t cols, size_t& index) {
@@ -736,62 +753,60 @@ __device__ __forceinline__ bool kv4_column(const Kv4AttendParams& p, uint32_t b,
   return true;
 }
 
-template <int D, int L, int KR, int VR, int MINB, bool RULES>
+// The positions of this thread's 16 tokens of the stage at token tb, or null
+// where positions are indices (or the page is not there).
+__device__ __forceinline__ const int32_t* kv4_positions(const Kv4AttendParams& p, uint32_t b, uint32_t h,
+                                                        uint32_t len, uint32_t tb) {
+  if (p.pool.pos == nullptr) return nullptr;
+  const uint32_t t = tb + 16 * (threadIdx.x & 3);
+  const uint32_t page = t < len ? __ldg(p.table + size_t(b) * p.table_stride + (t >> p.log2_page)) : kNoUnit;
+  if (page >= p.pool.pages) return nullptr;
+  return p.pool.pos + (size_t(page) * p.pool.kv_heads + h) * p.page_tokens + (t & (p.page_tokens - 1));
+}
+
+__device__ __forceinline__ void kv4_report_lengths(const Kv4AttendParams& p) {
+  if (blockIdx.x != 0) return;
+  for (uint32_t b = threadIdx.x; b < p.batch; b += kKv4Threads)
+    if (__ldg(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
+}
+
+template <int D, int L, int SLOTS, int MINB, bool RULES>
 __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4AttendParams p) {
-  using S = Kv4Smem<D, KR, VR>;
+  using S = Kv4Smem<D, SLOTS, true>;
   extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = lane >> 2, tig = lane & 3;
-  int* abort_flag = reinterpret_cast<int*>(smem + S::kOffAbort);
-  Kv4Feeder<D, KR, VR, RULES> feed;
-  feed.ring = smem + warp * S::kWarp;
-  feed.bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars) + warp * (KR + VR);
-  feed.policy = l2_evict_first_policy();
-  if (lane == 0) {
-    for (int i = 0; i < KR + VR; ++i) mbar_init(feed.bars + i, 1);
-    fence_barrier_init();
-  }
-  if (tid == 0) *abort_flag = 0;
-  __syncthreads();
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = lane >> 2, tig = lane & 3;
+  int* abort_flag = reinterpret_cast<int*>(smem + S::kOffAbort) + warp;  // of this warp's waits
+  if (lane == 0) *abort_flag = 0;
+  Kv4Feeder<D, SLOTS, true, RULES> feed;
+  feed.init(p, smem, warp);
   grid_launch_dependents();
   grid_dependency_wait();
 
+  const uint32_t worker = blockIdx.x * kKv4Warps + warp;
   const uint32_t segs = p.pool.kv_heads * p.col_groups;
   Kv4Cursor cur;
-  const uint32_t count = kv4_locate<RULES>(p, segs, cur);
-  if (p.direct ? blockIdx.x % segs == 0 && tid == 0 && __ldg(p.seq_lens + cur.b) > p.max_tokens
-               : blockIdx.x == 0 && warp == 0) {
-    bool over = p.direct;
-    if (!p.direct)
-      for (uint32_t b = lane; b < p.batch; b += 32) over = over || __ldg(p.seq_lens + b) > p.max_tokens;
-    if (over) atomicMax(&g_kvb_status, kKv4LenClamped);
-  }
-  if (count == 0 && !p.direct) return;
+  const uint32_t count = kv4_locate<RULES>(p, worker, segs, cur);
+  kv4_report_lengths(p);
+  if (count == 0 && (!p.direct || worker >= p.workers)) return;
 
-  // The warp's first stages.
   feed.cur = cur;
-  feed.next = warp;
+  feed.next = 0;
   feed.count = count;
   feed.segs = segs;
-  feed.k_used = feed.v_used = 0;
-  const uint32_t mine = count > warp ? (count - warp + kKv4Warps - 1) / kKv4Warps : 0;  // stages of this warp
+  feed.lookup(p);
 #pragma unroll
-  for (int i = 0; i <= KR; ++i) feed.unit[i] = feed.lookup(p);
-#pragma unroll
-  for (int i = 0; i < KR; ++i) {
-    if (uint32_t(i) < mine) feed.copy_k(p, feed.unit[i]);
-    if (i < VR && uint32_t(i) < mine) feed.copy_v(p, feed.unit[i]);
-  }
-  uint32_t done = 0;  // the warp's stages consumed
+  for (int i = 0; i < SLOTS; ++i)
+    if (uint32_t(i) < count) {
+      feed.copy(p);
+      feed.lookup(p);
+    }
+  uint32_t done = 0;
   bool failed = false;
-
-  float* combine = reinterpret_cast<float*>(smem + S::kOffCombine);
-  float* stat = reinterpret_cast<float*>(smem + S::kOffStats);  // [warp][8] max, then sums, then lo parts
   const uint32_t vpitch = kv4_v_pitch(p.page_tokens * (D / 2), p.page_tokens);
-  const bool positions = RULES && p.pool.pos != nullptr;
   constexpr uint32_t kCols = kv4_cols(L);
 
-  for (uint32_t rel = 0; rel < count || p.direct;) {
-    const uint32_t end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
+  do {  // pieces
+    const uint32_t first = done, end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
     const uint32_t h = cur.seg / p.col_groups;
     Kv4Query<D, L> qf;
     kv4_load_query<D, L, RULES>(p, cur.b, h, cur.seg % p.col_groups, cur.len, qf);
@@ -805,133 +820,101 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
       for (int e = 0; e < 4; ++e) st.o[j][e] = 0.f;
     st.m = -INFINITY;
     st.l = st.lo = 0.f;
-    for (; done < mine && warp + done * kKv4Warps < end; ++done) {
-      const uint32_t j = uint32_t(int32_t(warp + done * kKv4Warps) - cur.base);
+    for (; done < end; ++done) {
+      const uint32_t j = uint32_t(int32_t(done) - cur.base);
       const uint32_t tb = (RULES && j >= cur.head ? j + cur.skip : j) * kStageTokens;
-      const uint8_t* ks = feed.ring + (done % KR) * S::kKSlot;
-      const uint8_t* vs = feed.ring + KR * S::kKSlot + (done % VR) * S::kVSlot;
+      const uint8_t* slot = feed.ring + (done % SLOTS) * S::kSlot;
+      const int32_t* pos = RULES ? kv4_positions(p, cur.b, h, cur.len, tb) : nullptr;
+      const int got = mbar_wait_bounded(feed.bars + done % SLOTS, (done / SLOTS) & 1, abort_flag,
+                                        kStatusFullWaitTimeout, int(done), p.wait_limit_ns);
+      if (__any_sync(0xffffffffu, got != kWaitOk)) {
+        failed = true;
+        break;
+      }
       float sc[16];
       uint32_t digit[kv4_p_tiles(L)][2][4], seen;
       float out_scale;
-      if (!failed)
-        failed = mbar_wait_bounded(feed.bars + done % KR, (done / KR) & 1, abort_flag, kStatusFullWaitTimeout,
-                                   int(done), p.wait_limit_ns) != kWaitOk;
-      failed = __any_sync(0xffffffffu, failed);
-      if (failed) continue;
-      kv4_dots<D, L>(ks, qf.a, qf.start, sc);
-      const bool clean = !RULES && int32_t(tb + kStageTokens) <= clear;
-      if (clean)
-        seen = kv4_scores<D, RULES, false>(p, ks + S::kCodes, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope,
-                                           qf.pos, positions, sc);
-      else
-        seen = kv4_scores<D, RULES, true>(p, ks + S::kCodes, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope,
-                                          qf.pos, positions, sc);
-      __syncwarp();  // every lane has read the K slot
-      if (done + KR < mine) feed.copy_k(p, feed.unit[KR]);
-      failed = mbar_wait_bounded(feed.bars + KR + done % VR, (done / VR) & 1, abort_flag, kStatusFullWaitTimeout,
-                                 int(done), p.wait_limit_ns) != kWaitOk;
-      failed = __any_sync(0xffffffffu, failed);
-      if (failed) continue;
-      if (clean)
-        kv4_softmax<D, L, RULES, false>(vs + S::kVCodes, seen, sc, st, digit, out_scale);
-      else
-        kv4_softmax<D, L, RULES, true>(vs + S::kVCodes, seen, sc, st, digit, out_scale);
-      kv4_output<D, L>(vs, p.page_tokens, vpitch, digit, out_scale, st);
-      __syncwarp();  // every lane has read the V slot
-      if (done + VR < mine) feed.copy_v(p, feed.unit[VR]);
-#pragma unroll
-      for (int i = 0; i < KR; ++i) feed.unit[i] = feed.unit[i + 1];
-      feed.unit[KR] = feed.lookup(p);
+      kv4_dots<D, L>(slot, qf.a, qf.start, sc);
+      if (!RULES && int32_t(tb + kStageTokens) <= clear) {
+        seen = kv4_scores<D, RULES, false>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope,
+                                           qf.pos, pos, sc);
+        kv4_softmax<D, L, RULES, false>(slot + S::kOffVp, seen, sc, st, digit, out_scale);
+      } else {
+        seen = kv4_scores<D, RULES, true>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope,
+                                          qf.pos, pos, sc);
+        kv4_softmax<D, L, RULES, true>(slot + S::kOffVp, seen, sc, st, digit, out_scale);
+      }
+      kv4_output<D, L>(slot + S::kOffV, p.page_tokens, vpitch, digit, out_scale, st);
+      __syncwarp();  // every lane has read the slot
+      if (done + SLOTS < count) {
+        feed.copy(p);
+        feed.lookup(p);
+      }
     }
+    if (failed) break;
 
-    // The four warps' states to one: publish the maxima, scale, add.
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
     st.lo += __shfl_xor_sync(0xffffffffu, st.lo, 1);
     st.lo += __shfl_xor_sync(0xffffffffu, st.lo, 2);
-    if (tig == 0) {
-      stat[warp * 8 + grp] = st.m;
-      stat[32 + warp * 8 + grp] = st.l;
-      stat[64 + warp * 8 + grp] = st.lo;
-    }
-    __syncthreads();
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kKv4Warps; ++w) top = fmaxf(top, stat[w * 8 + grp]);
-    const float f = kv4_exp<RULES>(st.m, top == -INFINITY ? 0.f : top);
-    float* mine_o = combine + (warp * 8 + grp) * S::kPitch + 4 * tig;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
-      *reinterpret_cast<float4*>(mine_o + 16 * j) =
-          make_float4(st.o[j][0] * f, st.o[j][1] * f, st.o[j][2] * f, st.o[j][3] * f);
-    __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (L == kCols4) st.o[j][e] += __shfl_xor_sync(0xffffffffu, st.o[j][e], 16);
+        st.o[j][e] += st.lo;
+      }
+    // The whole segment: the output; else a partial.
+    const bool whole = int32_t(first) == cur.base && end - first == cur.stages;
     const uint32_t segment = cur.b * segs + cur.seg;
-    const uint32_t slot = blockIdx.x + segment;
-    for (uint32_t i = tid; i < kCols * (D / 4); i += kKv4Threads) {
-      const uint32_t c = i / (D / 4), d = 4 * (i % (D / 4));
-      size_t index;
-      if (!kv4_column(p, cur.b, cur.seg, c, kCols, index)) continue;
-      float cm = -INFINITY, l = 0.f, lo = 0.f;
+    size_t index;
+    if (grp < kCols && kv4_column(p, cur.b, cur.seg, grp, kCols, index)) {
+      if (whole) {
 #pragma unroll
-      for (int w = 0; w < kKv4Warps; ++w) cm = fmaxf(cm, stat[w * 8 + c]);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kKv4Warps; ++w) {
-        const float g = kv4_exp<RULES>(stat[w * 8 + c], cm == -INFINITY ? 0.f : cm);
-        l = fmaf(stat[32 + w * 8 + c], g, l);
-        lo = fmaf(stat[64 + w * 8 + c], g, lo);
-        const float4 x = *reinterpret_cast<const float4*>(combine + (w * 8 + c) * S::kPitch + d);
-        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
-        if constexpr (L == kCols4) {
-          const float4 y = *reinterpret_cast<const float4*>(combine + (w * 8 + c + 4) * S::kPitch + d);
-          o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
-        }
-      }
-      o.x += lo, o.y += lo, o.z += lo, o.w += lo;
-      if (p.direct) {
-        const size_t at = index * D + d;
-        kv4_store_out(p.out, at, p.type, kv4_normalised(o.x, l));
-        kv4_store_out(p.out, at + 1, p.type, kv4_normalised(o.y, l));
-        kv4_store_out(p.out, at + 2, p.type, kv4_normalised(o.z, l));
-        kv4_store_out(p.out, at + 3, p.type, kv4_normalised(o.w, l));
-        if (d == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(cm, l, RULES);
+        for (int j = 0; j < D / 16; ++j) kv4_store_out4(p.out, index * D + 16 * j + 4 * tig, p.type, st.o[j], st.l);
+        if (tig == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(st.m, st.l, RULES);
       } else {
-        *reinterpret_cast<float4*>(p.part + (size_t(slot) * kCols + c) * D + d) = o;
-        if (d == 0) p.part_ml[size_t(slot) * kCols + c] = make_float2(cm, l);
+        const size_t at = size_t(worker + segment) * kCols + grp;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+          *reinterpret_cast<float4*>(p.part + at * D + 16 * j + 4 * tig) =
+              make_float4(st.o[j][0], st.o[j][1], st.o[j][2], st.o[j][3]);
+        if (tig == 0) p.part_ml[at] = make_float2(st.m, st.l);
       }
     }
-    if (p.direct) break;
-    if (tid == 0) {
-      if (int32_t(rel) == cur.base) p.seg_ctas[segment].x = blockIdx.x;
-      if (int32_t(end) == cur.base + int32_t(cur.stages)) p.seg_ctas[segment].y = blockIdx.x;
+    if (lane == 0 && !p.direct) {
+      if (int32_t(first) == cur.base) p.seg_warps[segment].x = worker;
+      if (int32_t(end) == cur.base + int32_t(cur.stages)) p.seg_warps[segment].y = worker;
     }
-    rel = end;
-    if (rel < count) kv4_next_segment<RULES>(p, segs, cur);
-  }
+    if (done < count) kv4_next_segment<RULES>(p, segs, cur);
+  } while (done < count);
 
-  if (failed) {
-    kv4_drain(feed.bars, KR, feed.k_used, p.wait_limit_ns);
-    kv4_drain(feed.bars + KR, VR, feed.v_used, p.wait_limit_ns);
-  }
+  // A wait that gave up leaves copies in flight.
+  if (failed) kv4_drain(feed.bars, SLOTS, feed.used, p.wait_limit_ns);
 }
 
-// One CTA per (sequence, row, head): the partials of its segment's CTAs.
-constexpr int kKv4MergeWarps = 8;
+// The partials of one output row (sequence, row, head). Many partials a row:
+// the CTA's 16 warps share a row; few: a warp each.
+constexpr int kKv4MergeWarps = 16;
 
-template <int D, bool RULES>
+template <int D, bool RULES, bool MANY>
 __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv4AttendParams p, uint32_t cols) {
-  __shared__ float sum[kKv4MergeWarps][D];
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t index = blockIdx.x, head = index % p.q_heads, br = index / p.q_heads;
+  constexpr int kShare = MANY ? kKv4MergeWarps : 1;  // warps of a row
+  __shared__ float sum[MANY ? kKv4MergeWarps : 1][MANY ? D : 1];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = MANY ? tid >> 5 : 0;
+  const uint32_t index = MANY ? blockIdx.x : blockIdx.x * kKv4MergeWarps + (tid >> 5);
+  grid_launch_dependents();
+  if (index >= p.batch * p.rows * p.q_heads) return;  // not where warps meet
+  const uint32_t head = index % p.q_heads, br = index / p.q_heads;
   const uint32_t r = br % p.rows, b = br / p.rows, h = head / p.group;
   const uint32_t col = r * p.group + head % p.group, seg = h * p.col_groups + col / cols, c = col % cols;
   const uint32_t segment = b * p.pool.kv_heads * p.col_groups + seg;
-  grid_launch_dependents();
   grid_dependency_wait();
   const uint32_t stages = kv4_stage_count<RULES>(p, b);
   uint32_t first = 0, n = 0;
   if (stages != 0) {
-    const uint2 range = __ldcg(p.seg_ctas + segment);
+    const uint2 range = __ldcg(p.seg_warps + segment);
+    if (range.x == range.y) return;  // written by its warp
     first = range.x + segment;
     n = range.y - range.x + 1;
   }
@@ -947,8 +930,8 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv
   l = warp_sum(l);
   constexpr int kPer = D / 32;  // consecutive dims of a lane
   float o[kPer] = {};
-#pragma unroll 4
-  for (uint32_t i = warp; i < n; i += kKv4MergeWarps) {
+#pragma unroll 8
+  for (uint32_t i = warp; i < n; i += kShare) {
     const size_t at = size_t(first + i) * cols + c;
     const float f = kv4_exp<RULES>(__ldcg(&p.part_ml[at].x), sub);
     const float* src = p.part + at * D + lane * kPer;
@@ -964,159 +947,107 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv
       }
     }
   }
+  if constexpr (MANY) {
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) sum[warp][lane * kPer + k] = o[k];
-  __syncthreads();
-  for (uint32_t d = tid; d < D; d += 32 * kKv4MergeWarps) {
-    float x = 0.f;
+    for (int k = 0; k < kPer; ++k) sum[warp][lane * kPer + k] = o[k];
+    __syncthreads();
+    for (uint32_t d = tid; d < D; d += 32 * kKv4MergeWarps) {
+      float x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kKv4MergeWarps; ++w) x += sum[w][d];
-    kv4_store_out(p.out, size_t(index) * D + d, p.type, kv4_normalised(x, l));
+      for (int w = 0; w < kKv4MergeWarps; ++w) x += sum[w][d];
+      kv4_store_out(p.out, size_t(index) * D + d, p.type, kv4_normalised(x, l));
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      kv4_store_out(p.out, size_t(index) * D + lane * kPer + k, p.type, kv4_normalised(o[k], l));
   }
-  if (tid == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(top, l, RULES);
+  if (warp == 0 && lane == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(top, l, RULES);
 }
 
 // ---------------------------------------------------------------------------
-// Accumulated weights: the scores again, against the given log-sum-exp. The
-// segments are (sequence, KV head); a stage's K codes are multiplied with
-// every column group's queries, whose A fragments the CTA keeps in shared
-// memory, so that one thread adds up each token's weight in a fixed order.
+// Accumulated weights: the scores again, against the given log-sum-exp, for
+// one group of query columns a launch. The segments are (sequence, KV head);
+// one thread adds up a token's weight in a fixed order, so there are no
+// atomics, and the groups' launches follow one another.
 
-template <int D, int L>
-struct alignas(16) Kv4WeighFrag {
-  uint32_t a[kv4_q_tiles(L)][D / 32][4];
-  int start[kv4_q_tiles(L)][2];
-  float dot, sum, slope, lse;
-  int32_t pos;
-};
-
-template <int D, int L, int KR, int MINB, bool RULES>
-__global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4AttendParams p,
-                                                                      uint32_t query_groups) {
-  using S = Kv4Smem<D, KR, 0>;
-  using F = Kv4WeighFrag<D, L>;
+template <int D, int L, int SLOTS, int MINB, bool RULES>
+__global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4AttendParams p, uint32_t group) {
+  using S = Kv4Smem<D, SLOTS, false>;
   extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = lane >> 2, tig = lane & 3;
-  int* abort_flag = reinterpret_cast<int*>(smem + S::kOffAbort);
-  F* frags = reinterpret_cast<F*>(smem + S::kOffFrags);  // [group][lane]
-  Kv4Feeder<D, KR, 0, RULES> feed;
-  feed.ring = smem + warp * S::kWarp;
-  feed.bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars) + warp * KR;
-  feed.policy = l2_evict_first_policy();
-  if (lane == 0) {
-    for (int i = 0; i < KR; ++i) mbar_init(feed.bars + i, 1);
-    fence_barrier_init();
-  }
-  if (tid == 0) *abort_flag = 0;
-  __syncthreads();
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = lane >> 2, tig = lane & 3;
+  int* abort_flag = reinterpret_cast<int*>(smem + S::kOffAbort) + warp;
+  if (lane == 0) *abort_flag = 0;
+  Kv4Feeder<D, SLOTS, false, RULES> feed;
+  feed.init(p, smem, warp);
   grid_launch_dependents();
   grid_dependency_wait();
 
   const uint32_t segs = p.pool.kv_heads;  // p.col_groups is 1 here
   Kv4Cursor cur;
-  const uint32_t count = kv4_locate<RULES>(p, segs, cur);
-  if (blockIdx.x == 0 && warp == 0) {
-    bool over = false;
-    for (uint32_t b = lane; b < p.batch; b += 32) over = over || __ldg(p.seq_lens + b) > p.max_tokens;
-    if (over) atomicMax(&g_kvb_status, kKv4LenClamped);
-  }
+  const uint32_t count = kv4_locate<RULES>(p, blockIdx.x * kKv4Warps + warp, segs, cur);
+  kv4_report_lengths(p);
   if (count == 0) return;
   feed.cur = cur;
-  feed.next = warp;
+  feed.next = 0;
   feed.count = count;
   feed.segs = segs;
-  feed.k_used = feed.v_used = 0;
-  const uint32_t mine = count > warp ? (count - warp + kKv4Warps - 1) / kKv4Warps : 0;
+  feed.lookup(p);
 #pragma unroll
-  for (int i = 0; i <= KR; ++i) feed.unit[i] = feed.lookup(p);
-#pragma unroll
-  for (int i = 0; i < KR; ++i)
-    if (uint32_t(i) < mine) feed.copy_k(p, feed.unit[i]);
+  for (int i = 0; i < SLOTS; ++i)
+    if (uint32_t(i) < count) {
+      feed.copy(p);
+      feed.lookup(p);
+    }
   uint32_t done = 0;
   bool failed = false;
-  const bool positions = RULES && p.pool.pos != nullptr;
 
-  for (uint32_t rel = 0; rel < count;) {
+  while (done < count && !failed) {
     const uint32_t end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
-    __syncthreads();  // the last segment's fragments are read
-    for (uint32_t g = warp; g < query_groups; g += kKv4Warps) {
-      Kv4Query<D, L> qf;
-      kv4_load_query<D, L, RULES>(p, cur.b, cur.seg, g, cur.len, qf);
-      F& out = frags[g * 32 + lane];
-#pragma unroll
-      for (int m = 0; m < kv4_q_tiles(L); ++m) {
-        out.start[m][0] = qf.start[m][0];
-        out.start[m][1] = qf.start[m][1];
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-          *reinterpret_cast<uint4*>(out.a[m][i]) =
-              make_uint4(qf.a[m][i][0], qf.a[m][i][1], qf.a[m][i][2], qf.a[m][i][3]);
-      }
-      out.dot = qf.dot;
-      out.sum = qf.sum;
-      out.slope = qf.slope;
-      out.pos = qf.pos;
-      const uint32_t col = g * kv4_cols(L) + (L == kCols4 ? grp & 3 : grp);
-      const bool valid = col < p.rows * p.group && (L != kCols4 || grp < 4);
-      // infinite: a column that is not there, or a row that saw nothing
-      out.lse = INFINITY;
-      if (valid) {
-        const float lse = __ldg(p.lse_in + (size_t(cur.b) * p.rows + col / p.group) * p.q_heads +
-                                cur.seg * p.group + col % p.group);
-        if (lse != -INFINITY) out.lse = RULES ? lse : lse * kLog2e;
-      }
+    Kv4Query<D, L> qf;
+    kv4_load_query<D, L, RULES>(p, cur.b, cur.seg, group, cur.len, qf);
+    // Infinite: a column that is not there (or is lane - 16's), or a row that saw nothing.
+    float lse = INFINITY;
+    const uint32_t col = group * kv4_cols(L) + grp;
+    if (col < p.rows * p.group && grp < kv4_cols(L)) {
+      const float x = __ldg(p.lse_in + (size_t(cur.b) * p.rows + col / p.group) * p.q_heads + cur.seg * p.group +
+                            col % p.group);
+      if (x != -INFINITY) lse = RULES ? x : x * kLog2e;
     }
-    __syncthreads();
     const uint32_t prefix = RULES && p.rule.prefix != nullptr ? __ldg(p.rule.prefix + cur.b) : 0u;
     const int32_t clear = int32_t(cur.len) - int32_t(p.rows) + 1;
     float* weights = p.weights + (int64_t(cur.b) * p.pool.kv_heads + cur.seg) * p.weight_stride;
-    for (; done < mine && warp + done * kKv4Warps < end; ++done) {
-      const uint32_t j = uint32_t(int32_t(warp + done * kKv4Warps) - cur.base);
+    for (; done < end; ++done) {
+      const uint32_t j = uint32_t(int32_t(done) - cur.base);
       const uint32_t tb = (RULES && j >= cur.head ? j + cur.skip : j) * kStageTokens;
-      const uint8_t* ks = feed.ring + (done % KR) * S::kKSlot;
+      const uint8_t* slot = feed.ring + (done % SLOTS) * S::kSlot;
+      const int32_t* pos = RULES ? kv4_positions(p, cur.b, cur.seg, cur.len, tb) : nullptr;
       // After the reduction below this lane holds tokens 16 tig + 2 grp, + 1.
       const uint32_t t0 = tb + 16 * tig + 2 * grp;
       const float old0 = t0 < cur.len ? weights[t0] : 0.f, old1 = t0 + 1 < cur.len ? weights[t0 + 1] : 0.f;
-      if (!failed)
-        failed = mbar_wait_bounded(feed.bars + done % KR, (done / KR) & 1, abort_flag, kStatusFullWaitTimeout,
-                                   int(done), p.wait_limit_ns) != kWaitOk;
-      failed = __any_sync(0xffffffffu, failed);
-      if (failed) continue;
-      float w[16] = {};
-      const bool clean = !RULES && int32_t(tb + kStageTokens) <= clear;
-      for (uint32_t g = 0; g < query_groups; ++g) {
-        const F& fr = frags[g * 32 + lane];
-        uint32_t a[kv4_q_tiles(L)][D / 32][4];
-        int start[kv4_q_tiles(L)][2];
-#pragma unroll
-        for (int m = 0; m < kv4_q_tiles(L); ++m) {
-          start[m][0] = fr.start[m][0];
-          start[m][1] = fr.start[m][1];
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(fr.a[m][i]);
-            a[m][i][0] = x.x, a[m][i][1] = x.y, a[m][i][2] = x.z, a[m][i][3] = x.w;
-          }
-        }
-        float sc[16];
-        kv4_dots<D, L>(ks, a, start, sc);
-        if (clean)
-          kv4_scores<D, RULES, false>(p, ks + S::kCodes, tb, cur.len, prefix, fr.dot, fr.sum, fr.slope, fr.pos,
-                                      positions, sc);
-        else
-          kv4_scores<D, RULES, true>(p, ks + S::kCodes, tb, cur.len, prefix, fr.dot, fr.sum, fr.slope, fr.pos,
-                                     positions, sc);
-        const float lse = fr.lse;
-        if (lse != INFINITY) {
-#pragma unroll
-          for (int t = 0; t < 16; ++t) w[t] += sc[t] == -INFINITY ? 0.f : kv4_exp<RULES>(sc[t], lse);
-        }
+      const int got = mbar_wait_bounded(feed.bars + done % SLOTS, (done / SLOTS) & 1, abort_flag,
+                                        kStatusFullWaitTimeout, int(done), p.wait_limit_ns);
+      if (__any_sync(0xffffffffu, got != kWaitOk)) {
+        failed = true;
+        break;
       }
-      __syncwarp();
-      if (done + KR < mine) feed.copy_k(p, feed.unit[KR]);
+      float w[16];
+      kv4_dots<D, L>(slot, qf.a, qf.start, w);
+      uint32_t seen;
+      if (!RULES && int32_t(tb + kStageTokens) <= clear)
+        seen = kv4_scores<D, RULES, false>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope, qf.pos,
+                                           pos, w);
+      else
+        seen = kv4_scores<D, RULES, true>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope, qf.pos,
+                                          pos, w);
+      if (lse == INFINITY) seen = 0;
 #pragma unroll
-      for (int i = 0; i < KR; ++i) feed.unit[i] = feed.unit[i + 1];
-      feed.unit[KR] = feed.lookup(p);
+      for (int t = 0; t < 16; ++t) w[t] = seen >> t & 1u ? kv4_exp<RULES>(w[t], lse) : 0.f;
+      __syncwarp();  // every lane has read the slot
+      if (done + SLOTS < count) {
+        feed.copy(p);
+        feed.lookup(p);
+      }
       // Sum over the eight columns (lanes grp), halving the tokens held at
       // each step: lane grp ends with tokens 2 grp and 2 grp + 1.
 #pragma unroll
@@ -1133,10 +1064,9 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
       if (t0 < cur.len) weights[t0] = old0 + w[0];
       if (t0 + 1 < cur.len) weights[t0 + 1] = old1 + w[1];
     }
-    rel = end;
-    if (rel < count) kv4_next_segment<RULES>(p, segs, cur);
+    if (done < count) kv4_next_segment<RULES>(p, segs, cur);
   }
-  if (failed) kv4_drain(feed.bars, KR, feed.k_used, p.wait_limit_ns);
+  if (failed) kv4_drain(feed.bars, SLOTS, feed.used, p.wait_limit_ns);
 }
 
 }  // namespace kvb
