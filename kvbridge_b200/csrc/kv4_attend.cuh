@@ -146,18 +146,25 @@ __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t w, uint32_t se
     kv4_load_sequence<RULES>(p, c);
     return c.stages;
   }
+  // Up to 32 sequences: each lane keeps its count, read once.
+  const bool one_pass = p.batch <= 32;
+  uint32_t own = 0;
   uint64_t total = 0;
-  for (uint32_t b = lane; b < p.batch; b += 32) total += kv4_stage_count<RULES>(p, b);
+  for (uint32_t b = lane; b < p.batch; b += 32) total += own = kv4_stage_count<RULES>(p, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   total *= segs;
+  // Equal ranges, the first ones a stage longer. (A 64-bit division is a
+  // few hundred instructions on the path to the first copy.)
   const uint32_t workers = uint32_t(min(uint64_t(p.workers), total));
   if (w >= workers) return 0;
-  const uint64_t x0 = cta_stage_begin(w, total, workers);
-  const uint64_t x1 = cta_stage_begin(w + 1, total, workers);
+  const uint64_t each = total >> 32 ? total / workers : uint32_t(total) / workers;
+  const uint32_t more = uint32_t(total - each * workers);
+  const uint64_t x0 = w * each + min(w, more);
+  const uint32_t count = uint32_t(each) + (w < more ? 1u : 0u);
   uint64_t before = 0;
   for (uint32_t from = 0; from < p.batch; from += 32) {
-    const uint64_t n = from + lane < p.batch ? kv4_stage_count<RULES>(p, from + lane) : 0u;
+    const uint32_t n = one_pass ? own : from + lane < p.batch ? kv4_stage_count<RULES>(p, from + lane) : 0u;
     uint64_t upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -174,9 +181,10 @@ __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t w, uint32_t se
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
   kv4_load_sequence<RULES>(p, c);
-  c.seg = uint32_t((x0 - before) / c.stages);
-  c.base = -int32_t(x0 - before - uint64_t(c.seg) * c.stages);
-  return uint32_t(x1 - x0);
+  const uint64_t into = x0 - before;
+  c.seg = into >> 32 ? uint32_t(into / c.stages) : uint32_t(into) / c.stages;
+  c.base = -int32_t(into - uint64_t(c.seg) * c.stages);
+  return count;
 }
 
 // ---------------------------------------------------------------------------
@@ -893,61 +901,77 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
   if (failed) kv4_drain(feed.bars, SLOTS, feed.used, p.wait_limit_ns);
 }
 
-// The partials of one output row (sequence, row, head). Many partials a row:
-// the CTA's 16 warps share a row; few: a warp each.
+// The partials of one output row (sequence, row, head). Bound by latency: a
+// row's loads are a chain of the segment's warps, then the maxima and sums of
+// all partials at once, then their values. Many partials a row: a CTA's 16
+// warps share a row, a thread per partial for the weights; few: a warp a row,
+// a lane per partial.
 constexpr int kKv4MergeWarps = 16;
+
+template <int D>
+__device__ __forceinline__ void kv4_add_partial(const float* src, float f, float (&o)[D / 32]) {
+  const uint32_t lane = threadIdx.x & 31;
+  if constexpr (D == 64) {
+    const float2 x = __ldcg(reinterpret_cast<const float2*>(src) + lane);
+    o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < D / 128; ++k) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(src) + lane * (D / 128) + k);
+      o[4 * k] = fmaf(x.x, f, o[4 * k]), o[4 * k + 1] = fmaf(x.y, f, o[4 * k + 1]);
+      o[4 * k + 2] = fmaf(x.z, f, o[4 * k + 2]), o[4 * k + 3] = fmaf(x.w, f, o[4 * k + 3]);
+    }
+  }
+}
 
 template <int D, bool RULES, bool MANY>
 __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv4AttendParams p, uint32_t cols) {
-  constexpr int kShare = MANY ? kKv4MergeWarps : 1;  // warps of a row
   __shared__ float sum[MANY ? kKv4MergeWarps : 1][MANY ? D : 1];
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = MANY ? tid >> 5 : 0;
-  const uint32_t index = MANY ? blockIdx.x : blockIdx.x * kKv4MergeWarps + (tid >> 5);
+  __shared__ float weight[MANY ? 32 * kKv4MergeWarps : 1], part_max[kKv4MergeWarps], part_sum[kKv4MergeWarps];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t index = MANY ? blockIdx.x : blockIdx.x * kKv4MergeWarps + warp;
   grid_launch_dependents();
-  if (index >= p.batch * p.rows * p.q_heads) return;  // not where warps meet
+  if (index >= p.batch * p.rows * p.q_heads) return;  // (few partials: warps do not meet)
   const uint32_t head = index % p.q_heads, br = index / p.q_heads;
   const uint32_t r = br % p.rows, b = br / p.rows, h = head / p.group;
   const uint32_t col = r * p.group + head % p.group, seg = h * p.col_groups + col / cols, c = col % cols;
   const uint32_t segment = b * p.pool.kv_heads * p.col_groups + seg;
   grid_dependency_wait();
-  const uint32_t stages = kv4_stage_count<RULES>(p, b);
-  uint32_t first = 0, n = 0;
-  if (stages != 0) {
-    const uint2 range = __ldcg(p.seg_warps + segment);
-    if (range.x == range.y) return;  // written by its warp
-    first = range.x + segment;
-    n = range.y - range.x + 1;
-  }
-  float top = -INFINITY;
-  for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(p.part_ml + size_t(first + i) * cols + c).x);
-  top = warp_max(top);
-  const float sub = top == -INFINITY ? 0.f : top;
-  float l = 0.f;
-  for (uint32_t i = lane; i < n; i += 32) {
-    const float2 ml = __ldcg(p.part_ml + size_t(first + i) * cols + c);
-    l = fmaf(ml.y, kv4_exp<RULES>(ml.x, sub), l);
-  }
-  l = warp_sum(l);
+  const uint2 range = __ldcg(p.seg_warps + segment);  // of a segment with stages
+  const bool any = kv4_stage_count<RULES>(p, b) != 0;
+  if (any && range.x == range.y) return;  // written by its warp
+  const uint32_t n = any ? range.y - range.x + 1 : 0u;
+  const size_t first = size_t(range.x + segment) * cols + c;
   constexpr int kPer = D / 32;  // consecutive dims of a lane
-  float o[kPer] = {};
-#pragma unroll 8
-  for (uint32_t i = warp; i < n; i += kShare) {
-    const size_t at = size_t(first + i) * cols + c;
-    const float f = kv4_exp<RULES>(__ldcg(&p.part_ml[at].x), sub);
-    const float* src = p.part + at * D + lane * kPer;
-    if constexpr (kPer == 2) {
-      const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
-      o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kPer / 4; ++k) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(src) + k);
-        o[4 * k] = fmaf(x.x, f, o[4 * k]), o[4 * k + 1] = fmaf(x.y, f, o[4 * k + 1]);
-        o[4 * k + 2] = fmaf(x.z, f, o[4 * k + 2]), o[4 * k + 3] = fmaf(x.w, f, o[4 * k + 3]);
-      }
-    }
-  }
+  float o[kPer] = {}, top = -INFINITY, l = 0.f;
   if constexpr (MANY) {
+    for (uint32_t from = 0; from < n; from += 32 * kKv4MergeWarps) {
+      const uint32_t here = min(n - from, uint32_t(32 * kKv4MergeWarps));
+      const float2 ml = tid < here ? __ldcg(p.part_ml + first + size_t(from + tid) * cols) : make_float2(-INFINITY, 0.f);
+      float m = warp_max(ml.x);
+      if (lane == 0) part_max[warp] = m;
+      __syncthreads();
+      m = top;
+#pragma unroll
+      for (int w = 0; w < kKv4MergeWarps; ++w) m = fmaxf(m, part_max[w]);
+      const float sub = m == -INFINITY ? 0.f : m;
+      const float f = kv4_exp<RULES>(ml.x, sub);
+      weight[tid] = f;
+      const float s = warp_sum(ml.y * f);
+      if (lane == 0) part_sum[warp] = s;
+      const float alpha = kv4_exp<RULES>(top, sub);
+      l *= alpha;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) o[k] *= alpha;
+      top = m;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kKv4MergeWarps; ++w) l += part_sum[w];
+#pragma unroll 8
+      for (uint32_t i = warp; i < here; i += kKv4MergeWarps)
+        kv4_add_partial<D>(p.part + (first + size_t(from + i) * cols) * D, weight[i], o);
+      __syncthreads();
+    }
 #pragma unroll
     for (int k = 0; k < kPer; ++k) sum[warp][lane * kPer + k] = o[k];
     __syncthreads();
@@ -957,12 +981,29 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv
       for (int w = 0; w < kKv4MergeWarps; ++w) x += sum[w][d];
       kv4_store_out(p.out, size_t(index) * D + d, p.type, kv4_normalised(x, l));
     }
+    if (tid != 0) return;
   } else {
+    for (uint32_t from = 0; from < n; from += 32) {
+      const uint32_t here = min(n - from, 32u);
+      const float2 ml = lane < here ? __ldcg(p.part_ml + first + size_t(from + lane) * cols) : make_float2(-INFINITY, 0.f);
+      const float m = fmaxf(top, warp_max(ml.x)), sub = m == -INFINITY ? 0.f : m;
+      const float f = kv4_exp<RULES>(ml.x, sub), alpha = kv4_exp<RULES>(top, sub);
+      l = l * alpha + warp_sum(ml.y * f);
 #pragma unroll
-    for (int k = 0; k < kPer; ++k)
+      for (int k = 0; k < kPer; ++k) o[k] *= alpha;
+      top = m;
+#pragma unroll 4
+      for (uint32_t i = 0; i < here; ++i)
+        kv4_add_partial<D>(p.part + (first + size_t(from + i) * cols) * D, __shfl_sync(0xffffffffu, f, i), o);
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; k += 2) {
       kv4_store_out(p.out, size_t(index) * D + lane * kPer + k, p.type, kv4_normalised(o[k], l));
+      kv4_store_out(p.out, size_t(index) * D + lane * kPer + k + 1, p.type, kv4_normalised(o[k + 1], l));
+    }
+    if (lane != 0) return;
   }
-  if (warp == 0 && lane == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(top, l, RULES);
+  if (p.lse != nullptr) p.lse[index] = kv4_lse(top, l, RULES);
 }
 
 // ---------------------------------------------------------------------------
