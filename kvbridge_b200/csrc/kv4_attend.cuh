@@ -297,35 +297,52 @@ __device__ __forceinline__ void kv4_drain(uint64_t* bars, uint32_t ring, uint32_
 // ---------------------------------------------------------------------------
 // Queries.
 
-// Eight consecutive query values from element `at`.
-__device__ __forceinline__ void kv4_load8(const void* q, int64_t at, int32_t type, bool vector, float (&v)[8]) {
-  if (type == 0) {
-    const float* s = static_cast<const float*>(q) + at;
-    if (vector) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(s)), b = __ldg(reinterpret_cast<const float4*>(s) + 1);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __ldg(s + i);
-    }
-    return;
-  }
-  const uint16_t* s = static_cast<const uint16_t*>(q) + at;
-  uint32_t w[4];
-  if (vector) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(s));
-    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+__device__ __forceinline__ void kv4_half_pair(uint32_t w, bool bf16, float& a, float& b) {
+  if (bf16) {
+    a = __uint_as_float(w << 16), b = __uint_as_float(w & 0xffff0000u);
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __ldg(s + 2 * i) | (uint32_t(__ldg(s + 2 * i + 1)) << 16);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    a = f.x, b = f.y;
   }
+}
+
+// N runs of eight query values, run i from element at + step(i). Every load
+// is issued before any is used: one memory round trip.
+template <int N, class F>
+__device__ __forceinline__ void kv4_load_values(const void* q, int64_t at, F&& step, int32_t type, bool vector,
+                                                float (&v)[N][8]) {
+  if (!vector) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (type == 1) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    } else {
-      v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t x = at + step(i) + e;
+        if (type == 0) {
+          v[i][e] = __ldg(static_cast<const float*>(q) + x);
+        } else {
+          float unused;
+          kv4_half_pair(__ldg(static_cast<const uint16_t*>(q) + x), type == 2, v[i][e], unused);
+        }
+      }
+  } else if (type == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + step(i));
+      const float4 a = __ldg(src), b = __ldg(src + 1);
+      v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w, v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z,
+      v[i][7] = b.w;
+    }
+  } else {
+    uint4 raw[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + at + step(i)));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      kv4_half_pair(raw[i].x, type == 2, v[i][0], v[i][1]);
+      kv4_half_pair(raw[i].y, type == 2, v[i][2], v[i][3]);
+      kv4_half_pair(raw[i].z, type == 2, v[i][4], v[i][5]);
+      kv4_half_pair(raw[i].w, type == 2, v[i][6], v[i][7]);
     }
   }
 }
@@ -360,20 +377,20 @@ __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
   const uint32_t r = valid ? col / p.group : 0, head = h * p.group + (valid ? col % p.group : 0);
   const int64_t at = int64_t(b) * p.batch_stride + int64_t(r) * p.row_stride + int64_t(head) * D;
   float v[D / 32][8];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) kv4_load8(p.q, at + kv4_word_dim<D>(tig, i), p.type, p.vector_q, v[i]);
+  kv4_load_values(p.q, at, [&](int i) { return int64_t(kv4_word_dim<D>(tig, i)); }, p.type, p.vector_q, v);
   float amax = 0.f;
-  bool finite = true;
+  float wild = 0.f;  // NaN where a value is not finite
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      finite = finite && fabsf(v[i][e]) <= 3.402823466e38f;
+      wild = fmaf(v[i][e], 0.f, wild);
       amax = fmaxf(amax, fabsf(v[i][e]));
     }
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  finite = __reduce_and_sync(0xfu << (4 * grp), finite ? 1u : 0u) != 0;
+  wild += __shfl_xor_sync(0xffffffffu, wild, 1);
+  wild += __shfl_xor_sync(0xffffffffu, wild, 2);
   // Fixed point n = rint(q * up), |n| <= 2^22: n = d0 + 256 d1 + 65536 d2
   // with signed digits; up is a power of two.
   int e = int((__float_as_uint(amax) >> 23) & 0xffu) - 126;  // amax < 2^e
@@ -428,7 +445,7 @@ __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
   total += __shfl_xor_sync(0xffffffffu, total, 2);
   // Scores in log2 units, or in natural ones where rules come after.
   const float unit = RULES ? p.rule.scale : p.rule.scale * kLog2e;
-  qf.dot = finite ? down * unit : __int_as_float(0x7fffffff);
+  qf.dot = down * unit + wild;
   qf.sum = float(total) * qf.dot;
   qf.slope = RULES && p.rule.slopes != nullptr ? __ldg(p.rule.slopes + head) : 0.f;
   qf.pos = valid ? kv4_query_position(p.rule, b, r, p.rows, len) : -1;
