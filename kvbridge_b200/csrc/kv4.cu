@@ -225,17 +225,17 @@ struct Kv4Shape<256> {
   static constexpr int kSlots = 1, kCtas = 2, kWeighSlots = 2, kWeighCtas = 2;
 };
 
-template <int D, int L, bool RULES>
+template <int D, int C, int PD, bool RULES>
 Kv4Kernel attend_kernel() {
   using T = Kv4Shape<D>;
-  return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, L, T::kSlots, T::kCtas, RULES>),
+  return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, C, PD, T::kSlots, T::kCtas, RULES>),
           kvb::Kv4Smem<D, T::kSlots, true>::kBytes};
 }
 
-template <int D, int L, bool RULES>
+template <int D, int C, bool RULES>
 Kv4Kernel weigh_kernel() {
   using T = Kv4Shape<D>;
-  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, L, T::kWeighSlots, T::kWeighCtas, RULES>),
+  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, T::kWeighSlots, T::kWeighCtas, RULES>),
           kvb::Kv4Smem<D, T::kWeighSlots, false>::kBytes};
 }
 
@@ -243,29 +243,26 @@ bool has_rules(const Kv4Pool& pool, const Kv4Query& q) {
   return q.softcap > 0.f || q.window != 0 || q.slopes || q.prefix_lens || q.q_positions || pool.positions;
 }
 
-// Column layout: three digits where four columns are enough (they cost
-// nothing there) or fp32 outputs need them, else two.
-int attend_layout(const Kv4Pool& pool, const Kv4Query& q) {
-  if (q.rows * (q.q_heads / pool.kv_heads) <= 4) return kvb::kCols4;
-  return q.type == Kv4Type::f32 ? kvb::kCols8x3 : kvb::kCols8x2;
+// Query columns a segment: 4 where all of a KV head's fit, else 8.
+uint32_t segment_columns(const Kv4Pool& pool, const Kv4Query& q) {
+  return q.rows * (q.q_heads / pool.kv_heads) <= 4 ? 4 : 8;
 }
 
 template <bool RULES>
-Kv4Kernel attend_kernel(uint32_t dim, int layout) {
+Kv4Kernel attend_kernel(uint32_t dim, uint32_t cols, bool f32) {
   return by_dim(dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    return layout == kvb::kCols4     ? attend_kernel<D, kvb::kCols4, RULES>()
-           : layout == kvb::kCols8x2 ? attend_kernel<D, kvb::kCols8x2, RULES>()
-                                     : attend_kernel<D, kvb::kCols8x3, RULES>();
+    return cols == 4 ? f32 ? attend_kernel<D, 4, 3, RULES>() : attend_kernel<D, 4, 2, RULES>()
+           : f32     ? attend_kernel<D, 8, 3, RULES>()
+                     : attend_kernel<D, 8, 2, RULES>();
   });
 }
 
-// Weights are fp32 whatever the queries: three digits.
 template <bool RULES>
-Kv4Kernel weigh_kernel(uint32_t dim, bool four) {
+Kv4Kernel weigh_kernel(uint32_t dim, uint32_t cols) {
   return by_dim(dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    return four ? weigh_kernel<D, kvb::kCols4, RULES>() : weigh_kernel<D, kvb::kCols8x3, RULES>();
+    return cols == 4 ? weigh_kernel<D, 4, RULES>() : weigh_kernel<D, 8, RULES>();
   });
 }
 
@@ -302,9 +299,8 @@ uint32_t split_ctas(const Kv4Kernel& k, uint64_t segments, uint32_t max_tokens) 
 
 struct AttendPlan {
   Kv4Kernel kernel;
-  int layout;
   bool rules, direct, many;
-  uint32_t col_groups, segments, ctas, workers;
+  uint32_t cols, col_groups, segments, ctas, workers;
   size_t ml_offset, warps_offset, bytes;  // of the workspace
 };
 
@@ -314,9 +310,9 @@ constexpr uint32_t kDirectTokens = 128;
 AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
   AttendPlan a{};
   a.rules = has_rules(pool, q);
-  a.layout = attend_layout(pool, q);
-  a.kernel = a.rules ? attend_kernel<true>(pool.dim, a.layout) : attend_kernel<false>(pool.dim, a.layout);
-  const uint32_t cols = uint32_t(kvb::kv4_cols(a.layout)), all = q.rows * (q.q_heads / pool.kv_heads);
+  const bool f32 = q.type == Kv4Type::f32;
+  const uint32_t cols = a.cols = segment_columns(pool, q), all = q.rows * (q.q_heads / pool.kv_heads);
+  a.kernel = a.rules ? attend_kernel<true>(pool.dim, cols, f32) : attend_kernel<false>(pool.dim, cols, f32);
   a.col_groups = (all + cols - 1) / cols;
   a.segments = q.batch * pool.kv_heads * a.col_groups;
   a.direct = q.max_tokens <= kDirectTokens;
@@ -365,7 +361,7 @@ void launch_attention_kv4(const Kv4Pool& pool, const Kv4Query& q, void* workspac
   launch_kernel_pdl(a.kernel.fn, dim3(a.ctas), dim3(kvb::kKv4Threads), a.kernel.smem, stream, args,
                     "kv4 attention launch");
   if (a.direct) return;
-  uint32_t cols = uint32_t(kvb::kv4_cols(a.layout));
+  uint32_t cols = a.cols;
   void* merge_args[] = {&prm, &cols};
   const void* merge = by_dim(pool.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
@@ -388,10 +384,8 @@ void accumulate_weights_kv4(const Kv4Pool& pool, const Kv4Query& q, const float*
   if (weight_stride < int64_t(prm.max_tokens))
     throw std::invalid_argument("weight_stride must be at least max_tokens");
   if (prm.max_tokens == 0) return;
-  const uint32_t all = q.rows * prm.group;
-  const bool four = all <= 4;
-  const uint32_t groups = four ? 1 : (all + 7) / 8;
-  const Kv4Kernel k = has_rules(pool, q) ? weigh_kernel<true>(pool.dim, four) : weigh_kernel<false>(pool.dim, four);
+  const uint32_t cols = segment_columns(pool, q), groups = (q.rows * prm.group + cols - 1) / cols;
+  const Kv4Kernel k = has_rules(pool, q) ? weigh_kernel<true>(pool.dim, cols) : weigh_kernel<false>(pool.dim, cols);
   prm.col_groups = 1;
   const uint32_t ctas = split_ctas(k, uint64_t(q.batch) * pool.kv_heads, prm.max_tokens);
   prm.workers = ctas * kvb::kKv4Warps;

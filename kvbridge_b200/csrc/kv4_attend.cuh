@@ -27,23 +27,26 @@
 //            of P * 2^e + 2^23. These sums count codes from -8 too; the part
 //            that carries lo, sum exp(x - m) * (lo + 8 v_scale), is in fp32.
 //
-// Column layouts (template L):
-//   kCols4    up to 4 query columns a segment, three digits on both sides.
-//             One m16 tile holds digits 0 and 1 of column c in rows c and
-//             c + 8, digit 2 in row c + 4; lanes c and c + 4 share a column.
-//   kCols8x2  up to 8 columns, three digits of q in two m16 tiles (the lse is
-//             fp32 whatever the outputs are), two digits of P: 2^-16 of the
-//             tile's largest, below the rounding of 16-bit outputs.
-//   kCols8x3  up to 8 columns, three digits on both sides: fp32 outputs.
+// Column layouts: C query columns a segment (4 or 8) and PD digits of P.
+//   q      Rows c and c + 8 of the first m16 tile are digits 0 and 1 of
+//          column c; with 8 columns digit 2 is row c of a second tile, with 4
+//          it is row c + 4 of the first.
+//   P      8 columns: rows c and c + 8 are digits 0 and 1. 4 columns: lanes c
+//          and c + 4 share a column and split its tokens (and the work on
+//          them): rows c and c + 8 have the digits of one's tokens, rows c + 4
+//          and c + 12 those of the other's, zeros for the rest; each lane
+//          sums its own share of the output. PD = 3: digit 2 in the same rows
+//          of a second tile.
+// PD = 2 holds P to 2^-16 of the tile's largest, below the rounding of 16-bit
+// outputs; fp32 outputs take 3. The lse is fp32 always, hence three q digits.
 #include "kv4_common.cuh"
 #include "kvb_schedule.h"
 
 namespace kvb {
 
-enum : int { kCols4 = 0, kCols8x2 = 1, kCols8x3 = 2 };
-constexpr int kv4_cols(int layout) { return layout == kCols4 ? 4 : 8; }
-constexpr int kv4_q_tiles(int layout) { return layout == kCols4 ? 1 : 2; }    // m16 tiles of the scores
-constexpr int kv4_p_tiles(int layout) { return layout == kCols8x3 ? 2 : 1; }  // and of the output
+constexpr int kv4_q_tiles(int cols) { return cols == 4 ? 1 : 2; }       // m16 tiles of the scores
+constexpr int kv4_p_tiles(int digits) { return digits == 3 ? 2 : 1; }   // and of the output
+constexpr int kv4_tokens(int cols) { return cols == 4 ? 8 : 16; }       // of a stage, a lane
 
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Threads = 32 * kKv4Warps;
@@ -348,15 +351,18 @@ __device__ __forceinline__ void kv4_load_values(const void* q, int64_t at, F&& s
 }
 
 // The A operand of the scores for one group of columns. Lane (grp, tig) =
-// (lane / 4, lane % 4) holds column grp (kCols4: grp % 4) at the dims of its
+// (lane / 4, lane % 4) holds column grp (4 columns: grp % 4) at the dims of its
 // quarter of each K row: word i of the lane's packed row covers 8 dims, the
 // even ones in the low halves (a[.][0], a[.][1]), the odd ones in the high
 // halves (a[.][2], a[.][3]).
-template <int D, int L>
+template <int D, int C>
 struct Kv4Query {
-  uint32_t a[kv4_q_tiles(L)][D / 32][4];
-  int start[kv4_q_tiles(L)][2];  // -8 * digit sums of rows grp and grp + 8
-  float dot, sum;  // score = scale_t * dot * (A . (codes - 8)) + (lo_t + 8 scale_t) * sum
+  uint32_t a[kv4_q_tiles(C)][D / 32][4];
+  int start[kv4_q_tiles(C)][2];  // -8 * digit sums of rows grp and grp + 8
+  // score = scale_t * (A . (codes - 8)) + (lo_t + 8 scale_t) * sum, the dot
+  // product in parts: 8 columns digits 0 and 1, digit 2; 4 columns the
+  // lane's own digits, the other lane's.
+  float own, other, sum;
   float slope;
   int32_t pos;     // query position
 };
@@ -368,11 +374,11 @@ __device__ __forceinline__ uint32_t kv4_word_dim(uint32_t tig, uint32_t i) {
   return (D / 4) * tig + 8 * i;
 }
 
-template <int D, int L, bool RULES>
+template <int D, int C, bool RULES>
 __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h, uint32_t col_group,
-                               uint32_t len, Kv4Query<D, L>& qf) {
+                               uint32_t len, Kv4Query<D, C>& qf) {
   const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
-  const uint32_t col = col_group * kv4_cols(L) + (L == kCols4 ? grp & 3 : grp);
+  const uint32_t col = col_group * C + grp % C;
   const bool valid = col < p.rows * p.group;
   const uint32_t r = valid ? col / p.group : 0, head = h * p.group + (valid ? col % p.group : 0);
   const int64_t at = int64_t(b) * p.batch_stride + int64_t(r) * p.row_stride + int64_t(head) * D;
@@ -417,7 +423,7 @@ __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
       const uint32_t d0 = __byte_perm(x, y, 0x5410) ^ 0x80808080u, d1 = __byte_perm(x, y, 0x7632) ^ 0x80808080u;
       const uint32_t x2 = __byte_perm(w[0], w[1], 0x0062), y2 = __byte_perm(w[2], w[3], 0x0062);
       const uint32_t d2 = __byte_perm(x2, y2, 0x5410) ^ 0x80808080u;
-      if constexpr (L == kCols4) {
+      if constexpr (C == 4) {
         qf.a[0][i][2 * odd] = grp >= 4 ? d2 : d0;
         qf.a[0][i][2 * odd + 1] = grp >= 4 ? 0u : d1;
       } else {
@@ -428,7 +434,7 @@ __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
       }
     }
 #pragma unroll
-  for (int m = 0; m < kv4_q_tiles(L); ++m)
+  for (int m = 0; m < kv4_q_tiles(C); ++m)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       int s = 0;
@@ -445,22 +451,32 @@ __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
   total += __shfl_xor_sync(0xffffffffu, total, 2);
   // Scores in log2 units, or in natural ones where rules come after.
   const float unit = RULES ? p.rule.scale : p.rule.scale * kLog2e;
-  qf.dot = down * unit + wild;
-  qf.sum = float(total) * qf.dot;
+  const float dot = down * unit + wild;
+  qf.own = C == 4 && grp >= 4 ? 65536.f * dot : dot;
+  qf.other = C == 4 && grp >= 4 ? dot : 65536.f * dot;
+  qf.sum = float(total) * dot;
   qf.slope = RULES && p.rule.slopes != nullptr ? __ldg(p.rule.slopes + head) : 0.f;
   qf.pos = valid ? kv4_query_position(p.rule, b, r, p.rows, len) : -1;
 }
 
 // ---------------------------------------------------------------------------
-// Scores of one stage: thread (grp, tig) gets those of its column for the
-// tokens 16 tig + [0, 16). N-tile j takes tokens 16 (n / 2) + 2 j + n % 2, so
-// that the thread's C fragments (n = 2 tig, 2 tig + 1) are its tokens 2 j and
-// 2 j + 1, and a quarter-warp reads two neighbouring K rows.
-template <int D, int L>
-__device__ __forceinline__ void kv4_dots(const uint8_t* codes, const uint32_t (&a)[kv4_q_tiles(L)][D / 32][4],
-                                         const int (&start)[kv4_q_tiles(L)][2], float (&sc)[16]) {
+// Dot products of one stage's tokens with the thread's column. N-tile j takes
+// tokens 16 (n / 2) + 2 j + n % 2, so that a thread's C fragments (n = 2 tig,
+// 2 tig + 1) are tokens 16 tig + 2 j and the next, and a quarter-warp reads
+// two neighbouring K rows. 8 columns: sc[u] is token 16 tig + u. 4 columns:
+// lane c keeps tokens 0-3 and 8-11 of the 16 (u = 0..7), lane c + 4 the rest.
+__device__ __forceinline__ uint32_t kv4_token(int cols, int u) { return cols == 4 ? (u & 3) + 8 * (u >> 2) : u; }
+template <int C>
+__device__ __forceinline__ uint32_t kv4_first_token() {
+  const uint32_t lane = threadIdx.x & 31;
+  return 16 * (lane & 3) + (C == 4 ? 4 * (lane >> 4) : 0);
+}
+
+template <int D, int C>
+__device__ __forceinline__ void kv4_dots(const uint8_t* codes, const Kv4Query<D, C>& qf, float (&sc)[kv4_tokens(C)]) {
   const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
   constexpr int kWords = D / 32;
+  float part[C == 4 ? 16 : 1];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const uint8_t* row = codes + (16 * (grp >> 1) + 2 * j + (grp & 1)) * (D / 2);
@@ -475,28 +491,36 @@ __device__ __forceinline__ void kv4_dots(const uint8_t* codes, const uint32_t (&
         w[4 * c] = x.x, w[4 * c + 1] = x.y, w[4 * c + 2] = x.z, w[4 * c + 3] = x.w;
       }
     }
-    int acc[kv4_q_tiles(L)][4];
-#pragma unroll
-    for (int m = 0; m < kv4_q_tiles(L); ++m)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[m][e] = start[m][e / 2];
+    int acc[kv4_q_tiles(C)][4];
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
       const uint32_t lo = w[i] & 0x0f0f0f0fu, hi = (w[i] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-      for (int m = 0; m < kv4_q_tiles(L); ++m)
-        imma_16832(acc[m], a[m][i][0], a[m][i][1], a[m][i][2], a[m][i][3], lo, hi);
+      for (int m = 0; m < kv4_q_tiles(C); ++m) {
+        const uint32_t* a = qf.a[m][i];
+        const int s0 = qf.start[m][0], s1 = qf.start[m][1];
+        if (i == 0)
+          imma_16832(acc[m], a[0], a[1], a[2], a[3], lo, hi, s0, s0, s1, s1);
+        else
+          imma_16832(acc[m], a[0], a[1], a[2], a[3], lo, hi);
+      }
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       // |digit dot| <= 128 * 8 * 256: exact in s32 with its neighbour
-      float x = float(acc[0][e] + 256 * acc[0][2 + e]);
-      if constexpr (L != kCols4) x = fmaf(float(acc[1][e]), 65536.f, x);
-      if constexpr (L == kCols4) {
-        if (grp >= 4) x *= 65536.f;
-        x += __shfl_xor_sync(0xffffffffu, x, 16);
-      }
-      sc[2 * j + e] = x;
+      const float x = float(acc[0][e] + 256 * acc[0][2 + e]);
+      if constexpr (C == 8) sc[2 * j + e] = fmaf(x, qf.own, float(acc[1][e]) * qf.other);
+      else part[2 * j + e] = x;
+    }
+  }
+  if constexpr (C == 4) {
+    // Lane c has digits 0 and 1 of all 16 tokens, lane c + 4 digit 2: swap.
+    const bool upper = lane >= 16;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int t = kv4_token(4, u);
+      const float give = upper ? part[t] : part[t + 4], keep = upper ? part[t + 4] : part[t];
+      sc[u] = fmaf(keep, qf.own, __shfl_xor_sync(0xffffffffu, give, 16) * qf.other);
     }
   }
 }
@@ -522,65 +546,52 @@ __device__ __forceinline__ float kv4_exp(float x, float y) {
   return fast_exp2(RULES ? (x - y) * kLog2e : x - y);
 }
 
-// Scores from the digit dots; invisible ones -inf. Returns the thread's
-// visible tokens as a bit mask (all ones where MASK is false). pos: the
-// positions of the thread's 16 tokens, or null for their indices.
-template <int D, bool RULES, bool MASK>
+// Scores from the dot products; invisible ones -inf. Returns the thread's
+// visible tokens as a bit mask (all ones where MASK is false). tb: the stage's
+// first token; pos: the positions of the thread's quad's 16 tokens, or null
+// for their indices.
+template <int C, bool RULES, bool MASK>
 __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const uint8_t* params, uint32_t tb,
-                                               uint32_t len, uint32_t prefix, float dot, float sum, float slope,
-                                               int32_t pq, const int32_t* pos, float (&sc)[16]) {
-  const uint32_t tig = threadIdx.x & 3;
-  const float4* par = reinterpret_cast<const float4*>(params + 128 * tig);
-  if constexpr (!RULES) {
-    uint32_t seen = 0xffffu;
-    if (MASK) {
-      // tokens t <= pq < len
-      const int32_t n = pq + 1 - int32_t(tb + 16 * tig);
-      seen = n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u;
-    }
+                                               uint32_t len, uint32_t prefix, float sum, float slope, int32_t pq,
+                                               const int32_t* pos, float (&sc)[kv4_tokens(C)]) {
+  constexpr int kTokens = kv4_tokens(C);
+  const uint32_t at = kv4_first_token<C>();
+  const float4* par = reinterpret_cast<const float4*>(params + 8 * at);
+  const int32_t t0 = int32_t(tb + at);
+  uint32_t seen = (1u << kTokens) - 1;
+  const float cap = p.rule.softcap, inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
+  if (RULES) seen = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 f = par[i];
-      sc[2 * i] = fmaf(sc[2 * i] * dot, f.x, fmaf(8.f, f.x, f.y) * sum);
-      sc[2 * i + 1] = fmaf(sc[2 * i + 1] * dot, f.z, fmaf(8.f, f.z, f.w) * sum);
-    }
-    if (MASK) {
+  for (int u = 0; u < kTokens; u += 2) {
+    const float4 f = par[kv4_token(C, u) / 2];
+    sc[u] = fmaf(sc[u], f.x, fmaf(8.f, f.x, f.y) * sum);
+    sc[u + 1] = fmaf(sc[u + 1], f.z, fmaf(8.f, f.z, f.w) * sum);
+    if constexpr (RULES) {
 #pragma unroll
-      for (int t = 0; t < 16; ++t)
-        if (!(seen >> t & 1u)) sc[t] = -INFINITY;
-    }
-    return seen;
-  } else {
-    uint32_t seen = 0;
-    const float cap = p.rule.softcap, inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
-    const int32_t t0 = int32_t(tb + 16 * tig);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      int32_t pk[4];
-      if (pos != nullptr) {
-        const int4 x = __ldg(reinterpret_cast<const int4*>(pos) + i);
-        pk[0] = x.x, pk[1] = x.y, pk[2] = x.z, pk[3] = x.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) pk[e] = t0 + 4 * i + e;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = 4 * i + e;
-        const float4 f = par[2 * i + e / 2];
-        const float scale = e % 2 ? f.z : f.x, lo = e % 2 ? f.w : f.y;
-        float x = fmaf(sc[t] * dot, scale, fmaf(8.f, scale, lo) * sum);
+      for (int e = 0; e < 2; ++e) {
+        const int32_t token = int32_t(kv4_token(C, u + e));
+        const int32_t pk = pos != nullptr ? __ldg(pos + (at & 15) + token) : t0 + token;
+        float x = sc[u + e];
         if (cap > 0.f) x = kv4_cap(x, cap, inv_cap);
         // exact below 2^24; |pq - pk| as the larger minus the smaller
-        const uint32_t away = pq >= pk[e] ? uint32_t(pq) - uint32_t(pk[e]) : uint32_t(pk[e]) - uint32_t(pq);
+        const uint32_t away = pq >= pk ? uint32_t(pq) - uint32_t(pk) : uint32_t(pk) - uint32_t(pq);
         x = fmaf(-slope, float(away), x);
-        const bool on = uint32_t(t0 + t) < len && kv4_visible(pk[e], pq, p.rule.window, prefix);
-        sc[t] = on ? x : -INFINITY;
-        seen |= on ? 1u << t : 0u;
+        const bool on = uint32_t(t0 + token) < len && kv4_visible(pk, pq, p.rule.window, prefix);
+        sc[u + e] = on ? x : -INFINITY;
+        seen |= on ? 1u << (u + e) : 0u;
       }
     }
-    return seen;
   }
+  if (!RULES && MASK) {
+    seen = 0;
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+      const bool on = t0 + int32_t(kv4_token(C, u)) <= pq;  // pq < len
+      sc[u] = on ? sc[u] : -INFINITY;
+      seen |= on ? 1u << u : 0u;
+    }
+  }
+  return seen;
 }
 
 // ---------------------------------------------------------------------------
@@ -588,21 +599,29 @@ __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const u
 
 template <int D>
 struct Kv4State {
-  float o[D / 16][4];  // dims 16 j + 4 tig + [0, 4) of the thread's column (kCols4: its digits' share)
-  float m;             // running max, the same in a column's four lanes
+  float o[D / 16][4];  // dims 16 j + 4 tig + [0, 4) of the thread's column (or its share)
+  float m;             // running max, the same in all lanes of a column
   float l, lo;         // the thread's part of sum p and of sum p * (lo + 8 scale)
 };
 
-template <int D, int L, bool RULES, bool MASK>
-__device__ __forceinline__ void kv4_softmax(const uint8_t* vparams, uint32_t seen, float (&sc)[16],
-                                            Kv4State<D>& st, uint32_t (&digit)[kv4_p_tiles(L)][2][4],
-                                            float& out_scale) {
-  const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
-  float top = sc[0];
+template <int N>
+__device__ __forceinline__ float kv4_max(const float (&x)[N]) {
+  float y = x[0];
 #pragma unroll
-  for (int t = 1; t < 16; ++t) top = fmaxf(top, sc[t]);
+  for (int i = 1; i + 1 < N; i += 2) y = max3(y, x[i], x[i + 1]);
+  return fmaxf(y, x[N - 1]);
+}
+
+template <int D, int C, int PD, bool RULES, bool MASK>
+__device__ __forceinline__ void kv4_softmax(const uint8_t* vparams, uint32_t seen, float (&sc)[kv4_tokens(C)],
+                                            Kv4State<D>& st, uint32_t (&digit)[kv4_p_tiles(PD)][2][4],
+                                            float& out_scale) {
+  constexpr int kTokens = kv4_tokens(C);
+  const bool upper = C == 4 && (threadIdx.x & 16) != 0;
+  float top = kv4_max(sc);
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  if (C == 4) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
   const float m = fmaxf(st.m, top);
   const float sub = m == -INFINITY ? 0.f : m;
   const float alpha = m == st.m ? 1.f : kv4_exp<RULES>(st.m, sub);
@@ -615,78 +634,72 @@ __device__ __forceinline__ void kv4_softmax(const uint8_t* vparams, uint32_t see
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.o[j][e] *= alpha;
   }
-  const float4* par = reinterpret_cast<const float4*>(vparams + 128 * tig);
-  float big = 0.f;
+  const float4* par = reinterpret_cast<const float4*>(vparams + 8 * kv4_first_token<C>());
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float4 f = par[i];
+  for (int u = 0; u < kTokens; u += 2) {
+    const float4 f = par[kv4_token(C, u) / 2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int t = 2 * i + e;
       const float scale = e ? f.z : f.x, lo = e ? f.w : f.y;
-      const float pr = kv4_exp<RULES>(sc[t], sub);
+      const float pr = kv4_exp<RULES>(sc[u + e], sub);
       st.l += pr;
-      float w = pr * scale;
-      float mid = fmaf(8.f, scale, lo) * pr;
-      if (MASK && !(seen >> t & 1u)) w = 0.f, mid = 0.f;  // whatever the slot holds
-      st.lo += mid;
-      sc[t] = w;
-      big = fmaxf(big, w);
+      float w = pr * scale, mid = fmaf(8.f, scale, lo);
+      if (MASK && !(seen >> (u + e) & 1u)) w = 0.f, mid = 0.f;  // whatever the slot holds
+      st.lo = fmaf(mid, pr, st.lo);
+      sc[u + e] = w;
     }
   }
+  float big = kv4_max(sc);
   big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
   big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
   // Power of two (a little less, so that nothing rounds up to the next one)
   // that puts the tile's largest below 2^16 or 2^23: the fixed-point values
   // are the low bytes of sc * up + 2^23.
-  constexpr uint32_t kTop = L == kCols8x2 ? 269 : 276;
+  constexpr uint32_t kTop = PD == 2 ? 269 : 276;
   constexpr float kLess = 1.0f - 1.0f / 16384.0f;
   const uint32_t ex = max(__float_as_uint(big) >> 23, kTop - 253u);
   const float up = kLess * __uint_as_float((kTop - ex) << 23);
   out_scale = (1.0f / kLess) * __uint_as_float((ex - (kTop - 254u)) << 23);
+  // A fragments: tokens 8 i .. 8 i + 3 of the quad's 16 feed a[0] and a[1] of
+  // fragment i, the next four a[2] and a[3].
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
+  for (int h = 0; h < kTokens / 4; ++h) {
     uint32_t f[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = __float_as_uint(fmaf(sc[4 * h + e], up, 8388608.0f));
     const uint32_t x = __byte_perm(f[0], f[1], 0x5140), y = __byte_perm(f[2], f[3], 0x5140);
-    const uint32_t d0 = __byte_perm(x, y, 0x5410), d1 = __byte_perm(x, y, 0x7632);
-    // tokens 8 i .. 8 i + 3 feed a[0] and a[1], the next four a[2] and a[3]
-    uint32_t* a = digit[0][h / 2] + 2 * (h % 2);
-    if constexpr (L == kCols8x2) {
-      a[0] = d0;
-      a[1] = d1;
-    } else {
-      const uint32_t x2 = __byte_perm(f[0], f[1], 0x0062), y2 = __byte_perm(f[2], f[3], 0x0062);
-      const uint32_t d2 = __byte_perm(x2, y2, 0x5410);
-      if constexpr (L == kCols4) {
-        a[0] = grp >= 4 ? d2 : d0;
-        a[1] = grp >= 4 ? 0u : d1;
+    uint32_t d[3] = {__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632), 0u};
+    if constexpr (PD == 3)
+      d[2] = __byte_perm(__byte_perm(f[0], f[1], 0x0062), __byte_perm(f[2], f[3], 0x0062), 0x5410);
+#pragma unroll
+    for (int k = 0; k < PD; ++k) {
+      if constexpr (C == 4) {
+        digit[k / 2][h][k % 2] = upper ? 0u : d[k];
+        digit[k / 2][h][2 + k % 2] = upper ? d[k] : 0u;
       } else {
-        a[0] = d0;
-        a[1] = d1;
-        digit[1][h / 2][2 * (h % 2)] = d2;
-        digit[1][h / 2][2 * (h % 2) + 1] = 0u;
+        digit[k / 2][h / 2][2 * (h % 2) + k % 2] = d[k];
       }
     }
   }
-  if constexpr (L == kCols4) out_scale *= grp >= 4 ? 65536.f : 1.f;
+  if constexpr (PD == 3)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) digit[1][i][1] = digit[1][i][3] = 0u;
 }
 
 // O += P . V for one stage. Thread (grp, tig) reads, for the dim pair 8 j +
-// grp, the codes of its 16 tokens; low halves are the even dims' tile, high
-// halves the odd dims'.
-template <int D, int L>
+// grp, the codes of its quad's 16 tokens; low halves are the even dims' tile,
+// high halves (16 times the codes) the odd dims'.
+template <int D, int PD>
 __device__ __forceinline__ void kv4_output(const uint8_t* codes, uint32_t P, uint32_t pitch,
-                                           const uint32_t (&digit)[kv4_p_tiles(L)][2][4], float out_scale,
+                                           const uint32_t (&digit)[kv4_p_tiles(PD)][2][4], float out_scale,
                                            Kv4State<D>& st) {
   const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
   const uint8_t* base = codes + (16 * tig / P) * pitch + (16 * tig % P) + grp * P;
   const float odd_scale = out_scale * 0.0625f;
   // -8 * (sum of the row's digits): rows grp and grp + 8 of every tile.
-  int start[kv4_p_tiles(L)][2];
+  int start[kv4_p_tiles(PD)][2], start16[kv4_p_tiles(PD)][2];
 #pragma unroll
-  for (int m = 0; m < kv4_p_tiles(L); ++m)
+  for (int m = 0; m < kv4_p_tiles(PD); ++m)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       uint32_t s = 0;
@@ -698,30 +711,28 @@ __device__ __forceinline__ void kv4_output(const uint8_t* codes, uint32_t P, uin
       s += __shfl_xor_sync(0xffffffffu, s, 1);
       s += __shfl_xor_sync(0xffffffffu, s, 2);
       start[m][r] = -8 * int(s);
+      start16[m][r] = -128 * int(s);
     }
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) {
     const uint4 w = *reinterpret_cast<const uint4*>(base + 8 * j * P);
-    const uint32_t lo[4] = {w.x & 0x0f0f0f0fu, w.y & 0x0f0f0f0fu, w.z & 0x0f0f0f0fu, w.w & 0x0f0f0f0fu};
-    // 16 times the odd dims' codes
-    const uint32_t hi[4] = {w.x & 0xf0f0f0f0u, w.y & 0xf0f0f0f0u, w.z & 0xf0f0f0f0u, w.w & 0xf0f0f0f0u};
-    int even[kv4_p_tiles(L)][4], odd[kv4_p_tiles(L)][4];
+    int even[kv4_p_tiles(PD)][4], odd[kv4_p_tiles(PD)][4];
 #pragma unroll
-    for (int m = 0; m < kv4_p_tiles(L); ++m) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) even[m][e] = start[m][e / 2], odd[m][e] = 16 * start[m][e / 2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t* a = digit[m][i];
-        imma_u8_16832(even[m], a[0], a[1], a[2], a[3], lo[2 * i], lo[2 * i + 1]);
-        imma_u8_16832(odd[m], a[0], a[1], a[2], a[3], hi[2 * i], hi[2 * i + 1]);
-      }
+    for (int m = 0; m < kv4_p_tiles(PD); ++m) {
+      const uint32_t(&a)[2][4] = digit[m];
+      const int s0 = start[m][0], s1 = start[m][1], t0 = start16[m][0], t1 = start16[m][1];
+      imma_u8_16832(even[m], a[0][0], a[0][1], a[0][2], a[0][3], w.x & 0x0f0f0f0fu, w.y & 0x0f0f0f0fu, s0, s0, s1, s1);
+      imma_u8_16832(odd[m], a[0][0], a[0][1], a[0][2], a[0][3], w.x & 0xf0f0f0f0u, w.y & 0xf0f0f0f0u, t0, t0, t1, t1);
+      imma_u8_16832(even[m], a[1][0], a[1][1], a[1][2], a[1][3], w.z & 0x0f0f0f0fu, w.w & 0x0f0f0f0fu, even[m][0],
+                    even[m][1], even[m][2], even[m][3]);
+      imma_u8_16832(odd[m], a[1][0], a[1][1], a[1][2], a[1][3], w.z & 0xf0f0f0f0u, w.w & 0xf0f0f0f0u, odd[m][0],
+                    odd[m][1], odd[m][2], odd[m][3]);
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       // exact: |sum| <= 255 * 128 * 64 a digit, times 257 below 2^30
       float x = float(even[0][e] + 256 * even[0][2 + e]), y = float(odd[0][e] + 256 * odd[0][2 + e]);
-      if constexpr (L == kCols8x3) {
+      if constexpr (PD == 3) {
         x = fmaf(float(even[1][e]), 65536.f, x);
         y = fmaf(float(odd[1][e]), 65536.f, y);
       }
@@ -795,7 +806,7 @@ __device__ __forceinline__ void kv4_report_lengths(const Kv4AttendParams& p) {
     if (__ldg(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
 }
 
-template <int D, int L, int SLOTS, int MINB, bool RULES>
+template <int D, int C, int PD, int SLOTS, int MINB, bool RULES>
 __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4AttendParams p) {
   using S = Kv4Smem<D, SLOTS, true>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -828,13 +839,12 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
   uint32_t done = 0;
   bool failed = false;
   const uint32_t vpitch = kv4_v_pitch(p.page_tokens * (D / 2), p.page_tokens);
-  constexpr uint32_t kCols = kv4_cols(L);
 
   do {  // pieces
     const uint32_t first = done, end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
     const uint32_t h = cur.seg / p.col_groups;
-    Kv4Query<D, L> qf;
-    kv4_load_query<D, L, RULES>(p, cur.b, h, cur.seg % p.col_groups, cur.len, qf);
+    Kv4Query<D, C> qf;
+    kv4_load_query<D, C, RULES>(p, cur.b, h, cur.seg % p.col_groups, cur.len, qf);
     const uint32_t prefix = RULES && p.rule.prefix != nullptr ? __ldg(p.rule.prefix + cur.b) : 0u;
     // Tokens below this are visible to every row (no rules).
     const int32_t clear = int32_t(cur.len) - int32_t(p.rows) + 1;
@@ -856,20 +866,20 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
         failed = true;
         break;
       }
-      float sc[16];
-      uint32_t digit[kv4_p_tiles(L)][2][4], seen;
+      float sc[kv4_tokens(C)];
+      uint32_t digit[kv4_p_tiles(PD)][2][4];
       float out_scale;
-      kv4_dots<D, L>(slot, qf.a, qf.start, sc);
+      kv4_dots<D, C>(slot, qf, sc);
       if (!RULES && int32_t(tb + kStageTokens) <= clear) {
-        seen = kv4_scores<D, RULES, false>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope,
-                                           qf.pos, pos, sc);
-        kv4_softmax<D, L, RULES, false>(slot + S::kOffVp, seen, sc, st, digit, out_scale);
+        const uint32_t seen = kv4_scores<C, RULES, false>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope,
+                                                          qf.pos, pos, sc);
+        kv4_softmax<D, C, PD, RULES, false>(slot + S::kOffVp, seen, sc, st, digit, out_scale);
       } else {
-        seen = kv4_scores<D, RULES, true>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope,
-                                          qf.pos, pos, sc);
-        kv4_softmax<D, L, RULES, true>(slot + S::kOffVp, seen, sc, st, digit, out_scale);
+        const uint32_t seen = kv4_scores<C, RULES, true>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope,
+                                                         qf.pos, pos, sc);
+        kv4_softmax<D, C, PD, RULES, true>(slot + S::kOffVp, seen, sc, st, digit, out_scale);
       }
-      kv4_output<D, L>(slot + S::kOffV, p.page_tokens, vpitch, digit, out_scale, st);
+      kv4_output<D, PD>(slot + S::kOffV, p.page_tokens, vpitch, digit, out_scale, st);
       __syncwarp();  // every lane has read the slot
       if (done + SLOTS < count) {
         feed.copy(p);
@@ -882,24 +892,28 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
     st.lo += __shfl_xor_sync(0xffffffffu, st.lo, 1);
     st.lo += __shfl_xor_sync(0xffffffffu, st.lo, 2);
+    if (C == 4) {
+      st.l += __shfl_xor_sync(0xffffffffu, st.l, 16);
+      st.lo += __shfl_xor_sync(0xffffffffu, st.lo, 16);
+    }
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if constexpr (L == kCols4) st.o[j][e] += __shfl_xor_sync(0xffffffffu, st.o[j][e], 16);
+        if constexpr (C == 4) st.o[j][e] += __shfl_xor_sync(0xffffffffu, st.o[j][e], 16);
         st.o[j][e] += st.lo;
       }
     // The whole segment: the output; else a partial.
     const bool whole = int32_t(first) == cur.base && end - first == cur.stages;
     const uint32_t segment = cur.b * segs + cur.seg;
     size_t index;
-    if (grp < kCols && kv4_column(p, cur.b, cur.seg, grp, kCols, index)) {
+    if (grp < C && kv4_column(p, cur.b, cur.seg, grp, C, index)) {
       if (whole) {
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) kv4_store_out4(p.out, index * D + 16 * j + 4 * tig, p.type, st.o[j], st.l);
         if (tig == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(st.m, st.l, RULES);
       } else {
-        const size_t at = size_t(worker + segment) * kCols + grp;
+        const size_t at = size_t(worker + segment) * C + grp;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j)
           *reinterpret_cast<float4*>(p.part + at * D + 16 * j + 4 * tig) =
@@ -1029,7 +1043,7 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv
 // one thread adds up a token's weight in a fixed order, so there are no
 // atomics, and the groups' launches follow one another.
 
-template <int D, int L, int SLOTS, int MINB, bool RULES>
+template <int D, int C, int SLOTS, int MINB, bool RULES>
 __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4AttendParams p, uint32_t group) {
   using S = Kv4Smem<D, SLOTS, false>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -1062,12 +1076,12 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
 
   while (done < count && !failed) {
     const uint32_t end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
-    Kv4Query<D, L> qf;
-    kv4_load_query<D, L, RULES>(p, cur.b, cur.seg, group, cur.len, qf);
-    // Infinite: a column that is not there (or is lane - 16's), or a row that saw nothing.
+    Kv4Query<D, C> qf;
+    kv4_load_query<D, C, RULES>(p, cur.b, cur.seg, group, cur.len, qf);
+    // Infinite: a column that is not there, or a row that saw nothing.
     float lse = INFINITY;
-    const uint32_t col = group * kv4_cols(L) + grp;
-    if (col < p.rows * p.group && grp < kv4_cols(L)) {
+    const uint32_t col = group * C + grp % C;
+    if (col < p.rows * p.group) {
       const float x = __ldg(p.lse_in + (size_t(cur.b) * p.rows + col / p.group) * p.q_heads + cur.seg * p.group +
                             col % p.group);
       if (x != -INFINITY) lse = RULES ? x : x * kLog2e;
@@ -1080,8 +1094,8 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
       const uint32_t tb = (RULES && j >= cur.head ? j + cur.skip : j) * kStageTokens;
       const uint8_t* slot = feed.ring + (done % SLOTS) * S::kSlot;
       const int32_t* pos = RULES ? kv4_positions(p, cur.b, cur.seg, cur.len, tb) : nullptr;
-      // After the reduction below this lane holds tokens 16 tig + 2 grp, + 1.
-      const uint32_t t0 = tb + 16 * tig + 2 * grp;
+      // After the reduction below this lane holds token t0 and the next.
+      const uint32_t t0 = tb + 16 * tig + (C == 8 ? 2 * grp : 8 * (grp >> 1 & 1) + 4 * (grp >> 2) + 2 * (grp & 1));
       const float old0 = t0 < cur.len ? weights[t0] : 0.f, old1 = t0 + 1 < cur.len ? weights[t0 + 1] : 0.f;
       const int got = mbar_wait_bounded(feed.bars + done % SLOTS, (done / SLOTS) & 1, abort_flag,
                                         kStatusFullWaitTimeout, int(done), p.wait_limit_ns);
@@ -1089,28 +1103,28 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
         failed = true;
         break;
       }
-      float w[16];
-      kv4_dots<D, L>(slot, qf.a, qf.start, w);
+      constexpr int kTokens = kv4_tokens(C);
+      float w[kTokens];
+      kv4_dots<D, C>(slot, qf, w);
       uint32_t seen;
       if (!RULES && int32_t(tb + kStageTokens) <= clear)
-        seen = kv4_scores<D, RULES, false>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope, qf.pos,
-                                           pos, w);
+        seen = kv4_scores<C, RULES, false>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos, w);
       else
-        seen = kv4_scores<D, RULES, true>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.dot, qf.sum, qf.slope, qf.pos,
-                                          pos, w);
+        seen = kv4_scores<C, RULES, true>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos, w);
       if (lse == INFINITY) seen = 0;
 #pragma unroll
-      for (int t = 0; t < 16; ++t) w[t] = seen >> t & 1u ? kv4_exp<RULES>(w[t], lse) : 0.f;
+      for (int u = 0; u < kTokens; ++u) w[u] = seen >> u & 1u ? kv4_exp<RULES>(w[u], lse) : 0.f;
       __syncwarp();  // every lane has read the slot
       if (done + SLOTS < count) {
         feed.copy(p);
         feed.lookup(p);
       }
-      // Sum over the eight columns (lanes grp), halving the tokens held at
-      // each step: lane grp ends with tokens 2 grp and 2 grp + 1.
+      // Sum over the columns (lanes grp % C), halving the tokens held at each
+      // step; two are left: with 8 columns tokens 2 grp and the next, with 4
+      // tokens 4 (grp / 4) + 8 (grp / 2 % 2) + 2 (grp % 2).
 #pragma unroll
-      for (int half = 8; half >= 2; half >>= 1) {
-        const uint32_t bit = 2 * half;  // lanes grp ^ (half / 2)
+      for (int half = kTokens / 2; half >= 2; half >>= 1) {
+        const uint32_t bit = 2 * half;
         const bool upper = lane & bit;
 #pragma unroll
         for (int t = 0; t < half; ++t) {
