@@ -193,7 +193,6 @@ kvb::Kv4AttendParams check_query(const Kv4Pool& pool, const Kv4Query& q) {
   prm.type = int32_t(q.type);
   const int64_t per = int64_t(16 / type_bytes(q.type));  // elements of a vector load
   prm.vector_q = aligned_to(q.q, 16) && q.batch_stride % per == 0 && q.row_stride % per == 0;
-  prm.wait_limit_ns = wait_limit_ns();
   prm.max_tokens = uint32_t(std::min<uint64_t>(q.max_tokens, uint64_t(q.table_stride) * pool.page_tokens));
   return prm;
 }
@@ -208,35 +207,23 @@ struct Kv4Kernel {
   uint32_t smem;
 };
 
-// Stage slots a warp and CTAs an SM. Dim 128: 12 warps an SM with two 9.1 KB
-// slots each, at most 168 registers.
-template <int D>
-struct Kv4Shape;
-template <>
-struct Kv4Shape<64> {
-  static constexpr int kSlots = 2, kCtas = 4, kWeighSlots = 4, kWeighCtas = 4;
-};
-template <>
-struct Kv4Shape<128> {
-  static constexpr int kSlots = 2, kCtas = 3, kWeighSlots = 3, kWeighCtas = 3;
-};
-template <>
-struct Kv4Shape<256> {
-  static constexpr int kSlots = 1, kCtas = 2, kWeighSlots = 2, kWeighCtas = 2;
-};
+// CTAs of 128 threads an SM, i.e. the register cap: 128 registers at four,
+// 168 at three, 255 at two.
+constexpr int attend_ctas(int dim, int cols, int digits, bool rules) {
+  return dim == 256 ? 2 : dim == 64 ? 4 : cols == 4 && digits == 2 && !rules ? 4 : 3;
+}
+constexpr int weigh_ctas(int dim, int cols, bool rules) { return dim == 256 ? 2 : dim == 64 || cols == 4 ? 4 : 3; }
 
 template <int D, int C, int PD, bool RULES>
 Kv4Kernel attend_kernel() {
-  using T = Kv4Shape<D>;
-  return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, C, PD, T::kSlots, T::kCtas, RULES>),
-          kvb::Kv4Smem<D, T::kSlots, true>::kBytes};
+  return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, C, PD, attend_ctas(D, C, PD, RULES), RULES>),
+          kvb::Kv4Smem<D, true>::kBytes};
 }
 
 template <int D, int C, bool RULES>
 Kv4Kernel weigh_kernel() {
-  using T = Kv4Shape<D>;
-  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, T::kWeighSlots, T::kWeighCtas, RULES>),
-          kvb::Kv4Smem<D, T::kWeighSlots, false>::kBytes};
+  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, weigh_ctas(D, C, RULES), RULES>),
+          kvb::Kv4Smem<D, false>::kBytes};
 }
 
 bool has_rules(const Kv4Pool& pool, const Kv4Query& q) {

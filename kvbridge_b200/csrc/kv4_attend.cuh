@@ -10,10 +10,13 @@
 // A windowed call leaves the stages between the prefix and the window out of
 // the list, so they are never read.
 //
-// Warps share nothing: each has its own ring of stage slots and its own
-// mbarriers, and refills a slot (a few lanes start one bulk copy each: K and V
-// codes, K and V params of a page) as soon as it has read it. No producer
-// warp, no empty barriers and no CTA barriers.
+// Warps share nothing: each has its own slot for K and for V (codes and
+// params) and refills one with 16-byte asynchronous copies as soon as it has
+// read it: the next K arrives while this stage's softmax and output run, the
+// next V while the next scores do. No producer warp and no barriers. (One bulk
+// copy per array and page instead of the eighteen 512-byte copy instructions
+// of a stage left the warps queueing for the bulk-copy unit: 0.7 of 3.2 us a
+// stage with 64-token pages, 2 of 5.6 us with 16-token pages.)
 //
 // Arithmetic (int8 tensor cores, exact s32 sums; codes 0..15 are int8
 // operands after a mask or a shift and a mask, two values a byte):
@@ -66,7 +69,6 @@ struct Kv4AttendParams {
   int32_t type;   // of q and out: 0 f32, 1 f16, 2 bf16
   bool vector_q;  // 16-byte aligned query rows
   bool direct;    // one warp per segment, nothing to merge
-  unsigned long long wait_limit_ns;
   // Partials of piece (warp w, segment i) in slot w + i: per column D sums and
   // {max, sum}; the first and last warp of every segment.
   float* part;
@@ -191,111 +193,110 @@ __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t w, uint32_t se
 }
 
 // ---------------------------------------------------------------------------
-// One warp's ring.
+// One warp's slots.
 
-// A slot: K codes, V codes (pages of 16 and 32 tokens 32 and 64 bytes further
-// apart, so that a quarter-warp's reads of several pages hit different
-// banks), K params, V params. V false: K alone.
-template <int D, int SLOTS, bool V>
+// K codes, K params, V codes (pages of 16 and 32 tokens 32 and 64 bytes
+// further apart), V params. The params of 16 tokens are 144 bytes apart. With
+// these gaps a quarter-warp's reads of four token groups or several pages hit
+// different banks. V false: K alone.
+constexpr uint32_t kKv4ParamPitch = 144;
+template <int D, bool V>
 struct Kv4Smem {
   static constexpr uint32_t kCodes = kStageTokens * D / 2;
-  static constexpr uint32_t kParams = kStageTokens * 8;
-  static constexpr uint32_t kOffV = kCodes;
-  static constexpr uint32_t kOffKp = kOffV + (V ? kCodes + 128 : 0);
-  static constexpr uint32_t kOffVp = kOffKp + kParams;
-  static constexpr uint32_t kSlot = kOffVp + (V ? kParams : 0);
-  static constexpr uint32_t kOffBars = kKv4Warps * SLOTS * kSlot;
-  static constexpr uint32_t kOffAbort = kOffBars + kKv4Warps * SLOTS * 8;
-  static constexpr uint32_t kBytes = kOffAbort + 16;
+  static constexpr uint32_t kParams = kStageTokens / 16 * kKv4ParamPitch;
+  static constexpr uint32_t kOffKp = kCodes;
+  static constexpr uint32_t kOffV = kOffKp + kParams;
+  static constexpr uint32_t kOffVp = kOffV + kCodes + 128;
+  static constexpr uint32_t kWarp = V ? kOffVp + kParams : kOffV;
+  static constexpr uint32_t kBytes = kKv4Warps * kWarp;
 };
 
 __device__ __forceinline__ uint32_t kv4_v_pitch(uint32_t page_bytes, uint32_t P) {
   return P == 64 ? page_bytes : page_bytes + 2 * P;
 }
 
-template <int D, int SLOTS, bool V, bool RULES>
+// 16 bytes global -> shared, asynchronously and past L1.
+__device__ __forceinline__ void copy16_async(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until all but the latest `N` committed groups of this thread have landed.
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <int D, bool V, bool RULES>
 struct Kv4Feeder {
-  uint8_t* ring;
-  uint64_t* bars;
-  uint64_t policy;
+  uint8_t* slots;
+  uint32_t addr;   // of slots, in shared memory
   Kv4Cursor cur;   // the segment of the next stage to look up
   uint32_t next;   // that stage, relative to the warp's first
   uint32_t count;  // stages of the warp
   uint32_t segs;
-  uint32_t used;   // slots filled so far
-  // This lane's copy of a stage: array lane / 4 (K codes, K params, V codes,
-  // V params) of page lane % 4.
-  const uint8_t* base;
-  uint32_t bytes, dst;
-  bool copies;
-  // The page looked up last: in flight until it is used.
+  // The page of the stage's 16-token group lane % 4, looked up last: in
+  // flight until it is used.
   uint32_t phys, head;
 
-  __device__ void init(const Kv4AttendParams& p, uint8_t* smem, uint32_t warp) {
-    using S = Kv4Smem<D, SLOTS, V>;
-    const uint32_t lane = threadIdx.x & 31, part = lane >> 2, q = lane & 3;
-    const uint32_t P = p.page_tokens, codes = P * (D / 2);
-    ring = smem + warp * SLOTS * S::kSlot;
-    bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars) + warp * SLOTS;
-    policy = l2_evict_first_policy();
-    copies = q < (kStageTokens >> p.log2_page) && part < (V ? 4u : 2u);
-    base = part == 0   ? p.pool.k
-           : part == 1 ? reinterpret_cast<const uint8_t*>(p.pool.kp)
-           : part == 2 ? p.pool.v
-                       : reinterpret_cast<const uint8_t*>(p.pool.vp);
-    bytes = part & 1 ? P * 8 : codes;
-    dst = part == 0 ? q * codes : part == 1 ? S::kOffKp + q * P * 8
-        : part == 2 ? S::kOffV + q * kv4_v_pitch(codes, P) : S::kOffVp + q * P * 8;
-    used = 0;
-    if (lane == 0) {
-      for (int i = 0; i < SLOTS; ++i) mbar_init(bars + i, 1);
-      fence_barrier_init();
-    }
-    __syncwarp();
+  __device__ void init(uint8_t* smem, uint32_t warp) {
+    slots = smem + warp * Kv4Smem<D, V>::kWarp;
+    addr = smem_addr(slots);
   }
 
-  // Starts the lookup of the page of stage `next`; kNoUnit where there is none.
+  // Starts the lookup of the pages of stage `next`; kNoUnit where there is none.
   __device__ __forceinline__ void lookup(const Kv4AttendParams& p) {
     phys = kNoUnit;
     if (next < count) {
       while (int32_t(next) >= cur.base + int32_t(cur.stages)) kv4_next_segment<RULES>(p, segs, cur);
       const uint32_t j = uint32_t(int32_t(next) - cur.base);
       const uint32_t stage = RULES && j >= cur.head ? j + cur.skip : j;
-      const uint32_t page = (stage << (6 - p.log2_page)) + (threadIdx.x & 3);
+      const uint32_t t = stage * kStageTokens + 16 * (threadIdx.x & 3);
       head = p.col_groups == 1 ? cur.seg : cur.seg / p.col_groups;
-      if (copies && (page << p.log2_page) < cur.len) phys = __ldg(p.table + size_t(cur.b) * p.table_stride + page);
+      const uint32_t page = t >> p.log2_page;  // all of it: V's quarters are not tokens
+      if ((page << p.log2_page) < cur.len) phys = __ldg(p.table + size_t(cur.b) * p.table_stride + page);
       ++next;
     }
   }
 
-  // Starts the copies of the stage looked up last into the next slot.
+  // Starts the copies of the K or the V of the stage looked up last: a quarter
+  // of the stage (of 1, 2 or 4 pages' codes) at a time.
+  template <bool OF_V, bool ALL>
+  __device__ __forceinline__ void copy_groups(const Kv4AttendParams& p, uint32_t unit) {
+    using S = Kv4Smem<D, V>;
+    const uint32_t lane = threadIdx.x & 31, log2_page = p.log2_page;
+    const uint32_t page_bytes = (D / 2) << log2_page, in_page = p.page_tokens - 1;
+    const uint8_t* codes = (OF_V ? p.pool.v : p.pool.k) + 16 * lane;
+    const uint32_t dst = addr + (OF_V ? S::kOffV : 0u) + 16 * lane;
+    const uint32_t gap = OF_V ? kv4_v_pitch(page_bytes, p.page_tokens) - page_bytes : 0u;
+#pragma unroll
+    for (uint32_t g = 0; g < 4; ++g) {
+      const uint32_t u = __shfl_sync(0xffffffffu, unit, g);
+      const uint8_t* src = codes + size_t(u) * page_bytes + (16 * g & in_page) * (D / 2);
+      if (ALL || u != kNoUnit)
+#pragma unroll
+        for (uint32_t i = 0; i < D / 64; ++i)
+          copy16_async(dst + g * (8 * D) + 512 * i + ((16 * g) >> log2_page) * gap, src + 512 * i);
+    }
+    // Tokens 2 lane and 2 lane + 1 of group lane / 8.
+    const uint32_t u = __shfl_sync(0xffffffffu, unit, lane >> 3);
+    if (ALL || u != kNoUnit)
+      copy16_async(addr + (OF_V ? S::kOffVp : S::kOffKp) + (lane >> 3) * kKv4ParamPitch + (lane & 7) * 16,
+                   reinterpret_cast<const uint8_t*>((OF_V ? p.pool.vp : p.pool.kp) + (size_t(u) << log2_page) +
+                                                    (2 * lane & in_page)));
+  }
+
+  template <bool OF_V>
   __device__ __forceinline__ void copy(const Kv4AttendParams& p) {
-    using S = Kv4Smem<D, SLOTS, V>;
-    const uint32_t slot = used % SLOTS;
-    ++used;
-    uint64_t* bar = bars + slot;
-    const bool ok = phys < p.pool.pages;  // lanes without a copy hold kNoUnit
-    if (!ok && phys != kNoUnit) atomicMax(&g_kvb_status, kKv4BadPage);
-    // Lanes 0 to 3 stand for the stage's pages.
-    const uint32_t pages = __popc(__ballot_sync(0xffffffffu, ok) & 0xfu);
-    const uint32_t page_bytes = p.page_tokens * (V ? D + 16 : D / 2 + 8);
-    if ((threadIdx.x & 31) == 0) mbar_arrive_expect_tx(bar, pages * page_bytes);
-    __syncwarp();
-    if (ok)
-      bulk_copy_g2s(ring + slot * S::kSlot + dst, base + (size_t(phys) * p.pool.kv_heads + head) * bytes, bytes, bar,
-                    policy);
+    const bool ok = phys < p.pool.pages;
+    if (!OF_V && !ok && phys != kNoUnit) atomicMax(&g_kvb_status, kKv4BadPage);
+    const uint32_t unit = ok ? phys * p.pool.kv_heads + head : kNoUnit;
+    if (__all_sync(0xffffffffu, ok))
+      copy_groups<OF_V, true>(p, unit);
+    else
+      copy_groups<OF_V, false>(p, unit);
+    copy_commit();
   }
 };
-
-// After a wait that gave up: lets the copies in flight (the last `ring` of
-// `used` fills of the slots) land, each for at most limit_ns.
-__device__ __forceinline__ void kv4_drain(uint64_t* bars, uint32_t ring, uint32_t used, unsigned long long limit_ns) {
-  for (uint32_t use = used > ring ? used - ring : 0; use < used; ++use) {
-    const unsigned long long start = global_ns();
-    while (!mbar_try_wait(bars + use % ring, (use / ring) & 1) && global_ns() - start < limit_ns) {
-    }
-  }
-}
 
 // ---------------------------------------------------------------------------
 // Queries.
@@ -472,6 +473,13 @@ __device__ __forceinline__ uint32_t kv4_first_token() {
   return 16 * (lane & 3) + (C == 4 ? 4 * (lane >> 4) : 0);
 }
 
+// Where the params of the thread's first token lie in a slot.
+template <int C>
+__device__ __forceinline__ uint32_t kv4_params_at() {
+  const uint32_t t = kv4_first_token<C>();
+  return (t >> 4) * kKv4ParamPitch + (t & 15) * 8;
+}
+
 template <int D, int C>
 __device__ __forceinline__ void kv4_dots(const uint8_t* codes, const Kv4Query<D, C>& qf, float (&sc)[kv4_tokens(C)]) {
   const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
@@ -556,7 +564,7 @@ __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const u
                                                const int32_t* pos, float (&sc)[kv4_tokens(C)]) {
   constexpr int kTokens = kv4_tokens(C);
   const uint32_t at = kv4_first_token<C>();
-  const float4* par = reinterpret_cast<const float4*>(params + 8 * at);
+  const float4* par = reinterpret_cast<const float4*>(params + kv4_params_at<C>());
   const int32_t t0 = int32_t(tb + at);
   uint32_t seen = (1u << kTokens) - 1;
   const float cap = p.rule.softcap, inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
@@ -634,7 +642,7 @@ __device__ __forceinline__ void kv4_softmax(const uint8_t* vparams, uint32_t see
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.o[j][e] *= alpha;
   }
-  const float4* par = reinterpret_cast<const float4*>(vparams + 8 * kv4_first_token<C>());
+  const float4* par = reinterpret_cast<const float4*>(vparams + kv4_params_at<C>());
 #pragma unroll
   for (int u = 0; u < kTokens; u += 2) {
     const float4 f = par[kv4_token(C, u) / 2];
@@ -806,15 +814,13 @@ __device__ __forceinline__ void kv4_report_lengths(const Kv4AttendParams& p) {
     if (__ldg(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
 }
 
-template <int D, int C, int PD, int SLOTS, int MINB, bool RULES>
+template <int D, int C, int PD, int MINB, bool RULES>
 __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4AttendParams p) {
-  using S = Kv4Smem<D, SLOTS, true>;
+  using S = Kv4Smem<D, true>;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = lane >> 2, tig = lane & 3;
-  int* abort_flag = reinterpret_cast<int*>(smem + S::kOffAbort) + warp;  // of this warp's waits
-  if (lane == 0) *abort_flag = 0;
-  Kv4Feeder<D, SLOTS, true, RULES> feed;
-  feed.init(p, smem, warp);
+  Kv4Feeder<D, true, RULES> feed;
+  feed.init(smem, warp);
   grid_launch_dependents();
   grid_dependency_wait();
 
@@ -830,14 +836,12 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
   feed.count = count;
   feed.segs = segs;
   feed.lookup(p);
-#pragma unroll
-  for (int i = 0; i < SLOTS; ++i)
-    if (uint32_t(i) < count) {
-      feed.copy(p);
-      feed.lookup(p);
-    }
+  if (count != 0) {
+    feed.template copy<false>(p);
+    feed.template copy<true>(p);
+    feed.lookup(p);
+  }
   uint32_t done = 0;
-  bool failed = false;
   const uint32_t vpitch = kv4_v_pitch(p.page_tokens * (D / 2), p.page_tokens);
 
   do {  // pieces
@@ -858,35 +862,38 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
     for (; done < end; ++done) {
       const uint32_t j = uint32_t(int32_t(done) - cur.base);
       const uint32_t tb = (RULES && j >= cur.head ? j + cur.skip : j) * kStageTokens;
-      const uint8_t* slot = feed.ring + (done % SLOTS) * S::kSlot;
       const int32_t* pos = RULES ? kv4_positions(p, cur.b, h, cur.len, tb) : nullptr;
-      const int got = mbar_wait_bounded(feed.bars + done % SLOTS, (done / SLOTS) & 1, abort_flag,
-                                        kStatusFullWaitTimeout, int(done), p.wait_limit_ns);
-      if (__any_sync(0xffffffffu, got != kWaitOk)) {
-        failed = true;
-        break;
-      }
+      copy_wait<1>();  // K has landed, V may be on its way
+      __syncwarp();
       float sc[kv4_tokens(C)];
-      uint32_t digit[kv4_p_tiles(PD)][2][4];
+      uint32_t digit[kv4_p_tiles(PD)][2][4], seen;
       float out_scale;
-      kv4_dots<D, C>(slot, qf, sc);
-      if (!RULES && int32_t(tb + kStageTokens) <= clear) {
-        const uint32_t seen = kv4_scores<C, RULES, false>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope,
-                                                          qf.pos, pos, sc);
-        kv4_softmax<D, C, PD, RULES, false>(slot + S::kOffVp, seen, sc, st, digit, out_scale);
-      } else {
-        const uint32_t seen = kv4_scores<C, RULES, true>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope,
-                                                         qf.pos, pos, sc);
-        kv4_softmax<D, C, PD, RULES, true>(slot + S::kOffVp, seen, sc, st, digit, out_scale);
-      }
-      kv4_output<D, PD>(slot + S::kOffV, p.page_tokens, vpitch, digit, out_scale, st);
-      __syncwarp();  // every lane has read the slot
-      if (done + SLOTS < count) {
-        feed.copy(p);
+      kv4_dots<D, C>(feed.slots, qf, sc);
+      const bool clean = !RULES && int32_t(tb + kStageTokens) <= clear;
+      if (clean)
+        seen = kv4_scores<C, RULES, false>(p, feed.slots + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos,
+                                           sc);
+      else
+        seen = kv4_scores<C, RULES, true>(p, feed.slots + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos,
+                                          sc);
+      __syncwarp();  // every lane has read K
+      if (done + 1 < count)
+        feed.template copy<false>(p);
+      else
+        copy_commit();  // an empty group: the waits count groups
+      copy_wait<1>();   // V has landed
+      __syncwarp();
+      if (clean)
+        kv4_softmax<D, C, PD, RULES, false>(feed.slots + S::kOffVp, seen, sc, st, digit, out_scale);
+      else
+        kv4_softmax<D, C, PD, RULES, true>(feed.slots + S::kOffVp, seen, sc, st, digit, out_scale);
+      kv4_output<D, PD>(feed.slots + S::kOffV, p.page_tokens, vpitch, digit, out_scale, st);
+      __syncwarp();  // every lane has read V
+      if (done + 1 < count) {
+        feed.template copy<true>(p);
         feed.lookup(p);
       }
     }
-    if (failed) break;
 
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
@@ -927,9 +934,6 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
     }
     if (done < count) kv4_next_segment<RULES>(p, segs, cur);
   } while (done < count);
-
-  // A wait that gave up leaves copies in flight.
-  if (failed) kv4_drain(feed.bars, SLOTS, feed.used, p.wait_limit_ns);
 }
 
 // The partials of one output row (sequence, row, head). Bound by latency: a
@@ -1043,15 +1047,13 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv
 // one thread adds up a token's weight in a fixed order, so there are no
 // atomics, and the groups' launches follow one another.
 
-template <int D, int C, int SLOTS, int MINB, bool RULES>
+template <int D, int C, int MINB, bool RULES>
 __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4AttendParams p, uint32_t group) {
-  using S = Kv4Smem<D, SLOTS, false>;
+  using S = Kv4Smem<D, false>;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = lane >> 2, tig = lane & 3;
-  int* abort_flag = reinterpret_cast<int*>(smem + S::kOffAbort) + warp;
-  if (lane == 0) *abort_flag = 0;
-  Kv4Feeder<D, SLOTS, false, RULES> feed;
-  feed.init(p, smem, warp);
+  Kv4Feeder<D, false, RULES> feed;
+  feed.init(smem, warp);
   grid_launch_dependents();
   grid_dependency_wait();
 
@@ -1065,16 +1067,11 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
   feed.count = count;
   feed.segs = segs;
   feed.lookup(p);
-#pragma unroll
-  for (int i = 0; i < SLOTS; ++i)
-    if (uint32_t(i) < count) {
-      feed.copy(p);
-      feed.lookup(p);
-    }
+  feed.template copy<false>(p);
+  feed.lookup(p);
   uint32_t done = 0;
-  bool failed = false;
 
-  while (done < count && !failed) {
+  while (done < count) {
     const uint32_t end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
     Kv4Query<D, C> qf;
     kv4_load_query<D, C, RULES>(p, cur.b, cur.seg, group, cur.len, qf);
@@ -1092,33 +1089,28 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
     for (; done < end; ++done) {
       const uint32_t j = uint32_t(int32_t(done) - cur.base);
       const uint32_t tb = (RULES && j >= cur.head ? j + cur.skip : j) * kStageTokens;
-      const uint8_t* slot = feed.ring + (done % SLOTS) * S::kSlot;
       const int32_t* pos = RULES ? kv4_positions(p, cur.b, cur.seg, cur.len, tb) : nullptr;
       // After the reduction below this lane holds token t0 and the next.
       const uint32_t t0 = tb + 16 * tig + (C == 8 ? 2 * grp : 8 * (grp >> 1 & 1) + 4 * (grp >> 2) + 2 * (grp & 1));
       const float old0 = t0 < cur.len ? weights[t0] : 0.f, old1 = t0 + 1 < cur.len ? weights[t0 + 1] : 0.f;
-      const int got = mbar_wait_bounded(feed.bars + done % SLOTS, (done / SLOTS) & 1, abort_flag,
-                                        kStatusFullWaitTimeout, int(done), p.wait_limit_ns);
-      if (__any_sync(0xffffffffu, got != kWaitOk)) {
-        failed = true;
-        break;
-      }
+      copy_wait<0>();
+      __syncwarp();
       constexpr int kTokens = kv4_tokens(C);
       float w[kTokens];
-      kv4_dots<D, C>(slot, qf, w);
+      kv4_dots<D, C>(feed.slots, qf, w);
       uint32_t seen;
       if (!RULES && int32_t(tb + kStageTokens) <= clear)
-        seen = kv4_scores<C, RULES, false>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos, w);
+        seen = kv4_scores<C, RULES, false>(p, feed.slots + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos, w);
       else
-        seen = kv4_scores<C, RULES, true>(p, slot + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos, w);
+        seen = kv4_scores<C, RULES, true>(p, feed.slots + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos, w);
+      __syncwarp();  // every lane has read K
+      if (done + 1 < count) {
+        feed.template copy<false>(p);
+        feed.lookup(p);
+      }
       if (lse == INFINITY) seen = 0;
 #pragma unroll
       for (int u = 0; u < kTokens; ++u) w[u] = seen >> u & 1u ? kv4_exp<RULES>(w[u], lse) : 0.f;
-      __syncwarp();  // every lane has read the slot
-      if (done + SLOTS < count) {
-        feed.copy(p);
-        feed.lookup(p);
-      }
       // Sum over the columns (lanes grp % C), halving the tokens held at each
       // step; two are left: with 8 columns tokens 2 grp and the next, with 4
       // tokens 4 (grp / 4) + 8 (grp / 2 % 2) + 2 (grp % 2).
@@ -1138,7 +1130,6 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
     }
     if (done < count) kv4_next_segment<RULES>(p, segs, cur);
   }
-  if (failed) kv4_drain(feed.bars, SLOTS, feed.used, p.wait_limit_ns);
 }
 
 }  // namespace kvb
