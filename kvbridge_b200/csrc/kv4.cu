@@ -208,21 +208,21 @@ struct Kv4Kernel {
 };
 
 // CTAs of 128 threads an SM, i.e. the register cap: 128 registers at four,
-// 168 at three, 255 at two.
-constexpr int attend_ctas(int dim, int cols, int digits, bool rules) {
-  return dim == 256 ? 2 : dim == 64 ? 4 : cols == 4 && digits == 2 && !rules ? 4 : 3;
-}
-constexpr int weigh_ctas(int dim, int cols, bool rules) { return dim == 256 ? 2 : dim == 64 || cols == 4 ? 4 : 3; }
+// 168 at three, 255 at two. (Dim 128, 8 columns: three CTAs 83 us for 16x16K
+// tokens, four 94 us with 160 bytes of spills; 4 columns: 1x64K 26.6 us at
+// three, 28.0 us at four.)
+constexpr int attend_ctas(int dim) { return dim == 256 ? 2 : dim == 64 ? 4 : 3; }
+constexpr int weigh_ctas(int dim, int cols) { return dim == 256 ? 2 : dim == 64 || cols == 4 ? 4 : 3; }
 
 template <int D, int C, int PD, bool RULES>
 Kv4Kernel attend_kernel() {
-  return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, C, PD, attend_ctas(D, C, PD, RULES), RULES>),
+  return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, C, PD, attend_ctas(D), RULES>),
           kvb::Kv4Smem<D, true>::kBytes};
 }
 
 template <int D, int C, bool RULES>
 Kv4Kernel weigh_kernel() {
-  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, weigh_ctas(D, C, RULES), RULES>),
+  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, weigh_ctas(D, C), RULES>),
           kvb::Kv4Smem<D, false>::kBytes};
 }
 
@@ -312,7 +312,8 @@ AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
   }
   a.ctas = split_ctas(a.kernel, a.segments, q.max_tokens);
   a.workers = a.ctas * kvb::kKv4Warps;
-  a.many = a.workers > 8 * a.segments;
+  // A warp reads 32 partials a round; from about 24 on a CTA a row is faster.
+  a.many = a.workers > 24 * a.segments;
   const size_t slots = size_t(a.workers) + a.segments;
   a.ml_offset = slots * cols * pool.dim * sizeof(float);
   a.warps_offset = a.ml_offset + slots * cols * sizeof(float2);

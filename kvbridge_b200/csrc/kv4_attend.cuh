@@ -554,47 +554,65 @@ __device__ __forceinline__ float kv4_exp(float x, float y) {
   return fast_exp2(RULES ? (x - y) * kLog2e : x - y);
 }
 
+// Which tokens of the stage at tb every query row sees, by their indices:
+// those below the first row's position (and below the prefix), if they are
+// within the last row's window. A warp-uniform test that spares most stages
+// the masks. first, last: the rows' positions.
+template <bool RULES>
+__device__ __forceinline__ bool kv4_all_visible(const Kv4AttendParams& p, uint32_t tb, uint32_t len, uint32_t prefix) {
+  const int32_t first = int32_t(len) - int32_t(p.rows), end = int32_t(tb + kStageTokens);
+  if (!RULES) return end <= first + 1;
+  if (p.rule.q_pos != nullptr) return false;
+  if (uint32_t(end) <= min(prefix, len)) return true;
+  return end <= first + 1 && (p.rule.window == 0 || uint32_t(int32_t(len) - 1 - int32_t(tb)) < p.rule.window);
+}
+
 // Scores from the dot products; invisible ones -inf. Returns the thread's
-// visible tokens as a bit mask (all ones where MASK is false). tb: the stage's
-// first token; pos: the positions of the thread's quad's 16 tokens, or null
-// for their indices.
-template <int C, bool RULES, bool MASK>
+// visible tokens as a bit mask. tb: the stage's first token; all: every token
+// is visible; pos: the positions of the thread's quad's 16 tokens, or null for
+// their indices.
+template <int C, bool RULES>
 __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const uint8_t* params, uint32_t tb,
-                                               uint32_t len, uint32_t prefix, float sum, float slope, int32_t pq,
-                                               const int32_t* pos, float (&sc)[kv4_tokens(C)]) {
+                                               uint32_t len, uint32_t prefix, bool all, float sum, float slope,
+                                               int32_t pq, const int32_t* pos, float (&sc)[kv4_tokens(C)]) {
   constexpr int kTokens = kv4_tokens(C);
   const uint32_t at = kv4_first_token<C>();
   const float4* par = reinterpret_cast<const float4*>(params + kv4_params_at<C>());
-  const int32_t t0 = int32_t(tb + at);
-  uint32_t seen = (1u << kTokens) - 1;
-  const float cap = p.rule.softcap, inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
-  if (RULES) seen = 0;
 #pragma unroll
   for (int u = 0; u < kTokens; u += 2) {
     const float4 f = par[kv4_token(C, u) / 2];
     sc[u] = fmaf(sc[u], f.x, fmaf(8.f, f.x, f.y) * sum);
     sc[u + 1] = fmaf(sc[u + 1], f.z, fmaf(8.f, f.z, f.w) * sum);
-    if constexpr (RULES) {
+  }
+  const int32_t t0 = int32_t(tb + at);
+  int32_t pk[RULES ? kTokens : 1];
+  if constexpr (RULES) {
+    if (p.rule.softcap > 0.f) {
+      const float cap = p.rule.softcap, inv_cap = 1.0f / cap;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int32_t token = int32_t(kv4_token(C, u + e));
-        const int32_t pk = pos != nullptr ? __ldg(pos + (at & 15) + token) : t0 + token;
-        float x = sc[u + e];
-        if (cap > 0.f) x = kv4_cap(x, cap, inv_cap);
-        // exact below 2^24; |pq - pk| as the larger minus the smaller
-        const uint32_t away = pq >= pk ? uint32_t(pq) - uint32_t(pk) : uint32_t(pk) - uint32_t(pq);
-        x = fmaf(-slope, float(away), x);
-        const bool on = uint32_t(t0 + token) < len && kv4_visible(pk, pq, p.rule.window, prefix);
-        sc[u + e] = on ? x : -INFINITY;
-        seen |= on ? 1u << (u + e) : 0u;
-      }
+      for (int u = 0; u < kTokens; ++u) sc[u] = kv4_cap(sc[u], cap, inv_cap);
+    }
+    if (pos != nullptr) {
+#pragma unroll
+      for (int u = 0; u < kTokens; ++u) pk[u] = __ldg(pos + (at & 15) + kv4_token(C, u));
+    } else {
+#pragma unroll
+      for (int u = 0; u < kTokens; ++u) pk[u] = t0 + int32_t(kv4_token(C, u));
+    }
+    if (p.rule.slopes != nullptr) {
+      // Distances are exact in fp32 below 2^24; |pq - pk| as the larger minus the smaller.
+#pragma unroll
+      for (int u = 0; u < kTokens; ++u)
+        sc[u] = fmaf(-slope, float(uint32_t(max(pq, pk[u])) - uint32_t(min(pq, pk[u]))), sc[u]);
     }
   }
-  if (!RULES && MASK) {
+  uint32_t seen = (1u << kTokens) - 1;
+  if (!all) {
     seen = 0;
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
-      const bool on = t0 + int32_t(kv4_token(C, u)) <= pq;  // pq < len
+      const int32_t t = t0 + int32_t(kv4_token(C, u));
+      const bool on = RULES ? uint32_t(t) < len && kv4_visible(pk[u], pq, p.rule.window, prefix) : t <= pq;  // pq < len
       sc[u] = on ? sc[u] : -INFINITY;
       seen |= on ? 1u << u : 0u;
     }
@@ -850,8 +868,6 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
     Kv4Query<D, C> qf;
     kv4_load_query<D, C, RULES>(p, cur.b, h, cur.seg % p.col_groups, cur.len, qf);
     const uint32_t prefix = RULES && p.rule.prefix != nullptr ? __ldg(p.rule.prefix + cur.b) : 0u;
-    // Tokens below this are visible to every row (no rules).
-    const int32_t clear = int32_t(cur.len) - int32_t(p.rows) + 1;
     Kv4State<D> st;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
@@ -869,21 +885,12 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
       uint32_t digit[kv4_p_tiles(PD)][2][4], seen;
       float out_scale;
       kv4_dots<D, C>(feed.slots, qf, sc);
-      const bool clean = !RULES && int32_t(tb + kStageTokens) <= clear;
-      if (clean)
-        seen = kv4_scores<C, RULES, false>(p, feed.slots + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos,
-                                           sc);
-      else
-        seen = kv4_scores<C, RULES, true>(p, feed.slots + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos,
-                                          sc);
-      __syncwarp();  // every lane has read K
-      if (done + 1 < count)
-        feed.template copy<false>(p);
-      else
-        copy_commit();  // an empty group: the waits count groups
-      copy_wait<1>();   // V has landed
-      __syncwarp();
-      if (clean)
+      const bool all = kv4_all_visible<RULES>(p, tb, cur.len, prefix);
+      seen = kv4_scores<C, RULES>(p, feed.slots + S::kOffKp, tb, cur.len, prefix, all, qf.sum, qf.slope, qf.pos, pos, sc);
+      copy_wait<0>();  // V has landed
+      __syncwarp();    // and every lane has read K
+      if (done + 1 < count) feed.template copy<false>(p);
+      if (all)
         kv4_softmax<D, C, PD, RULES, false>(feed.slots + S::kOffVp, seen, sc, st, digit, out_scale);
       else
         kv4_softmax<D, C, PD, RULES, true>(feed.slots + S::kOffVp, seen, sc, st, digit, out_scale);
@@ -1084,7 +1091,6 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
       if (x != -INFINITY) lse = RULES ? x : x * kLog2e;
     }
     const uint32_t prefix = RULES && p.rule.prefix != nullptr ? __ldg(p.rule.prefix + cur.b) : 0u;
-    const int32_t clear = int32_t(cur.len) - int32_t(p.rows) + 1;
     float* weights = p.weights + (int64_t(cur.b) * p.pool.kv_heads + cur.seg) * p.weight_stride;
     for (; done < end; ++done) {
       const uint32_t j = uint32_t(int32_t(done) - cur.base);
@@ -1098,11 +1104,8 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
       constexpr int kTokens = kv4_tokens(C);
       float w[kTokens];
       kv4_dots<D, C>(feed.slots, qf, w);
-      uint32_t seen;
-      if (!RULES && int32_t(tb + kStageTokens) <= clear)
-        seen = kv4_scores<C, RULES, false>(p, feed.slots + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos, w);
-      else
-        seen = kv4_scores<C, RULES, true>(p, feed.slots + S::kOffKp, tb, cur.len, prefix, qf.sum, qf.slope, qf.pos, pos, w);
+      uint32_t seen = kv4_scores<C, RULES>(p, feed.slots + S::kOffKp, tb, cur.len, prefix,
+                                  kv4_all_visible<RULES>(p, tb, cur.len, prefix), qf.sum, qf.slope, qf.pos, pos, w);
       __syncwarp();  // every lane has read K
       if (done + 1 < count) {
         feed.template copy<false>(p);
