@@ -48,6 +48,8 @@ kvb::Kv4View view(const Kv4Pool& p) {
                       reinterpret_cast<float2*>(p.v_params), p.positions, p.kv_heads, p.pages};
 }
 
+uint32_t log2_page(const Kv4Pool& p) { return p.page_tokens == 64 ? 6 : p.page_tokens == 32 ? 5 : 4; }
+
 // Calls f(integral_constant<int, D>) with the pool's head dim.
 template <class F>
 auto by_dim(uint32_t dim, F&& f) {
@@ -104,16 +106,37 @@ bool check_rows(const Kv4Pool& pool, const Kv4Rows& rows) {
 }
 
 kvb::Kv4RowsParams rows_params(const Kv4Pool& pool, const Kv4Rows& rows) {
-  return kvb::Kv4RowsParams{view(pool),     rows.k,     rows.v,         rows.k_stride,
-                            rows.v_stride,  rows.slots, rows.positions, rows.tokens,
-                            uint64_t(pool.pages) * pool.page_tokens};
+  const int64_t per = int64_t(16 / type_bytes(rows.type));  // elements of a vector access
+  const bool vector = aligned_to(rows.k, 16) && aligned_to(rows.v, 16) && rows.k_stride % per == 0 &&
+                      rows.v_stride % per == 0;
+  return kvb::Kv4RowsParams{view(pool),
+                            rows.k,
+                            rows.v,
+                            rows.k_stride,
+                            rows.v_stride,
+                            rows.slots,
+                            rows.positions,
+                            rows.tokens,
+                            pool.page_tokens,
+                            log2_page(pool),
+                            uint64_t(pool.pages) * pool.page_tokens,
+                            vector};
 }
 
-uint32_t row_blocks(const Kv4Pool& pool, const Kv4Rows& rows) {
-  const uint64_t warps = uint64_t(rows.tokens) * pool.kv_heads * 2;
-  const uint64_t blocks = (warps + kvb::kKv4RowWarps - 1) / kvb::kKv4RowWarps;
-  if (blocks > 0x7fffffffull) throw std::invalid_argument("kv4 rows call too large for one grid");
-  return uint32_t(blocks);
+// Tokens a CTA: 64, or 16 where that would leave SMs without one.
+bool small_tiles(const Kv4Pool& pool, const Kv4Rows& rows) {
+  return uint64_t((rows.tokens + 63) / 64) * pool.kv_heads < uint64_t(2 * detail::device_sms());
+}
+
+template <class Kernel>
+void launch_rows(const Kv4Pool& pool, const Kv4Rows& rows, cudaStream_t stream, const char* what, Kernel&& kernel) {
+  kvb::Kv4RowsParams prm = rows_params(pool, rows);
+  const bool small = small_tiles(pool, rows);
+  const uint32_t tile = small ? 16 : 64;
+  const void* fn = by_dim(pool.dim, [&](auto d) { return by_type(rows.type, [&](auto t) { return kernel(d, t, small); }); });
+  void* args[] = {&prm};
+  launch_kernel_pdl(fn, dim3((rows.tokens + tile - 1) / tile, pool.kv_heads), dim3(32 * kvb::kKv4StoreWarps), 0, stream,
+                    args, what);
 }
 
 }  // namespace
@@ -122,24 +145,22 @@ void append_kv4(const Kv4Pool& pool, const Kv4Rows& rows, cudaStream_t stream) {
   if (!check_rows(pool, rows)) return;
   if (pool.positions != nullptr && rows.positions == nullptr)
     throw std::invalid_argument("the pool keeps positions: append_kv4 needs the rows' positions");
-  const void* fn = by_dim(pool.dim, [&](auto d) {
-    return by_type(rows.type, [&](auto t) {
-      return reinterpret_cast<const void*>(&kvb::append_kv4_rows_kernel<decltype(t), decltype(d)::value>);
-    });
+  launch_rows(pool, rows, stream, "kv4 append launch", [](auto d, auto t, bool small) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    return small ? reinterpret_cast<const void*>(&kvb::append_kv4_kernel<T, D, 16>)
+                 : reinterpret_cast<const void*>(&kvb::append_kv4_kernel<T, D, 64>);
   });
-  launch(fn, dim3(row_blocks(pool, rows)), 32 * kvb::kKv4RowWarps, 0, stream, rows_params(pool, rows),
-         pool.page_tokens, "kv4 append launch");
 }
 
 void load_kv4(const Kv4Pool& pool, const Kv4Rows& rows, cudaStream_t stream) {
   if (!check_rows(pool, rows)) return;
-  const void* fn = by_dim(pool.dim, [&](auto d) {
-    return by_type(rows.type, [&](auto t) {
-      return reinterpret_cast<const void*>(&kvb::load_kv4_rows_kernel<decltype(t), decltype(d)::value>);
-    });
+  launch_rows(pool, rows, stream, "kv4 load launch", [](auto d, auto t, bool small) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    return small ? reinterpret_cast<const void*>(&kvb::load_kv4_kernel<T, D, 16>)
+                 : reinterpret_cast<const void*>(&kvb::load_kv4_kernel<T, D, 64>);
   });
-  launch(fn, dim3(row_blocks(pool, rows)), 32 * kvb::kKv4RowWarps, 0, stream, rows_params(pool, rows),
-         pool.page_tokens, "kv4 load launch");
 }
 
 // ---------------------------------------------------------------------------
@@ -189,7 +210,7 @@ kvb::Kv4AttendParams check_query(const Kv4Pool& pool, const Kv4Query& q) {
   prm.group = q.q_heads / pool.kv_heads;
   prm.table_stride = q.table_stride;
   prm.page_tokens = pool.page_tokens;
-  prm.log2_page = pool.page_tokens == 64 ? 6 : pool.page_tokens == 32 ? 5 : 4;
+  prm.log2_page = log2_page(pool);
   prm.type = int32_t(q.type);
   const int64_t per = int64_t(16 / type_bytes(q.type));  // elements of a vector load
   prm.vector_q = aligned_to(q.q, 16) && q.batch_stride % per == 0 && q.row_stride % per == 0;
