@@ -92,18 +92,21 @@ uint32_t take_skip_stage() {
 std::atomic<unsigned long long> g_wait_limit_ns{kvb::kDefaultWaitLimitNs};
 
 void launch_pdl(const void* fn, dim3 grid, dim3 block, uint32_t smem, cudaStream_t stream,
-                void** args, const char* what) {
+                void** args, const char* what, uint32_t cluster = 1) {
   if (const cudaError_t injected = injected_launch_failure()) cuda_ok(injected, what);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   cuda_ok(cudaLaunchKernelExC(&cfg, fn, args), what);
 }
 
@@ -1128,6 +1131,11 @@ namespace detail {
 void launch_kernel_pdl(const void* fn, dim3 grid, dim3 block, uint32_t smem, cudaStream_t stream,
                        void** args, const char* what) {
   launch_pdl(fn, grid, block, smem, stream, args, what);
+}
+
+void launch_kernel_cluster(const void* fn, dim3 grid, dim3 block, uint32_t cluster, uint32_t smem, cudaStream_t stream,
+                           void** args, const char* what) {
+  launch_pdl(fn, grid, block, smem, stream, args, what, cluster);
 }
 
 int device_sms() { return current_device_facts().sms; }

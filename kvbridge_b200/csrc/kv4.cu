@@ -66,13 +66,6 @@ auto by_type(Kv4Type type, F&& f) {
   return f(__nv_bfloat16{});
 }
 
-template <class P>
-void launch(const void* fn, dim3 grid, uint32_t threads, uint32_t smem, cudaStream_t stream, P prm,
-            uint32_t page_tokens, const char* what) {
-  void* args[] = {&prm, &page_tokens};
-  launch_kernel_pdl(fn, grid, dim3(threads), smem, stream, args, what);
-}
-
 }  // namespace
 
 const char* kv4_pool_error(const Kv4Pool& p) noexcept {
@@ -276,7 +269,7 @@ Kv4Kernel weigh_kernel(uint32_t dim, uint32_t cols) {
 
 // CTAs of a kernel that the current device holds at once. The first use on a
 // device also raises the kernel's shared-memory limit.
-uint32_t resident_ctas(const Kv4Kernel& k) {
+uint32_t resident_ctas(const Kv4Kernel& k, int threads = kvb::kKv4Threads) {
   static std::mutex mu;
   static std::map<std::pair<int, const void*>, uint32_t> cache;
   int dev = 0;
@@ -291,7 +284,7 @@ uint32_t resident_ctas(const Kv4Kernel& k) {
                                int(cudaSharedmemCarveoutMaxShared)),
           "kv4 kernel carveout");
   int blocks = 0;
-  cuda_ok(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k.fn, kvb::kKv4Threads, k.smem), "occupancy query");
+  cuda_ok(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k.fn, threads, k.smem), "occupancy query");
   const uint32_t ctas = uint32_t(std::max(blocks, 1) * detail::device_sms());
   cache.emplace(key, ctas);
   return ctas;
@@ -439,9 +432,20 @@ void select_tokens(const Kv4Eviction& e, int32_t* keep, uint32_t* kept_lens, cud
     throw std::invalid_argument("keep and kept_lens must be 4-byte aligned");
   kvb::SelectParams prm{e.seq_lens, e.weights,    e.weight_stride, keep,    kept_lens, e.batch,
                         e.kv_heads, e.max_tokens, e.budget,        e.sinks, e.recent};
+  // CTAs a segment: one for every 2,048 tokens, at most the eight of a
+  // portable cluster, and no more than fill the SMs twice (16 x 16K tokens on
+  // 8 heads: 90 us in clusters of eight, whose shared histograms queue).
+  uint32_t ctas = 1;
+  while (ctas < 8 && uint64_t(ctas) * 2048 < e.max_tokens &&
+         uint64_t(e.batch) * e.kv_heads * ctas * 2 <= uint64_t(2 * detail::device_sms()))
+    ctas *= 2;
+  const uint32_t part = (e.max_tokens + ctas - 1) / ctas;
+  const uint32_t smem = std::min(part, kvb::kSelectKeys) * uint32_t(sizeof(uint32_t));
+  const Kv4Kernel k{reinterpret_cast<const void*>(&kvb::select_tokens_kernel), kvb::kSelectKeys * uint32_t(sizeof(uint32_t))};
+  resident_ctas(k, kvb::kSelectThreads);
   void* args[] = {&prm};
-  launch_kernel_pdl(reinterpret_cast<const void*>(&kvb::select_tokens_kernel), dim3(e.batch * e.kv_heads),
-                    dim3(kvb::kSelectThreads), 0, stream, args, "token selection launch");
+  detail::launch_kernel_cluster(k.fn, dim3(e.batch * e.kv_heads * ctas), dim3(kvb::kSelectThreads), ctas, smem, stream, args,
+                                "token selection launch");
 }
 
 void compact_kv4(const Kv4Pool& pool, const Kv4Eviction& e, const uint32_t* block_table,
@@ -462,14 +466,16 @@ void compact_kv4(const Kv4Pool& pool, const Kv4Eviction& e, const uint32_t* bloc
     throw std::invalid_argument("budget exceeds the new block-table row capacity");
   if (new_weights != nullptr && new_weight_stride < int64_t(e.budget))
     throw std::invalid_argument("new_weight_stride must be at least budget");
-  const uint32_t pages = (e.budget + pool.page_tokens - 1) / pool.page_tokens;
-  kvb::CompactParams prm{view(pool), e.seq_lens, e.weights,   e.weight_stride,   block_table,
-                         keep,       new_table,  new_weights, new_weight_stride, e.batch,
-                         e.max_tokens, e.budget, table_stride, new_stride};
+  kvb::CompactParams prm{view(pool),   e.seq_lens,   e.weights,   e.weight_stride,   block_table,
+                         keep,         new_table,    new_weights, new_weight_stride, e.batch,
+                         e.max_tokens, e.budget,     table_stride, new_stride,       pool.page_tokens,
+                         log2_page(pool)};
   const void* fn = by_dim(pool.dim, [&](auto d) {
     return reinterpret_cast<const void*>(&kvb::compact_kv4_kernel<decltype(d)::value>);
   });
-  launch(fn, dim3(pages, e.kv_heads, e.batch), 128, 0, stream, prm, pool.page_tokens, "kv4 compaction launch");
+  void* args[] = {&prm};
+  launch_kernel_pdl(fn, dim3((e.budget + kvb::kCompactTile - 1) / kvb::kCompactTile, e.kv_heads, e.batch),
+                    dim3(kvb::kCompactThreads), 0, stream, args, "kv4 compaction launch");
 }
 
 // ---------------------------------------------------------------------------

@@ -215,17 +215,6 @@ __device__ __forceinline__ uint32_t kv4_v_pitch(uint32_t page_bytes, uint32_t P)
   return P == 64 ? page_bytes : page_bytes + 2 * P;
 }
 
-// 16 bytes global -> shared, asynchronously and past L1.
-__device__ __forceinline__ void copy16_async(uint32_t dst, const uint8_t* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Until all but the latest `N` committed groups of this thread have landed.
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 template <int D, bool V, bool RULES>
 struct Kv4Feeder {
   uint8_t* slots;

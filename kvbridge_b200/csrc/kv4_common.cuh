@@ -66,4 +66,15 @@ __device__ __forceinline__ T from_f32(float x) {
   else return __float2bfloat16_rn(x);
 }
 
+// 16 bytes global -> shared, asynchronously and past L1.
+__device__ __forceinline__ void copy16_async(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until all but the latest `N` committed groups of this thread have landed.
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 }  // namespace kvb

@@ -10,6 +10,10 @@ namespace kvbridge::detail {
 void launch_kernel_pdl(const void* fn, dim3 grid, dim3 block, uint32_t smem, cudaStream_t stream,
                        void** args, const char* what);
 
+// The same in clusters of `cluster` consecutive CTAs (at most 8).
+void launch_kernel_cluster(const void* fn, dim3 grid, dim3 block, uint32_t cluster, uint32_t smem, cudaStream_t stream,
+                           void** args, const char* what);
+
 // SM count of the current device (cached per device).
 int device_sms();
 

@@ -23,15 +23,24 @@ TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 def _tensor(name: str, x, dtype, shape=None, like=None) -> int:
-    """Address of a contiguous CUDA tensor of this dtype (and shape)."""
+    """Address of a contiguous CUDA tensor of this dtype (and shape, a tuple)."""
+    try:
+        if (
+            x.dtype is dtype
+            and x.is_cuda
+            and (shape is None or x.shape == shape)
+            and (like is None or x.device == like)
+            and x.is_contiguous()
+        ):
+            return x.data_ptr()
+    except AttributeError:
+        pass
     _device(name, x, like)
     if x.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {x.dtype}")
-    if shape is not None and tuple(x.shape) != tuple(shape):
+    if shape is not None and x.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(x.shape)}")
-    if not x.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return x.data_ptr()
+    raise ValueError(f"{name} must be contiguous")
 
 
 def _device(name: str, x, like=None) -> None:
@@ -55,11 +64,18 @@ def _strides(name: str, x, inner: int) -> tuple:
     return x.stride()[:-inner]
 
 
+# The stream's handle without a Stream object around it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream
+)
+
+
 def _stream(stream, device) -> Optional[int]:
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         raise ValueError(f"the buffers are on {device}, the current device is cuda:{torch.cuda.current_device()}")
     if stream is None:
-        stream = torch.cuda.current_stream(device)
+        return _raw_stream(index) or None
     if not isinstance(stream, int):
         stream = stream.cuda_stream
     return stream or None
@@ -173,7 +189,8 @@ class Kv4Query:
             raise ValueError("q_heads must be divisible by kv_heads")
         if not 0 <= window < 1 << 32 or not 0 <= max_tokens < 1 << 31:
             raise ValueError("window and max_tokens must not be negative")
-        self.q, self.dtype, self.shape, self.kv_heads = q, q.dtype, tuple(q.shape), kv_heads
+        self.q, self.dtype, self.shape, self.kv_heads = q, q.dtype, q.shape, kv_heads
+        self.lse_shape = q.shape[:3]
         self.max_tokens = max_tokens
         self._kept = (seq_lens, block_table, slopes, prefix_lens, q_positions)
         strides = _strides("q", q, 2)
@@ -211,7 +228,7 @@ def launch_attention_kv4(pool: Kv4Pool, query: Kv4Query, workspace, out, lse=Non
         _lib.load().kvb_launch_attention_kv4(
             pool._ref, query._ref, _tensor("workspace", workspace, torch.uint8, None, pool.device), workspace.numel(),
             _tensor("out", out, query.dtype, query.shape, pool.device),
-            None if lse is None else _tensor("lse", lse, torch.float32, query.shape[:3], pool.device),
+            None if lse is None else _tensor("lse", lse, torch.float32, query.lse_shape, pool.device),
             _stream(stream, pool.device),
         )
     )
@@ -221,12 +238,12 @@ def accumulate_weights_kv4(pool: Kv4Pool, query: Kv4Query, lse, weights, stream=
     """Add to ``weights`` float32 [batch, kv_heads, >= max_tokens] the attention
     weight each token gets from the query rows, given their ``lse``."""
     _match_query(pool, query)
-    batch, rows, q_heads, _ = query.shape
+    batch = query.shape[0]
     if weights.dim() != 3 or weights.shape[:2] != (batch, pool.kv_heads):
         raise ValueError("weights must have shape [batch, kv_heads, >= max_tokens]")
     check(
         _lib.load().kvb_accumulate_weights_kv4(
-            pool._ref, query._ref, _tensor("lse", lse, torch.float32, (batch, rows, q_heads), pool.device),
+            pool._ref, query._ref, _tensor("lse", lse, torch.float32, query.lse_shape, pool.device),
             _tensor("weights", weights, torch.float32, None, pool.device), weights.shape[2],
             _stream(stream, pool.device),
         )
@@ -249,6 +266,7 @@ class EvictPlan:
         self.device, self.budget = weights.device, budget
         self.weights, self.block_table = weights, block_table
         self._kept = seq_lens
+        self._keep_shape, self._lens_shape = (self.batch, self.kv_heads, budget), (self.batch,)
         self._table = _tensor("block_table", block_table, torch.int32, None, self.device)
         if block_table.dim() != 2 or block_table.shape[0] != self.batch:
             raise ValueError("block_table must have shape [batch, pages]")
@@ -269,8 +287,8 @@ def select_tokens(plan: EvictPlan, keep, kept_lens, stream=None) -> None:
     zeros; ``kept_lens`` int32 [batch]."""
     check(
         _lib.load().kvb_select_tokens(
-            plan._ref, _tensor("keep", keep, torch.int32, (plan.batch, plan.kv_heads, plan.budget), plan.device),
-            _tensor("kept_lens", kept_lens, torch.int32, (plan.batch,), plan.device), _stream(stream, plan.device),
+            plan._ref, _tensor("keep", keep, torch.int32, plan._keep_shape, plan.device),
+            _tensor("kept_lens", kept_lens, torch.int32, plan._lens_shape, plan.device), _stream(stream, plan.device),
         )
     )
 
@@ -288,7 +306,7 @@ def compact_kv4(pool: Kv4Pool, plan: EvictPlan, keep, new_table, new_weights=Non
     check(
         _lib.load().kvb_compact_kv4(
             pool._ref, plan._ref, plan._table, plan._width,
-            _tensor("keep", keep, torch.int32, (plan.batch, plan.kv_heads, plan.budget), plan.device),
+            _tensor("keep", keep, torch.int32, plan._keep_shape, plan.device),
             _tensor("new_table", new_table, torch.int32, None, plan.device), new_table.shape[1],
             _optional("new_weights", new_weights, torch.float32, None, plan.device),
             0 if new_weights is None else new_weights.shape[2], _stream(stream, plan.device),
