@@ -94,36 +94,35 @@ struct Kv4Cursor {
   int32_t base;     // where the segment's stage 0 lies
 };
 
-template <bool RULES>
-__device__ __forceinline__ void kv4_stages(const Kv4AttendParams& p, uint32_t b, uint32_t& len,
-                                           uint32_t& stages, uint32_t& head, uint32_t& skip) {
-  len = kv4_len(p.seq_lens, b, p.max_tokens);
-  stages = (len + kStageTokens - 1) / kStageTokens;
-  head = stages;
-  skip = 0;
+// HINT: read before the wait for the preceding kernel, past L1; such values
+// only steer prefetches, or are compared with what the wait lets through.
+template <bool RULES, bool HINT = false>
+__device__ __forceinline__ void kv4_load_sequence(const Kv4AttendParams& p, Kv4Cursor& c) {
+  const uint32_t len = HINT ? __ldcg(p.seq_lens + c.b) : kv4_load(p.seq_lens + c.b);
+  c.len = min(len, p.max_tokens);
+  c.stages = (c.len + kStageTokens - 1) / kStageTokens;
+  c.head = c.stages;
+  c.skip = 0;
   if (RULES && p.rule.window != 0 && p.pool.pos == nullptr && p.rule.q_pos == nullptr) {
     // The first row's window starts at len - rows - window + 1.
     const uint64_t reach = uint64_t(p.rows) + p.rule.window - 1;
-    const uint32_t from = reach < len ? uint32_t(len - reach) / kStageTokens : 0u;
-    const uint32_t fix = p.rule.prefix != nullptr ? min(__ldg(p.rule.prefix + b), len) : 0u;
-    head = (fix + kStageTokens - 1) / kStageTokens;
-    if (head < from) {
-      skip = from - head;
-      stages -= skip;
+    const uint32_t from = reach < c.len ? uint32_t(c.len - reach) / kStageTokens : 0u;
+    uint32_t fix = 0;
+    if (p.rule.prefix != nullptr) fix = min(HINT ? __ldcg(p.rule.prefix + c.b) : kv4_load(p.rule.prefix + c.b), c.len);
+    c.head = (fix + kStageTokens - 1) / kStageTokens;
+    if (c.head < from) {
+      c.skip = from - c.head;
+      c.stages -= c.skip;
     }
   }
 }
 
 template <bool RULES>
 __device__ __forceinline__ uint32_t kv4_stage_count(const Kv4AttendParams& p, uint32_t b) {
-  uint32_t len, stages, head, skip;
-  kv4_stages<RULES>(p, b, len, stages, head, skip);
-  return stages;
-}
-
-template <bool RULES>
-__device__ __forceinline__ void kv4_load_sequence(const Kv4AttendParams& p, Kv4Cursor& c) {
-  kv4_stages<RULES>(p, c.b, c.len, c.stages, c.head, c.skip);
+  Kv4Cursor c;
+  c.b = b;
+  kv4_load_sequence<RULES>(p, c);
+  return c.stages;
 }
 
 // The next segment that has stages (b = batch at the end).
@@ -138,8 +137,48 @@ __device__ __forceinline__ void kv4_next_segment(const Kv4AttendParams& p, uint3
   }
 }
 
-// Warp-cooperative: the range of worker `w` and the cursor at its first
-// stage. Returns the number of stages of the range.
+// Equal ranges of the `total` stages, the first ones a stage longer. (A 64-bit
+// division is a few hundred instructions on the path to the first copy.)
+__device__ __forceinline__ uint32_t kv4_range(uint64_t total, uint32_t workers, uint32_t w, uint64_t& first) {
+  workers = uint32_t(min(uint64_t(workers), total));
+  if (w >= workers) return 0;
+  const uint64_t each = total >> 32 ? total / workers : uint32_t(total) / workers;
+  const uint32_t more = uint32_t(total - each * workers);
+  first = w * each + min(w, more);
+  return uint32_t(each) + (w < more ? 1u : 0u);
+}
+
+// `into`: the first stage, counted from the sequence's first.
+__device__ __forceinline__ void kv4_enter(uint64_t into, Kv4Cursor& c) {
+  c.seg = into >> 32 ? uint32_t(into / c.stages) : uint32_t(into) / c.stages;
+  c.base = -int32_t(into - uint64_t(c.seg) * c.stages);
+}
+
+// Up to 32 sequences, lane b holding sequence b in `own`: the range of worker
+// w and the cursor at its first stage. Returns its number of stages.
+__device__ __forceinline__ uint32_t kv4_locate_lanes(const Kv4AttendParams& p, uint32_t w, uint32_t segs,
+                                                     const Kv4Cursor& own, Kv4Cursor& c) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint64_t upto = lane < p.batch ? own.stages : 0u;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= uint32_t(o)) upto += y;
+  }
+  uint64_t first = 0;
+  const uint32_t count = kv4_range(__shfl_sync(0xffffffffu, upto, 31) * segs, p.workers, w, first);
+  if (count == 0) return 0;
+  const int at = __ffs(__ballot_sync(0xffffffffu, upto * segs > first)) - 1;
+  c.b = at;
+  c.len = __shfl_sync(0xffffffffu, own.len, at);
+  c.stages = __shfl_sync(0xffffffffu, own.stages, at);
+  c.head = __shfl_sync(0xffffffffu, own.head, at);
+  c.skip = __shfl_sync(0xffffffffu, own.skip, at);
+  kv4_enter(first - (__shfl_sync(0xffffffffu, upto, at) - c.stages) * segs, c);
+  return count;
+}
+
+// The same for more sequences, or for a direct call (worker w = segment w).
 template <bool RULES>
 __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t w, uint32_t segs, Kv4Cursor& c) {
   const uint32_t lane = threadIdx.x & 31;
@@ -151,32 +190,22 @@ __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t w, uint32_t se
     kv4_load_sequence<RULES>(p, c);
     return c.stages;
   }
-  // Up to 32 sequences: each lane keeps its count, read once.
-  const bool one_pass = p.batch <= 32;
-  uint32_t own = 0;
   uint64_t total = 0;
-  for (uint32_t b = lane; b < p.batch; b += 32) total += own = kv4_stage_count<RULES>(p, b);
+  for (uint32_t b = lane; b < p.batch; b += 32) total += kv4_stage_count<RULES>(p, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  total *= segs;
-  // Equal ranges, the first ones a stage longer. (A 64-bit division is a
-  // few hundred instructions on the path to the first copy.)
-  const uint32_t workers = uint32_t(min(uint64_t(p.workers), total));
-  if (w >= workers) return 0;
-  const uint64_t each = total >> 32 ? total / workers : uint32_t(total) / workers;
-  const uint32_t more = uint32_t(total - each * workers);
-  const uint64_t x0 = w * each + min(w, more);
-  const uint32_t count = uint32_t(each) + (w < more ? 1u : 0u);
-  uint64_t before = 0;
+  uint64_t first = 0, before = 0;
+  const uint32_t count = kv4_range(total * segs, p.workers, w, first);
+  if (count == 0) return 0;
   for (uint32_t from = 0; from < p.batch; from += 32) {
-    const uint32_t n = one_pass ? own : from + lane < p.batch ? kv4_stage_count<RULES>(p, from + lane) : 0u;
+    const uint32_t n = from + lane < p.batch ? kv4_stage_count<RULES>(p, from + lane) : 0u;
     uint64_t upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t y = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= uint32_t(o)) upto += y;
     }
-    const uint32_t hit = __ballot_sync(0xffffffffu, (before + upto) * segs > x0);
+    const uint32_t hit = __ballot_sync(0xffffffffu, (before + upto) * segs > first);
     if (hit != 0) {
       const int at = __ffs(hit) - 1;
       before = (before + __shfl_sync(0xffffffffu, upto - n, at)) * segs;
@@ -186,9 +215,60 @@ __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t w, uint32_t se
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
   kv4_load_sequence<RULES>(p, c);
-  const uint64_t into = x0 - before;
-  c.seg = into >> 32 ? uint32_t(into / c.stages) : uint32_t(into) / c.stages;
-  c.base = -int32_t(into - uint64_t(c.seg) * c.stages);
+  kv4_enter(first - before, c);
+  return count;
+}
+
+// Finds the warp's range around the wait for the preceding kernel. Up to 32
+// sequences are located before it, from lengths that are only taken if they
+// are the same after it; the first stage's pages, the next one's table entries
+// and the query rows are prefetched into L2 meanwhile.
+template <int D, bool V, bool RULES>
+__device__ __forceinline__ uint32_t kv4_start(const Kv4AttendParams& p, uint32_t w, uint32_t segs, uint32_t cols,
+                                              Kv4Cursor& c) {
+  const uint32_t lane = threadIdx.x & 31;
+  if (p.direct || p.batch > 32) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    return kv4_locate<RULES>(p, w, segs, c);
+  }
+  Kv4Cursor hint;
+  hint.b = min(lane, p.batch - 1);
+  kv4_load_sequence<RULES, true>(p, hint);
+  uint32_t count = kv4_locate_lanes(p, w, segs, hint, c);
+  if (count != 0) {
+    const uint32_t j = uint32_t(-c.base), stage = RULES && j >= c.head ? j + c.skip : j;
+    const uint32_t page = (stage * kStageTokens + 16 * (lane & 3)) >> p.log2_page;
+    const uint32_t* entry = p.table + size_t(c.b) * p.table_stride + page;
+    const uint32_t phys = (page << p.log2_page) < c.len ? __ldcg(entry) : kNoUnit;
+    const uint32_t h = c.seg / p.col_groups, part = lane >> 2;
+    const bool pages = (lane & 3) < (kStageTokens >> p.log2_page) && part < (V ? 4 : 2);
+    // Lane q + 4 part: array `part` of page q of the stage (with 16-token
+    // pages lane q has page q; with larger ones the first lanes').
+    const uint32_t mine = __shfl_sync(0xffffffffu, phys, (lane & 3) << (p.log2_page - 4));
+    if (pages && mine < p.pool.pages) {
+      const size_t unit = size_t(mine) * p.pool.kv_heads + h;
+      const uint32_t P = p.page_tokens;
+      if (part == 0) prefetch_l2(p.pool.k + unit * P * (D / 2), P * (D / 2));
+      if (part == 1) prefetch_l2(p.pool.kp + unit * P, P * 8);
+      if (part == 2) prefetch_l2(p.pool.v + unit * P * (D / 2), P * (D / 2));
+      if (part == 3) prefetch_l2(p.pool.vp + unit * P, P * 8);
+    }
+    const uint32_t col = (c.seg % p.col_groups) * cols + (lane >> 2) % cols;
+    if (col < p.rows * p.group) {
+      const int64_t at = int64_t(c.b) * p.batch_stride + int64_t(col / p.group) * p.row_stride +
+                         int64_t(h * p.group + col % p.group) * D + (D / 4) * (lane & 3);
+      prefetch_line_l2(static_cast<const uint8_t*>(p.q) + at * (p.type == 0 ? 4 : 2));
+    }
+  }
+  grid_launch_dependents();
+  grid_dependency_wait();
+  Kv4Cursor own;
+  own.b = hint.b;
+  kv4_load_sequence<RULES>(p, own);
+  if (!__all_sync(0xffffffffu, own.len == hint.len && own.stages == hint.stages && own.head == hint.head &&
+                                   own.skip == hint.skip))
+    count = kv4_locate_lanes(p, w, segs, own, c);
   return count;
 }
 
@@ -242,7 +322,7 @@ struct Kv4Feeder {
       const uint32_t t = stage * kStageTokens + 16 * (threadIdx.x & 3);
       head = p.col_groups == 1 ? cur.seg : cur.seg / p.col_groups;
       const uint32_t page = t >> p.log2_page;  // all of it: V's quarters are not tokens
-      if ((page << p.log2_page) < cur.len) phys = __ldg(p.table + size_t(cur.b) * p.table_stride + page);
+      if ((page << p.log2_page) < cur.len) phys = kv4_load(p.table + size_t(cur.b) * p.table_stride + page);
       ++next;
     }
   }
@@ -311,17 +391,17 @@ __device__ __forceinline__ void kv4_load_values(const void* q, int64_t at, F&& s
       for (int e = 0; e < 8; ++e) {
         const int64_t x = at + step(i) + e;
         if (type == 0) {
-          v[i][e] = __ldg(static_cast<const float*>(q) + x);
+          v[i][e] = kv4_load(static_cast<const float*>(q) + x);
         } else {
           float unused;
-          kv4_half_pair(__ldg(static_cast<const uint16_t*>(q) + x), type == 2, v[i][e], unused);
+          kv4_half_pair(kv4_load(static_cast<const uint16_t*>(q) + x), type == 2, v[i][e], unused);
         }
       }
   } else if (type == 0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + step(i));
-      const float4 a = __ldg(src), b = __ldg(src + 1);
+      const float4 a = kv4_load(src), b = kv4_load(src + 1);
       v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w, v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z,
       v[i][7] = b.w;
     }
@@ -329,7 +409,7 @@ __device__ __forceinline__ void kv4_load_values(const void* q, int64_t at, F&& s
     uint4 raw[N];
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + at + step(i)));
+      raw[i] = kv4_load(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + at + step(i)));
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       kv4_half_pair(raw[i].x, type == 2, v[i][0], v[i][1]);
@@ -445,7 +525,7 @@ __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
   qf.own = C == 4 && grp >= 4 ? 65536.f * dot : dot;
   qf.other = C == 4 && grp >= 4 ? dot : 65536.f * dot;
   qf.sum = float(total) * dot;
-  qf.slope = RULES && p.rule.slopes != nullptr ? __ldg(p.rule.slopes + head) : 0.f;
+  qf.slope = RULES && p.rule.slopes != nullptr ? kv4_load(p.rule.slopes + head) : 0.f;
   qf.pos = valid ? kv4_query_position(p.rule, b, r, p.rows, len) : -1;
 }
 
@@ -583,7 +663,7 @@ __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const u
     }
     if (pos != nullptr) {
 #pragma unroll
-      for (int u = 0; u < kTokens; ++u) pk[u] = __ldg(pos + (at & 15) + kv4_token(C, u));
+      for (int u = 0; u < kTokens; ++u) pk[u] = kv4_load(pos + (at & 15) + kv4_token(C, u));
     } else {
 #pragma unroll
       for (int u = 0; u < kTokens; ++u) pk[u] = t0 + int32_t(kv4_token(C, u));
@@ -810,7 +890,7 @@ __device__ __forceinline__ const int32_t* kv4_positions(const Kv4AttendParams& p
                                                         uint32_t len, uint32_t tb) {
   if (p.pool.pos == nullptr) return nullptr;
   const uint32_t t = tb + 16 * (threadIdx.x & 3);
-  const uint32_t page = t < len ? __ldg(p.table + size_t(b) * p.table_stride + (t >> p.log2_page)) : kNoUnit;
+  const uint32_t page = t < len ? kv4_load(p.table + size_t(b) * p.table_stride + (t >> p.log2_page)) : kNoUnit;
   if (page >= p.pool.pages) return nullptr;
   return p.pool.pos + (size_t(page) * p.pool.kv_heads + h) * p.page_tokens + (t & (p.page_tokens - 1));
 }
@@ -818,7 +898,7 @@ __device__ __forceinline__ const int32_t* kv4_positions(const Kv4AttendParams& p
 __device__ __forceinline__ void kv4_report_lengths(const Kv4AttendParams& p) {
   if (blockIdx.x != 0) return;
   for (uint32_t b = threadIdx.x; b < p.batch; b += kKv4Threads)
-    if (__ldg(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
+    if (kv4_load(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
 }
 
 template <int D, int C, int PD, int MINB, bool RULES>
@@ -828,13 +908,10 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = lane >> 2, tig = lane & 3;
   Kv4Feeder<D, true, RULES> feed;
   feed.init(smem, warp);
-  grid_launch_dependents();
-  grid_dependency_wait();
-
   const uint32_t worker = blockIdx.x * kKv4Warps + warp;
   const uint32_t segs = p.pool.kv_heads * p.col_groups;
   Kv4Cursor cur;
-  const uint32_t count = kv4_locate<RULES>(p, worker, segs, cur);
+  const uint32_t count = kv4_start<D, true, RULES>(p, worker, segs, C, cur);
   kv4_report_lengths(p);
   if (count == 0 && (!p.direct || worker >= p.workers)) return;
 
@@ -856,7 +933,7 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
     const uint32_t h = cur.seg / p.col_groups;
     Kv4Query<D, C> qf;
     kv4_load_query<D, C, RULES>(p, cur.b, h, cur.seg % p.col_groups, cur.len, qf);
-    const uint32_t prefix = RULES && p.rule.prefix != nullptr ? __ldg(p.rule.prefix + cur.b) : 0u;
+    const uint32_t prefix = RULES && p.rule.prefix != nullptr ? kv4_load(p.rule.prefix + cur.b) : 0u;
     Kv4State<D> st;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
@@ -1050,12 +1127,9 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = lane >> 2, tig = lane & 3;
   Kv4Feeder<D, false, RULES> feed;
   feed.init(smem, warp);
-  grid_launch_dependents();
-  grid_dependency_wait();
-
   const uint32_t segs = p.pool.kv_heads;  // p.col_groups is 1 here
   Kv4Cursor cur;
-  const uint32_t count = kv4_locate<RULES>(p, blockIdx.x * kKv4Warps + warp, segs, cur);
+  const uint32_t count = kv4_start<D, false, RULES>(p, blockIdx.x * kKv4Warps + warp, segs, C, cur);
   kv4_report_lengths(p);
   if (count == 0) return;
   feed.cur = cur;
@@ -1075,11 +1149,11 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
     float lse = INFINITY;
     const uint32_t col = group * C + grp % C;
     if (col < p.rows * p.group) {
-      const float x = __ldg(p.lse_in + (size_t(cur.b) * p.rows + col / p.group) * p.q_heads + cur.seg * p.group +
+      const float x = kv4_load(p.lse_in + (size_t(cur.b) * p.rows + col / p.group) * p.q_heads + cur.seg * p.group +
                             col % p.group);
       if (x != -INFINITY) lse = RULES ? x : x * kLog2e;
     }
-    const uint32_t prefix = RULES && p.rule.prefix != nullptr ? __ldg(p.rule.prefix + cur.b) : 0u;
+    const uint32_t prefix = RULES && p.rule.prefix != nullptr ? kv4_load(p.rule.prefix + cur.b) : 0u;
     float* weights = p.weights + (int64_t(cur.b) * p.pool.kv_heads + cur.seg) * p.weight_stride;
     for (; done < end; ++done) {
       const uint32_t j = uint32_t(int32_t(done) - cur.base);

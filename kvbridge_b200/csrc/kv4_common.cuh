@@ -16,6 +16,19 @@ enum : int {
   kKv4BadKept = 8,
 };
 
+// Loads of what the preceding kernel may have written. These kernels start
+// before it has ended (programmatic dependent launch), so nothing of theirs is
+// read-only for their lifetime, as the non-coherent load instructions ask.
+template <class T>
+__device__ __forceinline__ T kv4_load(const T* p) {
+  return *p;
+}
+// The same for data used once.
+template <class T>
+__device__ __forceinline__ T kv4_stream(const T* p) {
+  return __ldcs(p);
+}
+
 struct Kv4View {
   uint8_t* k;
   uint8_t* v;
@@ -36,7 +49,7 @@ struct Kv4Rule {
 // Row r of `rows` query rows of a sequence of `len` tokens.
 __device__ __forceinline__ int32_t kv4_query_position(const Kv4Rule& rule, uint32_t b, uint32_t r,
                                                       uint32_t rows, uint32_t len) {
-  return rule.q_pos != nullptr ? __ldg(rule.q_pos + size_t(b) * rows + r)
+  return rule.q_pos != nullptr ? kv4_load(rule.q_pos + size_t(b) * rows + r)
                                : int32_t(len) - int32_t(rows) + int32_t(r);
 }
 
@@ -50,7 +63,7 @@ __device__ __forceinline__ bool kv4_visible(int32_t pk, int32_t pq, uint32_t win
 
 __device__ __forceinline__ uint32_t kv4_len(const uint32_t* seq_lens, uint32_t b,
                                             uint32_t max_tokens) {
-  const uint32_t len = __ldg(seq_lens + b);
+  const uint32_t len = kv4_load(seq_lens + b);
   return len > max_tokens ? max_tokens : len;
 }
 

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectPar
   const uint32_t len = kv4_len(p.seq_lens, b, p.max_tokens), kept = min(len, p.budget);
   if (tid == 0 && rank == 0 && segment % p.kv_heads == 0) {
     p.kept_lens[b] = kept;
-    if (__ldg(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
+    if (kv4_load(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
   }
   int32_t* keep = p.keep + size_t(segment) * p.budget;
   for (uint32_t i = kept + rank * kSelectThreads + tid; i < p.budget; i += ctas * kSelectThreads) keep[i] = 0;
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectPar
   const uint32_t first = p.sinks, last = len - p.recent;  // the middle tokens
   const uint32_t lo = max(from, first), hi = max(min(to, last), lo);  // of this CTA
   const bool cached = part <= kSelectKeys;
-  auto key_of = [&](uint32_t t) { return cached ? keys[t - from] : weight_key(__ldg(weights + t)); };
+  auto key_of = [&](uint32_t t) { return cached ? keys[t - from] : weight_key(kv4_load(weights + t)); };
   // A thread goes over tokens in a row; the odd count keeps a warp's reads of
   // the keys in different banks.
   const uint32_t run = ((part + kSelectThreads - 1) / kSelectThreads) | 1u;
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectPar
   if (any) {
     if (cached) {
 #pragma unroll 8
-      for (uint32_t t = lo + tid; t < hi; t += kSelectThreads) keys[t - from] = weight_key(__ldg(weights + t));
+      for (uint32_t t = lo + tid; t < hi; t += kSelectThreads) keys[t - from] = weight_key(kv4_load(weights + t));
     }
 #pragma unroll 1
     for (int round = 0; round < 3; ++round) {
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kCompactThreads) compact_kv4_kernel(const Comp
   grid_launch_dependents();
   grid_dependency_wait();
   const uint32_t len = kv4_len(p.seq_lens, b, p.max_tokens), kept = min(len, p.budget);
-  if (first == 0 && h == 0 && tid == 0 && __ldg(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
+  if (first == 0 && h == 0 && tid == 0 && kv4_load(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
   const size_t row = size_t(b) * H + h;
   const int32_t* keep = p.keep + row * p.budget;
   if (tid < 64) {  // two whole warps
@@ -229,10 +229,10 @@ __global__ void __launch_bounds__(kCompactThreads) compact_kv4_kernel(const Comp
     uint32_t page = 0xffffffffu, slot = 0;
     float weight = 0.f;
     if (i < kept) {
-      const uint32_t t = uint32_t(__ldg(keep + i));
+      const uint32_t t = uint32_t(kv4_load(keep + i));
       if (t < len && (t >> p.log2_page) < p.table_stride) {
-        weight = __ldg(p.weights + int64_t(row) * p.weight_stride + t);
-        page = __ldg(p.table + size_t(b) * p.table_stride + (t >> p.log2_page));
+        weight = kv4_load(p.weights + int64_t(row) * p.weight_stride + t);
+        page = kv4_load(p.table + size_t(b) * p.table_stride + (t >> p.log2_page));
         slot = t & (P - 1);
         if (page < p.pool.pages)
           at = (uint64_t(page) * H + h) * P + slot;
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kCompactThreads) compact_kv4_kernel(const Comp
     const uint32_t j = (first + 16 * tid) >> p.log2_page;
     uint64_t unit = kNowhere;
     if (first + 16 * tid < kept) {
-      const uint32_t page = __ldg(p.new_table + size_t(b) * p.new_stride + j);
+      const uint32_t page = kv4_load(p.new_table + size_t(b) * p.new_stride + j);
       if (page < p.pool.pages)
         unit = uint64_t(page) * H + h;
       else
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kCompactThreads) compact_kv4_kernel(const Comp
     const uint64_t from = src_at[t], unit = dst_unit[t / 16];
     if (from == kNowhere || unit == kNowhere) continue;
     const uint64_t to = unit * P + ((first + t) & (P - 1));
-    reinterpret_cast<uint4*>(p.pool.k)[to * kChunks + c] = __ldcs(reinterpret_cast<const uint4*>(p.pool.k) + from * kChunks + c);
+    reinterpret_cast<uint4*>(p.pool.k)[to * kChunks + c] = kv4_stream(reinterpret_cast<const uint4*>(p.pool.k) + from * kChunks + c);
     if (c == 0) p.pool.kp[to] = p.pool.kp[from];
     if (c == 1) p.pool.vp[to] = p.pool.vp[from];
     if (c == kChunks - 1 && p.pool.pos != nullptr) p.pool.pos[to] = p.pool.pos[from];

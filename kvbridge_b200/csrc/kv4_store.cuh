@@ -49,7 +49,7 @@ template <int D, int TILE>
 __device__ __forceinline__ void kv4_map_tile(const Kv4RowsParams& p, uint32_t first, uint32_t h, Kv4Tile<D, TILE>& t) {
   const uint32_t P = p.page_tokens;
   for (uint32_t i = threadIdx.x; i < TILE; i += blockDim.x) {
-    const int64_t slot = first + i < p.tokens ? __ldg(p.slots + first + i) : -1;
+    const int64_t slot = first + i < p.tokens ? kv4_load(p.slots + first + i) : -1;
     const bool ok = slot >= 0 && uint64_t(slot) < p.slots_total;
     if (slot >= 0 && !ok) atomicMax(&g_kvb_status, kKv4BadSlot);
     const uint32_t s = uint32_t(slot) & (P - 1);
@@ -100,7 +100,7 @@ __device__ __forceinline__ Eight<T> load_eight(const T* src, bool vector) {
     const uint4* s = reinterpret_cast<const uint4*>(src);
     uint4* d = reinterpret_cast<uint4*>(&e);
 #pragma unroll
-    for (int i = 0; i < int(sizeof(e) / 16); ++i) d[i] = __ldcs(s + i);
+    for (int i = 0; i < int(sizeof(e) / 16); ++i) d[i] = kv4_stream(s + i);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) e.x[i] = src[i];
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(32 * kKv4StoreWarps) append_kv4_kernel(const K
       }
       if (part == 0) {
         (is_v ? p.pool.vp : p.pool.kp)[at] = make_float2(scale, lo);
-        if (!is_v && p.pool.pos != nullptr) p.pool.pos[at] = __ldg(p.positions + first + t);
+        if (!is_v && p.pool.pos != nullptr) p.pool.pos[at] = kv4_load(p.positions + first + t);
       }
     }
   }
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(32 * kKv4StoreWarps) load_kv4_kernel(const Kv4
     if (i % (TILE / 4) >= quads || q >= D / 8) continue;
     const uint8_t* src = p.pool.v + tile.v_at[tile.quads[i % (TILE / 4)]] + 4 * q * P;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[n][j] = __ldcs(reinterpret_cast<const uint32_t*>(src + j * P));
+    for (int j = 0; j < 4; ++j) w[n][j] = kv4_stream(reinterpret_cast<const uint32_t*>(src + j * P));
   }
   constexpr int kFirstK = M::kWarpTokens / M::kRows;  // the pass with the first K rows
   constexpr int kHalf = kFirstK == 0 ? M::kPasses : kFirstK, kBatch = kHalf < M::kBatch ? kHalf : M::kBatch;
@@ -309,12 +309,12 @@ __global__ void __launch_bounds__(32 * kKv4StoreWarps) load_kv4_kernel(const Kv4
         par[i] = make_float2(0.f, 0.f);  // zeros where the slot is not in the pool
         if (is_v != want_v || at == kNowhere) continue;
         const bool in_quad = tile.in_quad[t / 32] >> (t % 32) & 1u;
-        par[i] = __ldg((is_v ? p.pool.vp : p.pool.kp) + at);
+        par[i] = kv4_load((is_v ? p.pool.vp : p.pool.kp) + at);
 #pragma unroll
         for (int r = 0; r < M::kRuns; ++r) {
           const uint32_t q = part + r * M::kLanes;
           if (!is_v) {
-            word[i][r] = __ldcs(reinterpret_cast<const uint32_t*>(p.pool.k) + at * (D / 8) + q);
+            word[i][r] = kv4_stream(reinterpret_cast<const uint32_t*>(p.pool.k) + at * (D / 8) + q);
           } else if (in_quad) {
             word[i][r] = tile.v[t][q];
           } else {
