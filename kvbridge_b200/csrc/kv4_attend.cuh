@@ -327,8 +327,23 @@ struct Kv4Feeder {
     }
   }
 
-  // Starts the copies of the K or the V of the stage looked up last: a quarter
-  // of the stage (of 1, 2 or 4 pages' codes) at a time.
+  // Starts the copies of the K or the V of the stage looked up last. 64-token
+  // pages: every lane has looked up the same page.
+  template <bool OF_V>
+  __device__ __forceinline__ void copy_page(const Kv4AttendParams& p) {
+    using S = Kv4Smem<D, V>;
+    const uint32_t lane = threadIdx.x & 31;
+    const size_t unit = size_t(phys) * p.pool.kv_heads + head;
+    const uint8_t* src = (OF_V ? p.pool.v : p.pool.k) + unit * (32 * D) + 16 * lane;
+    const uint32_t dst = addr + (OF_V ? S::kOffV : 0u) + 16 * lane;
+#pragma unroll
+    for (uint32_t i = 0; i < D / 16; ++i) copy16_async(dst + 512 * i, src + 512 * i);
+    copy16_async(addr + (OF_V ? S::kOffVp : S::kOffKp) + (lane >> 3) * kKv4ParamPitch + (lane & 7) * 16,
+                 reinterpret_cast<const uint8_t*>((OF_V ? p.pool.vp : p.pool.kp) + unit * 64 + 2 * lane));
+  }
+
+  // Smaller pages: a quarter of the stage (of its 2 or 4 pages' codes) at a
+  // time, from the unit that lane g has looked up.
   template <bool OF_V, bool ALL>
   __device__ __forceinline__ void copy_groups(const Kv4AttendParams& p, uint32_t unit) {
     using S = Kv4Smem<D, V>;
@@ -358,11 +373,15 @@ struct Kv4Feeder {
   __device__ __forceinline__ void copy(const Kv4AttendParams& p) {
     const bool ok = phys < p.pool.pages;
     if (!OF_V && !ok && phys != kNoUnit) atomicMax(&g_kvb_status, kKv4BadPage);
-    const uint32_t unit = ok ? phys * p.pool.kv_heads + head : kNoUnit;
-    if (__all_sync(0xffffffffu, ok))
-      copy_groups<OF_V, true>(p, unit);
-    else
-      copy_groups<OF_V, false>(p, unit);
+    if (p.log2_page == 6) {
+      if (ok) copy_page<OF_V>(p);
+    } else {
+      const uint32_t unit = ok ? phys * p.pool.kv_heads + head : kNoUnit;
+      if (__all_sync(0xffffffffu, ok))
+        copy_groups<OF_V, true>(p, unit);
+      else
+        copy_groups<OF_V, false>(p, unit);
+    }
     copy_commit();
   }
 };
