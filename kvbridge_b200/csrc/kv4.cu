@@ -228,20 +228,29 @@ struct Kv4Kernel {
 constexpr int attend_ctas(int dim) { return dim == 256 ? 2 : dim == 64 ? 4 : 3; }
 constexpr int weigh_ctas(int dim, int cols) { return dim == 256 ? 2 : dim == 64 || cols == 4 ? 4 : 3; }
 
-template <int D, int C, int PD, bool RULES>
+template <int D, int C, int PD, int RULES>
 Kv4Kernel attend_kernel() {
   return {reinterpret_cast<const void*>(&kvb::attend_kv4_kernel<D, C, PD, attend_ctas(D), RULES>),
           kvb::Kv4Smem<D, true>::kBytes};
 }
 
-template <int D, int C, bool RULES>
+template <int D, int C, int RULES>
 Kv4Kernel weigh_kernel() {
   return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, weigh_ctas(D, C), RULES>),
           kvb::Kv4Smem<D, false>::kBytes};
 }
 
-bool has_rules(const Kv4Pool& pool, const Kv4Query& q) {
-  return q.softcap > 0.f || q.window != 0 || q.slopes || q.prefix_lens || q.q_positions || pool.positions;
+int rules_of(const Kv4Pool& pool, const Kv4Query& q) {
+  if (q.softcap > 0.f || q.slopes || q.q_positions || pool.positions) return kvb::kRulesAll;
+  return q.window != 0 || q.prefix_lens ? kvb::kRulesMask : kvb::kRulesNone;
+}
+
+// Calls f(integral_constant<int, RULES>).
+template <class F>
+auto by_rules(int rules, F&& f) {
+  if (rules == kvb::kRulesNone) return f(std::integral_constant<int, kvb::kRulesNone>{});
+  if (rules == kvb::kRulesMask) return f(std::integral_constant<int, kvb::kRulesMask>{});
+  return f(std::integral_constant<int, kvb::kRulesAll>{});
 }
 
 // Query columns a segment: 4 where all of a KV head's fit, else 8.
@@ -249,21 +258,23 @@ uint32_t segment_columns(const Kv4Pool& pool, const Kv4Query& q) {
   return q.rows * (q.q_heads / pool.kv_heads) <= 4 ? 4 : 8;
 }
 
-template <bool RULES>
-Kv4Kernel attend_kernel(uint32_t dim, uint32_t cols, bool f32) {
+Kv4Kernel attend_kernel(uint32_t dim, uint32_t cols, bool f32, int rules) {
   return by_dim(dim, [&](auto d) {
-    constexpr int D = decltype(d)::value;
-    return cols == 4 ? f32 ? attend_kernel<D, 4, 3, RULES>() : attend_kernel<D, 4, 2, RULES>()
-           : f32     ? attend_kernel<D, 8, 3, RULES>()
-                     : attend_kernel<D, 8, 2, RULES>();
+    return by_rules(rules, [&](auto r) {
+      constexpr int D = decltype(d)::value, RULES = decltype(r)::value;
+      return cols == 4 ? f32 ? attend_kernel<D, 4, 3, RULES>() : attend_kernel<D, 4, 2, RULES>()
+             : f32     ? attend_kernel<D, 8, 3, RULES>()
+                       : attend_kernel<D, 8, 2, RULES>();
+    });
   });
 }
 
-template <bool RULES>
-Kv4Kernel weigh_kernel(uint32_t dim, uint32_t cols) {
+Kv4Kernel weigh_kernel(uint32_t dim, uint32_t cols, int rules) {
   return by_dim(dim, [&](auto d) {
-    constexpr int D = decltype(d)::value;
-    return cols == 4 ? weigh_kernel<D, 4, RULES>() : weigh_kernel<D, 8, RULES>();
+    return by_rules(rules, [&](auto r) {
+      constexpr int D = decltype(d)::value, RULES = decltype(r)::value;
+      return cols == 4 ? weigh_kernel<D, 4, RULES>() : weigh_kernel<D, 8, RULES>();
+    });
   });
 }
 
@@ -300,7 +311,8 @@ uint32_t split_ctas(const Kv4Kernel& k, uint64_t segments, uint32_t max_tokens) 
 
 struct AttendPlan {
   Kv4Kernel kernel;
-  bool rules, direct, many;
+  int rules;
+  bool direct, many;
   uint32_t cols, col_groups, segments, ctas, workers;
   size_t ml_offset, warps_offset, bytes;  // of the workspace
 };
@@ -310,10 +322,10 @@ constexpr uint32_t kDirectTokens = 128;
 
 AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
   AttendPlan a{};
-  a.rules = has_rules(pool, q);
+  a.rules = rules_of(pool, q);
   const bool f32 = q.type == Kv4Type::f32;
   const uint32_t cols = a.cols = segment_columns(pool, q), all = q.rows * (q.q_heads / pool.kv_heads);
-  a.kernel = a.rules ? attend_kernel<true>(pool.dim, cols, f32) : attend_kernel<false>(pool.dim, cols, f32);
+  a.kernel = attend_kernel(pool.dim, cols, f32, a.rules);
   a.col_groups = (all + cols - 1) / cols;
   a.segments = q.batch * pool.kv_heads * a.col_groups;
   a.direct = q.max_tokens <= kDirectTokens;
@@ -367,10 +379,11 @@ void launch_attention_kv4(const Kv4Pool& pool, const Kv4Query& q, void* workspac
   void* merge_args[] = {&prm, &cols};
   const void* merge = by_dim(pool.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    return a.rules ? a.many ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, true, true>)
-                            : reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, true, false>)
-           : a.many ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, false, true>)
-                    : reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, false, false>);
+    return by_rules(a.rules, [&](auto r) {
+      constexpr int RULES = decltype(r)::value;
+      return a.many ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, RULES, true>)
+                    : reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, RULES, false>);
+    });
   });
   const uint32_t rows = q.batch * q.rows * q.q_heads;
   launch_kernel_pdl(merge, dim3(a.many ? rows : (rows + kvb::kKv4MergeWarps - 1) / kvb::kKv4MergeWarps),
@@ -387,7 +400,7 @@ void accumulate_weights_kv4(const Kv4Pool& pool, const Kv4Query& q, const float*
     throw std::invalid_argument("weight_stride must be at least max_tokens");
   if (prm.max_tokens == 0) return;
   const uint32_t cols = segment_columns(pool, q), groups = (q.rows * prm.group + cols - 1) / cols;
-  const Kv4Kernel k = has_rules(pool, q) ? weigh_kernel<true>(pool.dim, cols) : weigh_kernel<false>(pool.dim, cols);
+  const Kv4Kernel k = weigh_kernel(pool.dim, cols, rules_of(pool, q));
   prm.col_groups = 1;
   const uint32_t ctas = split_ctas(k, uint64_t(q.batch) * pool.kv_heads, prm.max_tokens);
   prm.workers = ctas * kvb::kKv4Warps;

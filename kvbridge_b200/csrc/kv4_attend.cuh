@@ -51,6 +51,10 @@ constexpr int kv4_q_tiles(int cols) { return cols == 4 ? 1 : 2; }       // m16 t
 constexpr int kv4_p_tiles(int digits) { return digits == 3 ? 2 : 1; }   // and of the output
 constexpr int kv4_tokens(int cols) { return cols == 4 ? 8 : 16; }       // of a stage, a lane
 
+// What a kernel knows of the score rule: causal by index alone; also window
+// and prefix by index; or everything (cap, bias, explicit positions).
+enum : int { kRulesNone = 0, kRulesMask = 1, kRulesAll = 2 };
+
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Threads = 32 * kKv4Warps;
 constexpr uint32_t kNoUnit = 0xffffffffu;
@@ -96,14 +100,14 @@ struct Kv4Cursor {
 
 // HINT: read before the wait for the preceding kernel, past L1; such values
 // only steer prefetches, or are compared with what the wait lets through.
-template <bool RULES, bool HINT = false>
+template <int RULES, bool HINT = false>
 __device__ __forceinline__ void kv4_load_sequence(const Kv4AttendParams& p, Kv4Cursor& c) {
   const uint32_t len = HINT ? __ldcg(p.seq_lens + c.b) : kv4_load(p.seq_lens + c.b);
   c.len = min(len, p.max_tokens);
   c.stages = (c.len + kStageTokens - 1) / kStageTokens;
   c.head = c.stages;
   c.skip = 0;
-  if (RULES && p.rule.window != 0 && p.pool.pos == nullptr && p.rule.q_pos == nullptr) {
+  if (RULES != kRulesNone && p.rule.window != 0 && p.pool.pos == nullptr && p.rule.q_pos == nullptr) {
     // The first row's window starts at len - rows - window + 1.
     const uint64_t reach = uint64_t(p.rows) + p.rule.window - 1;
     const uint32_t from = reach < c.len ? uint32_t(c.len - reach) / kStageTokens : 0u;
@@ -117,7 +121,7 @@ __device__ __forceinline__ void kv4_load_sequence(const Kv4AttendParams& p, Kv4C
   }
 }
 
-template <bool RULES>
+template <int RULES>
 __device__ __forceinline__ uint32_t kv4_stage_count(const Kv4AttendParams& p, uint32_t b) {
   Kv4Cursor c;
   c.b = b;
@@ -126,7 +130,7 @@ __device__ __forceinline__ uint32_t kv4_stage_count(const Kv4AttendParams& p, ui
 }
 
 // The next segment that has stages (b = batch at the end).
-template <bool RULES>
+template <int RULES>
 __device__ __forceinline__ void kv4_next_segment(const Kv4AttendParams& p, uint32_t segs, Kv4Cursor& c) {
   c.base += int32_t(c.stages);
   if (++c.seg < segs) return;
@@ -179,7 +183,7 @@ __device__ __forceinline__ uint32_t kv4_locate_lanes(const Kv4AttendParams& p, u
 }
 
 // The same for more sequences, or for a direct call (worker w = segment w).
-template <bool RULES>
+template <int RULES>
 __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t w, uint32_t segs, Kv4Cursor& c) {
   const uint32_t lane = threadIdx.x & 31;
   if (p.direct) {
@@ -223,7 +227,7 @@ __device__ uint32_t kv4_locate(const Kv4AttendParams& p, uint32_t w, uint32_t se
 // sequences are located before it, from lengths that are only taken if they
 // are the same after it; the first stage's pages, the next one's table entries
 // and the query rows are prefetched into L2 meanwhile.
-template <int D, bool V, bool RULES>
+template <int D, bool V, int RULES>
 __device__ __forceinline__ uint32_t kv4_start(const Kv4AttendParams& p, uint32_t w, uint32_t segs, uint32_t cols,
                                               Kv4Cursor& c) {
   const uint32_t lane = threadIdx.x & 31;
@@ -295,7 +299,7 @@ __device__ __forceinline__ uint32_t kv4_v_pitch(uint32_t page_bytes, uint32_t P)
   return P == 64 ? page_bytes : page_bytes + 2 * P;
 }
 
-template <int D, bool V, bool RULES>
+template <int D, bool V, int RULES>
 struct Kv4Feeder {
   uint8_t* slots;
   uint32_t addr;   // of slots, in shared memory
@@ -463,7 +467,7 @@ __device__ __forceinline__ uint32_t kv4_word_dim(uint32_t tig, uint32_t i) {
   return (D / 4) * tig + 8 * i;
 }
 
-template <int D, int C, bool RULES>
+template <int D, int C, int RULES>
 __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h, uint32_t col_group,
                                uint32_t len, Kv4Query<D, C>& qf) {
   const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
@@ -538,13 +542,13 @@ __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
     }
   total += __shfl_xor_sync(0xffffffffu, total, 1);
   total += __shfl_xor_sync(0xffffffffu, total, 2);
-  // Scores in log2 units, or in natural ones where rules come after.
-  const float unit = RULES ? p.rule.scale : p.rule.scale * kLog2e;
+  // Scores in log2 units, or in natural ones where a cap or a bias comes after.
+  const float unit = RULES == kRulesAll ? p.rule.scale : p.rule.scale * kLog2e;
   const float dot = down * unit + wild;
   qf.own = C == 4 && grp >= 4 ? 65536.f * dot : dot;
   qf.other = C == 4 && grp >= 4 ? dot : 65536.f * dot;
   qf.sum = float(total) * dot;
-  qf.slope = RULES && p.rule.slopes != nullptr ? kv4_load(p.rule.slopes + head) : 0.f;
+  qf.slope = RULES == kRulesAll && p.rule.slopes != nullptr ? kv4_load(p.rule.slopes + head) : 0.f;
   qf.pos = valid ? kv4_query_position(p.rule, b, r, p.rows, len) : -1;
 }
 
@@ -635,22 +639,22 @@ __device__ __forceinline__ float kv4_cap(float x, float cap, float inv_cap) {
   return cap * (y2 < 0.09f ? near : far);
 }
 
-// exp(x - y) of scores x and y: log2 units without rules, natural units with
-// them (differences are small where the result is not).
-template <bool RULES>
+// exp(x - y) of scores x and y: in natural units with kRulesAll (differences
+// are small where the result is not), else in log2 units.
+template <int RULES>
 __device__ __forceinline__ float kv4_exp(float x, float y) {
-  return fast_exp2(RULES ? (x - y) * kLog2e : x - y);
+  return fast_exp2(RULES == kRulesAll ? (x - y) * kLog2e : x - y);
 }
 
 // Which tokens of the stage at tb every query row sees, by their indices:
 // those below the first row's position (and below the prefix), if they are
 // within the last row's window. A warp-uniform test that spares most stages
 // the masks. first, last: the rows' positions.
-template <bool RULES>
+template <int RULES>
 __device__ __forceinline__ bool kv4_all_visible(const Kv4AttendParams& p, uint32_t tb, uint32_t len, uint32_t prefix) {
   const int32_t first = int32_t(len) - int32_t(p.rows), end = int32_t(tb + kStageTokens);
-  if (!RULES) return end <= first + 1;
-  if (p.rule.q_pos != nullptr) return false;
+  if (RULES == kRulesNone) return end <= first + 1;
+  if (RULES == kRulesAll && p.rule.q_pos != nullptr) return false;
   if (uint32_t(end) <= min(prefix, len)) return true;
   return end <= first + 1 && (p.rule.window == 0 || uint32_t(int32_t(len) - 1 - int32_t(tb)) < p.rule.window);
 }
@@ -659,7 +663,7 @@ __device__ __forceinline__ bool kv4_all_visible(const Kv4AttendParams& p, uint32
 // visible tokens as a bit mask. tb: the stage's first token; all: every token
 // is visible; pos: the positions of the thread's quad's 16 tokens, or null for
 // their indices.
-template <int C, bool RULES>
+template <int C, int RULES>
 __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const uint8_t* params, uint32_t tb,
                                                uint32_t len, uint32_t prefix, bool all, float sum, float slope,
                                                int32_t pq, const int32_t* pos, float (&sc)[kv4_tokens(C)]) {
@@ -673,8 +677,8 @@ __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const u
     sc[u + 1] = fmaf(sc[u + 1], f.z, fmaf(8.f, f.z, f.w) * sum);
   }
   const int32_t t0 = int32_t(tb + at);
-  int32_t pk[RULES ? kTokens : 1];
-  if constexpr (RULES) {
+  int32_t pk[RULES == kRulesAll ? kTokens : 1];
+  if constexpr (RULES == kRulesAll) {
     if (p.rule.softcap > 0.f) {
       const float cap = p.rule.softcap, inv_cap = 1.0f / cap;
 #pragma unroll
@@ -700,7 +704,9 @@ __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const u
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
       const int32_t t = t0 + int32_t(kv4_token(C, u));
-      const bool on = RULES ? uint32_t(t) < len && kv4_visible(pk[u], pq, p.rule.window, prefix) : t <= pq;  // pq < len
+      bool on = t <= pq;  // pq < len
+      if constexpr (RULES != kRulesNone)
+        on = uint32_t(t) < len && kv4_visible(RULES == kRulesAll ? pk[u] : t, pq, p.rule.window, prefix);
       sc[u] = on ? sc[u] : -INFINITY;
       seen |= on ? 1u << u : 0u;
     }
@@ -726,7 +732,7 @@ __device__ __forceinline__ float kv4_max(const float (&x)[N]) {
   return fmaxf(y, x[N - 1]);
 }
 
-template <int D, int C, int PD, bool RULES, bool MASK>
+template <int D, int C, int PD, int RULES, bool MASK>
 __device__ __forceinline__ void kv4_softmax(const uint8_t* vparams, uint32_t seen, float (&sc)[kv4_tokens(C)],
                                             Kv4State<D>& st, uint32_t (&digit)[kv4_p_tiles(PD)][2][4],
                                             float& out_scale) {
@@ -864,8 +870,8 @@ __device__ __forceinline__ void kv4_store_out(void* out, size_t at, int32_t type
 
 // o / l; zero for a row that saw nothing, NaN where l is.
 __device__ __forceinline__ float kv4_normalised(float o, float l) { return l == 0.f ? 0.f : o / l; }
-__device__ __forceinline__ float kv4_lse(float m, float l, bool rules) {
-  return l == 0.f ? -INFINITY : rules ? m + logf(l) : (m + log2f(l)) * kLn2;
+__device__ __forceinline__ float kv4_lse(float m, float l, bool natural) {
+  return l == 0.f ? -INFINITY : natural ? m + logf(l) : (m + log2f(l)) * kLn2;
 }
 
 // Four neighbouring outputs; their alignment is only that of the buffer.
@@ -920,7 +926,7 @@ __device__ __forceinline__ void kv4_report_lengths(const Kv4AttendParams& p) {
     if (kv4_load(p.seq_lens + b) > p.max_tokens) atomicMax(&g_kvb_status, kKv4LenClamped);
 }
 
-template <int D, int C, int PD, int MINB, bool RULES>
+template <int D, int C, int PD, int MINB, int RULES>
 __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4AttendParams p) {
   using S = Kv4Smem<D, true>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -963,7 +969,7 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
     for (; done < end; ++done) {
       const uint32_t j = uint32_t(int32_t(done) - cur.base);
       const uint32_t tb = (RULES && j >= cur.head ? j + cur.skip : j) * kStageTokens;
-      const int32_t* pos = RULES ? kv4_positions(p, cur.b, h, cur.len, tb) : nullptr;
+      const int32_t* pos = RULES == kRulesAll ? kv4_positions(p, cur.b, h, cur.len, tb) : nullptr;
       copy_wait<1>();  // K has landed, V may be on its way
       __syncwarp();
       float sc[kv4_tokens(C)];
@@ -1010,7 +1016,7 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
       if (whole) {
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) kv4_store_out4(p.out, index * D + 16 * j + 4 * tig, p.type, st.o[j], st.l);
-        if (tig == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(st.m, st.l, RULES);
+        if (tig == 0 && p.lse != nullptr) p.lse[index] = kv4_lse(st.m, st.l, RULES == kRulesAll);
       } else {
         const size_t at = size_t(worker + segment) * C + grp;
 #pragma unroll
@@ -1051,7 +1057,7 @@ __device__ __forceinline__ void kv4_add_partial(const float* src, float f, float
   }
 }
 
-template <int D, bool RULES, bool MANY>
+template <int D, int RULES, bool MANY>
 __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv4AttendParams p, uint32_t cols) {
   __shared__ float sum[MANY ? kKv4MergeWarps : 1][MANY ? D : 1];
   __shared__ float weight[MANY ? 32 * kKv4MergeWarps : 1], part_max[kKv4MergeWarps], part_sum[kKv4MergeWarps];
@@ -1130,7 +1136,7 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv
     }
     if (lane != 0) return;
   }
-  if (p.lse != nullptr) p.lse[index] = kv4_lse(top, l, RULES);
+  if (p.lse != nullptr) p.lse[index] = kv4_lse(top, l, RULES == kRulesAll);
 }
 
 // ---------------------------------------------------------------------------
@@ -1139,7 +1145,7 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv
 // one thread adds up a token's weight in a fixed order, so there are no
 // atomics, and the groups' launches follow one another.
 
-template <int D, int C, int MINB, bool RULES>
+template <int D, int C, int MINB, int RULES>
 __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4AttendParams p, uint32_t group) {
   using S = Kv4Smem<D, false>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -1170,14 +1176,14 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
     if (col < p.rows * p.group) {
       const float x = kv4_load(p.lse_in + (size_t(cur.b) * p.rows + col / p.group) * p.q_heads + cur.seg * p.group +
                             col % p.group);
-      if (x != -INFINITY) lse = RULES ? x : x * kLog2e;
+      if (x != -INFINITY) lse = RULES == kRulesAll ? x : x * kLog2e;
     }
     const uint32_t prefix = RULES && p.rule.prefix != nullptr ? kv4_load(p.rule.prefix + cur.b) : 0u;
     float* weights = p.weights + (int64_t(cur.b) * p.pool.kv_heads + cur.seg) * p.weight_stride;
     for (; done < end; ++done) {
       const uint32_t j = uint32_t(int32_t(done) - cur.base);
       const uint32_t tb = (RULES && j >= cur.head ? j + cur.skip : j) * kStageTokens;
-      const int32_t* pos = RULES ? kv4_positions(p, cur.b, cur.seg, cur.len, tb) : nullptr;
+      const int32_t* pos = RULES == kRulesAll ? kv4_positions(p, cur.b, cur.seg, cur.len, tb) : nullptr;
       // After the reduction below this lane holds token t0 and the next.
       const uint32_t t0 = tb + 16 * tig + (C == 8 ? 2 * grp : 8 * (grp >> 1 & 1) + 4 * (grp >> 2) + 2 * (grp & 1));
       const float old0 = t0 < cur.len ? weights[t0] : 0.f, old1 = t0 + 1 < cur.len ? weights[t0 + 1] : 0.f;
