@@ -625,18 +625,30 @@ __device__ __forceinline__ void kv4_dots(const uint8_t* codes, const Kv4Query<D,
   }
 }
 
-// softcap * tanh(x / softcap).
-__device__ __forceinline__ float kv4_cap(float x, float cap, float inv_cap) {
-  const float y = x * inv_cap;
-  // tanh y = 1 - 2 / (e^2y + 1); near 0, where that cancels, its series.
-  const float u = fast_exp2(y * (2.0f * kLog2e));
-  const float far = 1.0f - __fdividef(2.0f, u + 1.0f);
-  const float y2 = y * y;
-  float s = fmaf(y2, 62.0f / 2835.0f, -17.0f / 315.0f);
-  s = fmaf(s, y2, 2.0f / 15.0f);
-  s = fmaf(s, y2, -1.0f / 3.0f);
-  const float near = fmaf(s * y2, y, y);
-  return cap * (y2 < 0.09f ? near : far);
+// x = softcap * tanh(x / softcap): the series where |x / softcap| < 0.3, which
+// is all of most stages, else 1 - 2 / (e^2y + 1), which cancels near 0.
+template <int N>
+__device__ __forceinline__ void kv4_cap(float cap, float (&x)[N]) {
+  const float inv = 1.0f / cap;
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(x[i]));  // (a NaN takes either way)
+  const bool far = __any_sync(0xffffffffu, top * inv >= 0.3f);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = x[i] * inv, y2 = y * y;
+    float s = fmaf(y2, 62.0f / 2835.0f, -17.0f / 315.0f);
+    s = fmaf(s, y2, 2.0f / 15.0f);
+    s = fmaf(s, y2, -1.0f / 3.0f);
+    const float near = fmaf(x[i], s * y2, x[i]);
+    if (far) {
+      const float u = fast_exp2(y * (2.0f * kLog2e));
+      const float t = 1.0f - __fdividef(2.0f, u + 1.0f);
+      x[i] = fabsf(y) < 0.3f ? near : cap * t;
+    } else {
+      x[i] = near;
+    }
+  }
 }
 
 // exp(x - y) of scores x and y: in natural units with kRulesAll (differences
@@ -679,11 +691,7 @@ __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const u
   const int32_t t0 = int32_t(tb + at);
   int32_t pk[RULES == kRulesAll ? kTokens : 1];
   if constexpr (RULES == kRulesAll) {
-    if (p.rule.softcap > 0.f) {
-      const float cap = p.rule.softcap, inv_cap = 1.0f / cap;
-#pragma unroll
-      for (int u = 0; u < kTokens; ++u) sc[u] = kv4_cap(sc[u], cap, inv_cap);
-    }
+    if (p.rule.softcap > 0.f) kv4_cap(p.rule.softcap, sc);
     if (pos != nullptr) {
 #pragma unroll
       for (int u = 0; u < kTokens; ++u) pk[u] = kv4_load(pos + (at & 15) + kv4_token(C, u));
@@ -691,11 +699,18 @@ __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const u
 #pragma unroll
       for (int u = 0; u < kTokens; ++u) pk[u] = t0 + int32_t(kv4_token(C, u));
     }
+    // Distances are exact in fp32 below 2^24. Positions of rows may be
+    // negative: |pq - pk| as the larger minus the smaller.
     if (p.rule.slopes != nullptr) {
-      // Distances are exact in fp32 below 2^24; |pq - pk| as the larger minus the smaller.
+      if (pos != nullptr) {
 #pragma unroll
-      for (int u = 0; u < kTokens; ++u)
-        sc[u] = fmaf(-slope, float(uint32_t(max(pq, pk[u])) - uint32_t(min(pq, pk[u]))), sc[u]);
+        for (int u = 0; u < kTokens; ++u)
+          sc[u] = fmaf(-slope, float(uint32_t(max(pq, pk[u])) - uint32_t(min(pq, pk[u]))), sc[u]);
+      } else {
+        const float away = float(int64_t(pq) - t0);
+#pragma unroll
+        for (int u = 0; u < kTokens; ++u) sc[u] = fmaf(-slope, fabsf(away - float(kv4_token(C, u))), sc[u]);
+      }
     }
   }
   uint32_t seen = (1u << kTokens) - 1;
@@ -816,23 +831,19 @@ __device__ __forceinline__ void kv4_output(const uint8_t* codes, uint32_t P, uin
   const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
   const uint8_t* base = codes + (16 * tig / P) * pitch + (16 * tig % P) + grp * P;
   const float odd_scale = out_scale * 0.0625f;
-  // -8 * (sum of the row's digits): rows grp and grp + 8 of every tile.
+  // -8 * (sum of the row's digits), rows grp and grp + 8 of every tile: the
+  // product with ones has it in every column.
   int start[kv4_p_tiles(PD)][2], start16[kv4_p_tiles(PD)][2];
 #pragma unroll
-  for (int m = 0; m < kv4_p_tiles(PD); ++m)
+  for (int m = 0; m < kv4_p_tiles(PD); ++m) {
+    const uint32_t(&a)[2][4] = digit[m];
+    constexpr uint32_t kOnes = 0x01010101u;
+    int s[4];
+    imma_u8_16832(s, a[0][0], a[0][1], a[0][2], a[0][3], kOnes, kOnes, 0, 0, 0, 0);
+    imma_u8_16832(s, a[1][0], a[1][1], a[1][2], a[1][3], kOnes, kOnes, s[0], s[1], s[2], s[3]);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      uint32_t s = 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s = __dp4a(digit[m][i][r], 0x01010101u, s);
-        s = __dp4a(digit[m][i][2 + r], 0x01010101u, s);
-      }
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      start[m][r] = -8 * int(s);
-      start16[m][r] = -128 * int(s);
-    }
+    for (int r = 0; r < 2; ++r) start[m][r] = -8 * s[2 * r], start16[m][r] = -128 * s[2 * r];
+  }
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) {
     const uint4 w = *reinterpret_cast<const uint4*>(base + 8 * j * P);
