@@ -402,46 +402,13 @@ __device__ __forceinline__ void kv4_half_pair(uint32_t w, bool bf16, float& a, f
   }
 }
 
-// N runs of eight query values, run i from element at + step(i). Every load
-// is issued before any is used: one memory round trip.
-template <int N, class F>
-__device__ __forceinline__ void kv4_load_values(const void* q, int64_t at, F&& step, int32_t type, bool vector,
-                                                float (&v)[N][8]) {
-  if (!vector) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int64_t x = at + step(i) + e;
-        if (type == 0) {
-          v[i][e] = kv4_load(static_cast<const float*>(q) + x);
-        } else {
-          float unused;
-          kv4_half_pair(kv4_load(static_cast<const uint16_t*>(q) + x), type == 2, v[i][e], unused);
-        }
-      }
-  } else if (type == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + step(i));
-      const float4 a = kv4_load(src), b = kv4_load(src + 1);
-      v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w, v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z,
-      v[i][7] = b.w;
-    }
-  } else {
-    uint4 raw[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      raw[i] = kv4_load(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + at + step(i)));
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      kv4_half_pair(raw[i].x, type == 2, v[i][0], v[i][1]);
-      kv4_half_pair(raw[i].y, type == 2, v[i][2], v[i][3]);
-      kv4_half_pair(raw[i].z, type == 2, v[i][4], v[i][5]);
-      kv4_half_pair(raw[i].w, type == 2, v[i][6], v[i][7]);
-    }
-  }
-}
+// Eight values of each word of a lane's part of a query row, as they lie in
+// memory: loads in flight until they are used. Rows that are not 16-byte
+// aligned are read where the values are wanted.
+template <int D>
+struct Kv4RawQuery {
+  uint4 w[D / 32][2];  // 16-bit values: the first alone
+};
 
 // The A operand of the scores for one group of columns. Lane (grp, tig) =
 // (lane / 4, lane % 4) holds column grp (4 columns: grp % 4) at the dims of its
@@ -467,29 +434,79 @@ __device__ __forceinline__ uint32_t kv4_word_dim(uint32_t tig, uint32_t i) {
   return (D / 4) * tig + 8 * i;
 }
 
-template <int D, int C, int RULES>
-__device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h, uint32_t col_group,
-                               uint32_t len, Kv4Query<D, C>& qf) {
-  const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
-  const uint32_t col = col_group * C + grp % C;
+// Where a lane's column of a segment is: the query row's first element.
+template <int D, int C>
+__device__ __forceinline__ bool kv4_query_at(const Kv4AttendParams& p, uint32_t b, uint32_t h, uint32_t col_group,
+                                             uint32_t& r, uint32_t& head, int64_t& at) {
+  const uint32_t col = col_group * C + ((threadIdx.x & 31) >> 2) % C;
   const bool valid = col < p.rows * p.group;
-  const uint32_t r = valid ? col / p.group : 0, head = h * p.group + (valid ? col % p.group : 0);
-  const int64_t at = int64_t(b) * p.batch_stride + int64_t(r) * p.row_stride + int64_t(head) * D;
+  r = valid ? col / p.group : 0;
+  head = h * p.group + (valid ? col % p.group : 0);
+  at = int64_t(b) * p.batch_stride + int64_t(r) * p.row_stride + int64_t(head) * D;
+  return valid;
+}
+
+template <int D, int C>
+__device__ __forceinline__ void kv4_fetch_query(const Kv4AttendParams& p, uint32_t b, uint32_t h, uint32_t col_group,
+                                                Kv4RawQuery<D>& raw) {
+  if (!p.vector_q) return;
+  uint32_t r, head;
+  int64_t at;
+  kv4_query_at<D, C>(p, b, h, col_group, r, head, at);
+  const int bytes = p.type == 0 ? 4 : 2;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.q) +
+                                                      (at + kv4_word_dim<D>(threadIdx.x & 3, i)) * bytes);
+    raw.w[i][0] = kv4_load(src);
+    if (p.type == 0) raw.w[i][1] = kv4_load(src + 1);
+  }
+}
+
+template <int D, int C, int RULES>
+__device__ void kv4_make_query(const Kv4AttendParams& p, uint32_t b, uint32_t h, uint32_t col_group, uint32_t len,
+                               const Kv4RawQuery<D>& raw, Kv4Query<D, C>& qf) {
+  const uint32_t lane = threadIdx.x & 31, grp = lane >> 2, tig = lane & 3;
+  uint32_t r, head;
+  int64_t at;
+  const bool valid = kv4_query_at<D, C>(p, b, h, col_group, r, head, at);
   float v[D / 32][8];
-  kv4_load_values(p.q, at, [&](int i) { return int64_t(kv4_word_dim<D>(tig, i)); }, p.type, p.vector_q, v);
-  float amax = 0.f;
-  float wild = 0.f;  // NaN where a value is not finite
+  if (!p.vector_q) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t x = at + kv4_word_dim<D>(tig, i) + e;
+        float unused;
+        if (p.type == 0) v[i][e] = kv4_load(static_cast<const float*>(p.q) + x);
+        else kv4_half_pair(kv4_load(static_cast<const uint16_t*>(p.q) + x), p.type == 2, v[i][e], unused);
+      }
+  } else if (p.type == 0) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint4 w = raw.w[i][k];
+        v[i][4 * k] = __uint_as_float(w.x), v[i][4 * k + 1] = __uint_as_float(w.y);
+        v[i][4 * k + 2] = __uint_as_float(w.z), v[i][4 * k + 3] = __uint_as_float(w.w);
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const uint4 w = raw.w[i][0];
+      kv4_half_pair(w.x, p.type == 2, v[i][0], v[i][1]);
+      kv4_half_pair(w.y, p.type == 2, v[i][2], v[i][3]);
+      kv4_half_pair(w.z, p.type == 2, v[i][4], v[i][5]);
+      kv4_half_pair(w.w, p.type == 2, v[i][6], v[i][7]);
+    }
+  }
+  float amax = 0.f;  // NaN if a value is
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      wild = fmaf(v[i][e], 0.f, wild);
-      amax = fmaxf(amax, fabsf(v[i][e]));
-    }
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  wild += __shfl_xor_sync(0xffffffffu, wild, 1);
-  wild += __shfl_xor_sync(0xffffffffu, wild, 2);
+    for (int e = 0; e < 8; e += 2) amax = max3_abs_nan(amax, v[i][e], v[i][e + 1]);
+  amax = max3_abs_nan(amax, amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = max3_abs_nan(amax, amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   // Fixed point n = rint(q * up), |n| <= 2^22: n = d0 + 256 d1 + 65536 d2
   // with signed digits; up is a power of two.
   int e = int((__float_as_uint(amax) >> 23) & 0xffu) - 126;  // amax < 2^e
@@ -501,17 +518,13 @@ __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
   // bytes are the digits + 128.
   constexpr float kRoundInt = 12582912.0f;
   constexpr uint32_t kBias = 0x808080u - 0x4B400000u;
-  int total = 0;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int odd = 0; odd < 2; ++odd) {
       uint32_t w[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        w[x] = valid ? __float_as_uint(fmaf(v[i][2 * x + odd], up, kRoundInt)) + kBias : 0x808080u;
-        total += int(w[x]) - 0x808080;
-      }
+      for (int x = 0; x < 4; ++x) w[x] = valid ? __float_as_uint(fmaf(v[i][2 * x + odd], up, kRoundInt)) + kBias : 0x808080u;
       const uint32_t x = __byte_perm(w[0], w[1], 0x5140), y = __byte_perm(w[2], w[3], 0x5140);
       const uint32_t d0 = __byte_perm(x, y, 0x5410) ^ 0x80808080u, d1 = __byte_perm(x, y, 0x7632) ^ 0x80808080u;
       const uint32_t x2 = __byte_perm(w[0], w[1], 0x0062), y2 = __byte_perm(w[2], w[3], 0x0062);
@@ -540,11 +553,18 @@ __device__ void kv4_load_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
       s += __shfl_xor_sync(0xffffffffu, s, 2);
       qf.start[m][r] = -8 * s;
     }
-  total += __shfl_xor_sync(0xffffffffu, total, 1);
-  total += __shfl_xor_sync(0xffffffffu, total, 2);
+  // sum of n, from the digit sums; exact: |n| <= 2^22, 256 of them.
+  int total = qf.start[0][0] + 256 * qf.start[0][1];
+  if constexpr (C == 8) {
+    total += 65536 * qf.start[1][0];
+  } else {
+    const int other = __shfl_xor_sync(0xffffffffu, total, 16);  // the upper lane has digit 2
+    total = grp >= 4 ? 65536 * total + other : total + 65536 * other;
+  }
+  total /= -8;
   // Scores in log2 units, or in natural ones where a cap or a bias comes after.
   const float unit = RULES == kRulesAll ? p.rule.scale : p.rule.scale * kLog2e;
-  const float dot = down * unit + wild;
+  const float dot = amax <= 3.402823466e38f ? down * unit : __int_as_float(0x7fffffff);
   qf.own = C == 4 && grp >= 4 ? 65536.f * dot : dot;
   qf.other = C == 4 && grp >= 4 ? dot : 65536.f * dot;
   qf.sum = float(total) * dot;
@@ -955,7 +975,9 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
   feed.next = 0;
   feed.count = count;
   feed.segs = segs;
+  Kv4RawQuery<D> raw;
   feed.lookup(p);
+  kv4_fetch_query<D, C>(p, cur.b, cur.seg / p.col_groups, cur.seg % p.col_groups, raw);
   if (count != 0) {
     feed.template copy<false>(p);
     feed.template copy<true>(p);
@@ -968,7 +990,7 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
     const uint32_t first = done, end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
     const uint32_t h = cur.seg / p.col_groups;
     Kv4Query<D, C> qf;
-    kv4_load_query<D, C, RULES>(p, cur.b, h, cur.seg % p.col_groups, cur.len, qf);
+    kv4_make_query<D, C, RULES>(p, cur.b, h, cur.seg % p.col_groups, cur.len, raw, qf);
     const uint32_t prefix = RULES && p.rule.prefix != nullptr ? kv4_load(p.rule.prefix + cur.b) : 0u;
     Kv4State<D> st;
 #pragma unroll
@@ -1041,35 +1063,45 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
       if (int32_t(first) == cur.base) p.seg_warps[segment].x = worker;
       if (int32_t(end) == cur.base + int32_t(cur.stages)) p.seg_warps[segment].y = worker;
     }
-    if (done < count) kv4_next_segment<RULES>(p, segs, cur);
+    if (done < count) {
+      kv4_next_segment<RULES>(p, segs, cur);
+      kv4_fetch_query<D, C>(p, cur.b, cur.seg / p.col_groups, cur.seg % p.col_groups, raw);
+    }
   } while (done < count);
 }
 
-// The partials of one output row (sequence, row, head). Bound by latency: a
-// row's loads are a chain of the segment's warps, then the maxima and sums of
-// all partials at once, then their values. Many partials a row: a CTA's 16
-// warps share a row, a thread per partial for the weights; few: a warp a row,
-// a lane per partial.
+// The partials of one output row (sequence, row, head). Bound by latency: two
+// round trips, the segment's warps and then eight of a row's partials a warp
+// with their maxima and sums. Many partials a row: a CTA's 16 warps
+// share a row, a thread per partial for the weights; few: a warp a row, a lane
+// per partial.
 constexpr int kKv4MergeWarps = 16;
 
 template <int D>
-__device__ __forceinline__ void kv4_add_partial(const float* src, float f, float (&o)[D / 32]) {
-  const uint32_t lane = threadIdx.x & 31;
-  if constexpr (D == 64) {
-    const float2 x = __ldcg(reinterpret_cast<const float2*>(src) + lane);
-    o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]);
-  } else {
+struct Kv4Partial {
+  static constexpr int kPer = D / 32;  // consecutive dims of a lane
+  float x[kPer];
+  __device__ __forceinline__ void load(const float* src) {
+    const uint32_t lane = threadIdx.x & 31;
+    if constexpr (D == 64) {
+      const float2 y = __ldcg(reinterpret_cast<const float2*>(src) + lane);
+      x[0] = y.x, x[1] = y.y;
+    } else {
 #pragma unroll
-    for (int k = 0; k < D / 128; ++k) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(src) + lane * (D / 128) + k);
-      o[4 * k] = fmaf(x.x, f, o[4 * k]), o[4 * k + 1] = fmaf(x.y, f, o[4 * k + 1]);
-      o[4 * k + 2] = fmaf(x.z, f, o[4 * k + 2]), o[4 * k + 3] = fmaf(x.w, f, o[4 * k + 3]);
+      for (int k = 0; k < D / 128; ++k) {
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(src) + lane * (D / 128) + k);
+        x[4 * k] = y.x, x[4 * k + 1] = y.y, x[4 * k + 2] = y.z, x[4 * k + 3] = y.w;
+      }
     }
   }
-}
+  __device__ __forceinline__ void add_to(float (&o)[kPer], float f) const {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) o[k] = fmaf(x[k], f, o[k]);
+  }
+};
 
 template <int D, int RULES, bool MANY>
-__global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv4AttendParams p, uint32_t cols) {
+__global__ void __launch_bounds__(32 * kKv4MergeWarps, 2) merge_kv4_kernel(const Kv4AttendParams p, uint32_t cols) {
   __shared__ float sum[MANY ? kKv4MergeWarps : 1][MANY ? D : 1];
   __shared__ float weight[MANY ? 32 * kKv4MergeWarps : 1], part_max[kKv4MergeWarps], part_sum[kKv4MergeWarps];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1086,36 +1118,47 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv
   if (any && range.x == range.y) return;  // written by its warp
   const uint32_t n = any ? range.y - range.x + 1 : 0u;
   const size_t first = size_t(range.x + segment) * cols + c;
-  constexpr int kPer = D / 32;  // consecutive dims of a lane
+  constexpr int kPer = D / 32;
+  // Partials a warp has in flight. 64 registers a thread, so that a CTA can
+  // start on an SM beside the attention's last ones.
+  constexpr int kHeld = D == 256 ? 4 : 8;
+  constexpr uint32_t kRound = MANY ? kHeld * kKv4MergeWarps : kHeld, kStep = MANY ? kKv4MergeWarps : 1;
   float o[kPer] = {}, top = -INFINITY, l = 0.f;
-  if constexpr (MANY) {
-    for (uint32_t from = 0; from < n; from += 32 * kKv4MergeWarps) {
-      const uint32_t here = min(n - from, uint32_t(32 * kKv4MergeWarps));
-      const float2 ml = tid < here ? __ldcg(p.part_ml + first + size_t(from + tid) * cols) : make_float2(-INFINITY, 0.f);
-      float m = warp_max(ml.x);
+  for (uint32_t from = 0; from < n; from += kRound) {
+    const uint32_t here = min(n - from, kRound), mine = MANY ? tid : lane, start = MANY ? warp : 0u;
+    const float2 ml = mine < here ? __ldcg(p.part_ml + first + size_t(from + mine) * cols) : make_float2(-INFINITY, 0.f);
+    Kv4Partial<D> held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (start + i * kStep < here) held[i].load(p.part + (first + size_t(from + start + i * kStep) * cols) * D);
+    float m = warp_max(ml.x);
+    if constexpr (MANY) {
       if (lane == 0) part_max[warp] = m;
       __syncthreads();
-      m = top;
-#pragma unroll
-      for (int w = 0; w < kKv4MergeWarps; ++w) m = fmaxf(m, part_max[w]);
-      const float sub = m == -INFINITY ? 0.f : m;
-      const float f = kv4_exp<RULES>(ml.x, sub);
-      weight[tid] = f;
-      const float s = warp_sum(ml.y * f);
-      if (lane == 0) part_sum[warp] = s;
-      const float alpha = kv4_exp<RULES>(top, sub);
-      l *= alpha;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) o[k] *= alpha;
-      top = m;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kKv4MergeWarps; ++w) l += part_sum[w];
-#pragma unroll 8
-      for (uint32_t i = warp; i < here; i += kKv4MergeWarps)
-        kv4_add_partial<D>(p.part + (first + size_t(from + i) * cols) * D, weight[i], o);
-      __syncthreads();
+      m = warp_max(lane < kKv4MergeWarps ? part_max[lane] : -INFINITY);
     }
+    m = fmaxf(m, top);
+    const float sub = m == -INFINITY ? 0.f : m;
+    const float f = kv4_exp<RULES>(ml.x, sub), alpha = kv4_exp<RULES>(top, sub);
+    top = m;
+    float s = warp_sum(ml.y * f);
+    if constexpr (MANY) {
+      weight[tid] = f;
+      if (lane == 0) part_sum[warp] = s;
+      __syncthreads();
+      s = warp_sum(lane < kKv4MergeWarps ? part_sum[lane] : 0.f);
+    }
+    l = fmaf(l, alpha, s);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) o[k] *= alpha;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const float g = MANY ? weight[(start + i * kStep) % (32 * kKv4MergeWarps)] : __shfl_sync(0xffffffffu, f, i);
+      if (start + i * kStep < here) held[i].add_to(o, g);
+    }
+    if constexpr (MANY) __syncthreads();  // the weights are read
+  }
+  if constexpr (MANY) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k) sum[warp][lane * kPer + k] = o[k];
     __syncthreads();
@@ -1127,24 +1170,9 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps) merge_kv4_kernel(const Kv
     }
     if (tid != 0) return;
   } else {
-    for (uint32_t from = 0; from < n; from += 32) {
-      const uint32_t here = min(n - from, 32u);
-      const float2 ml = lane < here ? __ldcg(p.part_ml + first + size_t(from + lane) * cols) : make_float2(-INFINITY, 0.f);
-      const float m = fmaxf(top, warp_max(ml.x)), sub = m == -INFINITY ? 0.f : m;
-      const float f = kv4_exp<RULES>(ml.x, sub), alpha = kv4_exp<RULES>(top, sub);
-      l = l * alpha + warp_sum(ml.y * f);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) o[k] *= alpha;
-      top = m;
-#pragma unroll 4
-      for (uint32_t i = 0; i < here; ++i)
-        kv4_add_partial<D>(p.part + (first + size_t(from + i) * cols) * D, __shfl_sync(0xffffffffu, f, i), o);
-    }
-#pragma unroll
-    for (int k = 0; k < kPer; k += 2) {
+    for (int k = 0; k < kPer; ++k)
       kv4_store_out(p.out, size_t(index) * D + lane * kPer + k, p.type, kv4_normalised(o[k], l));
-      kv4_store_out(p.out, size_t(index) * D + lane * kPer + k + 1, p.type, kv4_normalised(o[k + 1], l));
-    }
     if (lane != 0) return;
   }
   if (p.lse != nullptr) p.lse[index] = kv4_lse(top, l, RULES == kRulesAll);
@@ -1179,8 +1207,10 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
 
   while (done < count) {
     const uint32_t end = min(count, uint32_t(cur.base + int32_t(cur.stages)));
+    Kv4RawQuery<D> raw;
+    kv4_fetch_query<D, C>(p, cur.b, cur.seg, group, raw);
     Kv4Query<D, C> qf;
-    kv4_load_query<D, C, RULES>(p, cur.b, cur.seg, group, cur.len, qf);
+    kv4_make_query<D, C, RULES>(p, cur.b, cur.seg, group, cur.len, raw, qf);
     // Infinite: a column that is not there, or a row that saw nothing.
     float lse = INFINITY;
     const uint32_t col = group * C + grp % C;

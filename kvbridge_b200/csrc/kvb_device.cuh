@@ -236,6 +236,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return y;
 }
 
+// Largest magnitude of three; NaN if one is.
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 // 2^x on the MUFU unit (ex2.approx, denormal results flushed to zero).
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
