@@ -312,7 +312,7 @@ uint32_t split_ctas(const Kv4Kernel& k, uint64_t segments, uint32_t max_tokens) 
 struct AttendPlan {
   Kv4Kernel kernel;
   int rules;
-  bool direct, many;
+  bool direct, many, most;
   uint32_t cols, col_groups, segments, ctas, workers;
   size_t ml_offset, warps_offset, bytes;  // of the workspace
 };
@@ -340,6 +340,8 @@ AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
   a.workers = a.ctas * kvb::kKv4Warps;
   // A warp reads 32 partials a round; from about 24 on a CTA a row is faster.
   a.many = a.workers > 24 * a.segments;
+  // More than a round of eight a warp (1x64K tokens, 222 a row: 25.2 against 23.6 us).
+  a.most = a.workers > (pool.dim == 256 ? 64 : 128) * a.segments;
   const size_t slots = size_t(a.workers) + a.segments;
   a.ml_offset = slots * cols * pool.dim * sizeof(float);
   a.warps_offset = a.ml_offset + slots * cols * sizeof(float2);
@@ -381,8 +383,9 @@ void launch_attention_kv4(const Kv4Pool& pool, const Kv4Query& q, void* workspac
     constexpr int D = decltype(d)::value;
     return by_rules(a.rules, [&](auto r) {
       constexpr int RULES = decltype(r)::value;
-      return a.many ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, RULES, true>)
-                    : reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, RULES, false>);
+      return !a.many  ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, RULES, false, 8>)
+             : a.most ? reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, RULES, true, 16>)
+                      : reinterpret_cast<const void*>(&kvb::merge_kv4_kernel<D, RULES, true, 8>);
     });
   });
   const uint32_t rows = q.batch * q.rows * q.q_heads;
