@@ -116,16 +116,22 @@ kvb::Kv4RowsParams rows_params(const Kv4Pool& pool, const Kv4Rows& rows) {
                             vector};
 }
 
-// Tokens a CTA: 64, or 16 where that would leave SMs without one.
+// Tokens a CTA: 16 where 64 would leave SMs without one; else 64, but 32 to
+// append rows of dim 128, whose loads are then one batch a lane (65,536 bf16
+// tokens on 8 heads 114 us for 129; fp32 111 for 113; dims 64 and 256 the other
+// way round, 70 us for 85 and 235 for 294; to load, 64 is better at any dim).
 bool small_tiles(const Kv4Pool& pool, const Kv4Rows& rows) {
   return uint64_t((rows.tokens + 63) / 64) * pool.kv_heads < uint64_t(2 * detail::device_sms());
 }
 
+constexpr uint32_t append_tile(uint32_t dim) { return dim == 128 ? 32 : 64; }
+
 template <class Kernel>
-void launch_rows(const Kv4Pool& pool, const Kv4Rows& rows, cudaStream_t stream, const char* what, Kernel&& kernel) {
+void launch_rows(const Kv4Pool& pool, const Kv4Rows& rows, uint32_t large, cudaStream_t stream, const char* what,
+                 Kernel&& kernel) {
   kvb::Kv4RowsParams prm = rows_params(pool, rows);
   const bool small = small_tiles(pool, rows);
-  const uint32_t tile = small ? 16 : 64;
+  const uint32_t tile = small ? 16 : large;
   const void* fn = by_dim(pool.dim, [&](auto d) { return by_type(rows.type, [&](auto t) { return kernel(d, t, small); }); });
   void* args[] = {&prm};
   launch_kernel_pdl(fn, dim3((rows.tokens + tile - 1) / tile, pool.kv_heads), dim3(32 * kvb::kKv4StoreWarps), 0, stream,
@@ -138,17 +144,17 @@ void append_kv4(const Kv4Pool& pool, const Kv4Rows& rows, cudaStream_t stream) {
   if (!check_rows(pool, rows)) return;
   if (pool.positions != nullptr && rows.positions == nullptr)
     throw std::invalid_argument("the pool keeps positions: append_kv4 needs the rows' positions");
-  launch_rows(pool, rows, stream, "kv4 append launch", [](auto d, auto t, bool small) {
+  launch_rows(pool, rows, append_tile(pool.dim), stream, "kv4 append launch", [](auto d, auto t, bool small) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     return small ? reinterpret_cast<const void*>(&kvb::append_kv4_kernel<T, D, 16>)
-                 : reinterpret_cast<const void*>(&kvb::append_kv4_kernel<T, D, 64>);
+                 : reinterpret_cast<const void*>(&kvb::append_kv4_kernel<T, D, append_tile(D)>);
   });
 }
 
 void load_kv4(const Kv4Pool& pool, const Kv4Rows& rows, cudaStream_t stream) {
   if (!check_rows(pool, rows)) return;
-  launch_rows(pool, rows, stream, "kv4 load launch", [](auto d, auto t, bool small) {
+  launch_rows(pool, rows, 64, stream, "kv4 load launch", [](auto d, auto t, bool small) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     return small ? reinterpret_cast<const void*>(&kvb::load_kv4_kernel<T, D, 16>)
@@ -336,7 +342,9 @@ AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
     a.bytes = 16;
     return a;
   }
-  a.ctas = split_ctas(a.kernel, a.segments, q.max_tokens);
+  // At most 512 partials a segment: one KV head of 131,072 tokens takes 18.5 us
+  // so, 26.9 us with a full wave's 1,776 partials to merge.
+  a.ctas = std::min(split_ctas(a.kernel, a.segments, q.max_tokens), uint32_t(std::min<uint64_t>(128ull * a.segments, 0xffffffffull)));
   a.workers = a.ctas * kvb::kKv4Warps;
   // A warp reads 32 partials a round; from about 24 on a CTA a row is faster.
   a.many = a.workers > 24 * a.segments;
@@ -449,7 +457,8 @@ void select_tokens(const Kv4Eviction& e, int32_t* keep, uint32_t* kept_lens, cud
   kvb::SelectParams prm{e.seq_lens, e.weights,    e.weight_stride, keep,    kept_lens, e.batch,
                         e.kv_heads, e.max_tokens, e.budget,        e.sinks, e.recent};
   // CTAs a segment: one for every 2,048 tokens, at most the eight of a
-  // portable cluster, and no more than fill the SMs twice (16 x 16K tokens on
+  // portable cluster (sixteen are slower: 8,192 of 65,536 tokens 73 us for 51),
+  // and no more than fill the SMs twice (16 x 16K tokens on
   // 8 heads: 90 us in clusters of eight, whose shared histograms queue).
   uint32_t ctas = 1;
   while (ctas < 8 && uint64_t(ctas) * 2048 < e.max_tokens &&

@@ -167,12 +167,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // How a warp holds the V and then the K rows of its tokens: kRuns runs of
 // eight values a lane, run r of lane `part` being run part + r * kLanes of the
-// row; kBatch passes' loads are in flight together.
-template <class T, int D, int TILE>
+// row; kBatch passes' loads are in flight together (MOST runs of a lane).
+template <int D, int TILE, int MOST>
 struct Kv4RowMap {
   static constexpr int kRuns = D == 64 ? 1 : 2, kLanes = D / 8 / kRuns, kRows = 32 / kLanes;
   static constexpr int kWarpTokens = TILE / kKv4StoreWarps, kPasses = 2 * kWarpTokens / kRows;
-  static constexpr int kMost = (sizeof(T) == 2 ? 8 : 4) / kRuns;
+  static constexpr int kMost = MOST / kRuns;
   static constexpr int kBatch = kPasses < kMost ? kPasses : kMost;
   // Row of this lane in a pass: its token in the tile, and whether it is V.
   __device__ static uint32_t token(uint32_t pass, bool& is_v) {
@@ -183,8 +183,8 @@ struct Kv4RowMap {
 };
 
 template <class T, int D, int TILE>
-__global__ void __launch_bounds__(32 * kKv4StoreWarps) append_kv4_kernel(const Kv4RowsParams p) {
-  using M = Kv4RowMap<T, D, TILE>;
+__global__ void __launch_bounds__(32 * kKv4StoreWarps, 4) append_kv4_kernel(const Kv4RowsParams p) {
+  using M = Kv4RowMap<D, TILE, 4>;
   __shared__ Kv4Tile<D, TILE> tile;
   const uint32_t part = threadIdx.x % M::kLanes;
   const uint32_t first = blockIdx.x * TILE, h = blockIdx.y, P = p.page_tokens;
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(32 * kKv4StoreWarps) append_kv4_kernel(const K
 
 template <class T, int D, int TILE>
 __global__ void __launch_bounds__(32 * kKv4StoreWarps) load_kv4_kernel(const Kv4RowsParams p) {
-  using M = Kv4RowMap<T, D, TILE>;
+  using M = Kv4RowMap<D, TILE, sizeof(T) == 2 ? 8 : 4>;
   __shared__ Kv4Tile<D, TILE> tile;
   const uint32_t part = threadIdx.x % M::kLanes;
   const uint32_t first = blockIdx.x * TILE, h = blockIdx.y, P = p.page_tokens;
