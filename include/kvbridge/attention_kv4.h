@@ -146,10 +146,9 @@ void compact_kv4(const Kv4Pool&, const Kv4Eviction&, const uint32_t* block_table
                  uint32_t new_stride, float* new_weights, int64_t new_weight_stride, cudaStream_t);
 
 namespace detail {
-// Status word and first failed wait of the kernels of this header (they live
-// in their own module); read_device_status and read_wait_failure include them.
+// Status word of the kernels of this header (they live in their own module and
+// wait for nothing but the kernel before); read_device_status includes it.
 cudaError_t read_kv4_status(int* status) noexcept;
-cudaError_t read_kv4_wait_failure(long long* record6) noexcept;
 }  // namespace detail
 
 }  // namespace kvbridge

@@ -1112,12 +1112,7 @@ cudaError_t read_wait_failure(long long* record6) {
   cudaError_t code = cudaMemcpyFromSymbol(record6, kvb::g_kvb_first_failure, 6 * sizeof(long long));
   if (code != cudaSuccess) return code;
   const long long zeros[6] = {0, 0, 0, 0, 0, 0};
-  code = cudaMemcpyToSymbol(kvb::g_kvb_first_failure, zeros, sizeof(zeros));
-  if (code != cudaSuccess) return code;
-  long long kv4[6] = {};
-  code = detail::read_kv4_wait_failure(kv4);
-  if (record6[0] == 0) std::copy(kv4, kv4 + 6, record6);
-  return code;
+  return cudaMemcpyToSymbol(kvb::g_kvb_first_failure, zeros, sizeof(zeros));
 }
 
 void set_wait_limit_ns(unsigned long long ns) noexcept {

@@ -116,8 +116,8 @@ kvb::Kv4RowsParams rows_params(const Kv4Pool& pool, const Kv4Rows& rows) {
                             vector};
 }
 
-// Tokens a CTA: 16 where 64 would leave SMs without one; else 64, but 32 to
-// append rows of dim 128, whose loads are then one batch a lane (65,536 bf16
+// Tokens a CTA: 16 where 64 would leave SMs without one (64 tokens appended and
+// loaded 6.9 us for 10.3, 1,024 tokens 18 us for 32); else 64, but 32 to append rows of dim 128, whose loads are then one batch a lane (65,536 bf16
 // tokens on 8 heads 114 us for 129; fp32 111 for 113; dims 64 and 256 the other
 // way round, 70 us for 85 and 235 for 294; to load, 64 is better at any dim).
 bool small_tiles(const Kv4Pool& pool, const Kv4Rows& rows) {
@@ -232,7 +232,9 @@ struct Kv4Kernel {
 // tokens, four 94 us with 160 bytes of spills; 4 columns: 1x64K 26.6 us at
 // three, 28.0 us at four.)
 constexpr int attend_ctas(int dim) { return dim == 256 ? 2 : dim == 64 ? 4 : 3; }
-constexpr int weigh_ctas(int dim, int cols) { return dim == 256 ? 2 : dim == 64 || cols == 4 ? 4 : 3; }
+// (32 sequences of 1K to 32K tokens, 8 columns of dim 128: four 81 us, three 84
+// us, two 92 us.)
+constexpr int weigh_ctas(int dim) { return dim == 256 ? 2 : 4; }
 
 template <int D, int C, int PD, int RULES>
 Kv4Kernel attend_kernel() {
@@ -242,7 +244,7 @@ Kv4Kernel attend_kernel() {
 
 template <int D, int C, int RULES>
 Kv4Kernel weigh_kernel() {
-  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, weigh_ctas(D, C), RULES>),
+  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, weigh_ctas(D), RULES>),
           kvb::Kv4Smem<D, false>::kBytes};
 }
 
@@ -259,7 +261,9 @@ auto by_rules(int rules, F&& f) {
   return f(std::integral_constant<int, kvb::kRulesAll>{});
 }
 
-// Query columns a segment: 4 where all of a KV head's fit, else 8.
+// Query columns a segment: 4 where all of a KV head's fit (32 sequences of 1K to
+// 32K tokens, group 4: 106 us, with 8 half of whose rows are idle 126 us), else 8
+// (64 x 16K tokens, group 8: 248 us, with 4 and every page read twice 454 us).
 uint32_t segment_columns(const Kv4Pool& pool, const Kv4Query& q) {
   return q.rows * (q.q_heads / pool.kv_heads) <= 4 ? 4 : 8;
 }
@@ -324,6 +328,8 @@ struct AttendPlan {
 };
 
 // Short sequences: one warp per segment writes the result, nothing is merged.
+// (64 sequences of 128 tokens 9.6 us, split and merged 11.4 us, and one launch
+// less; eight of up to 256 tokens 12.3 us so and 9.0 us split.)
 constexpr uint32_t kDirectTokens = 128;
 
 AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
@@ -344,7 +350,8 @@ AttendPlan plan_attention(const Kv4Pool& pool, const Kv4Query& q) {
   }
   // At most 512 partials a segment: one KV head of 131,072 tokens takes 18.5 us
   // so, 26.9 us with a full wave's 1,776 partials to merge.
-  a.ctas = std::min(split_ctas(a.kernel, a.segments, q.max_tokens), uint32_t(std::min<uint64_t>(128ull * a.segments, 0xffffffffull)));
+  const uint64_t capped = uint64_t(512 / kvb::kKv4Warps) * a.segments;
+  a.ctas = uint32_t(std::min<uint64_t>(split_ctas(a.kernel, a.segments, q.max_tokens), capped));
   a.workers = a.ctas * kvb::kKv4Warps;
   // A warp reads 32 partials a round; from about 24 on a CTA a row is faster.
   a.many = a.workers > 24 * a.segments;
@@ -457,9 +464,9 @@ void select_tokens(const Kv4Eviction& e, int32_t* keep, uint32_t* kept_lens, cud
   kvb::SelectParams prm{e.seq_lens, e.weights,    e.weight_stride, keep,    kept_lens, e.batch,
                         e.kv_heads, e.max_tokens, e.budget,        e.sinks, e.recent};
   // CTAs a segment: one for every 2,048 tokens, at most the eight of a
-  // portable cluster (sixteen are slower: 8,192 of 65,536 tokens 73 us for 51),
-  // and no more than fill the SMs twice (16 x 16K tokens on
-  // 8 heads: 90 us in clusters of eight, whose shared histograms queue).
+  // portable cluster (sixteen: selecting and moving 8,192 of 65,536 tokens 73 us
+  // for 51), and no more than fill the SMs twice (16 x 16K tokens on 8 heads: 90
+  // us in clusters of eight, whose shared histograms queue).
   uint32_t ctas = 1;
   while (ctas < 8 && uint64_t(ctas) * 2048 < e.max_tokens &&
          uint64_t(e.batch) * e.kv_heads * ctas * 2 <= uint64_t(2 * detail::device_sms()))
@@ -512,13 +519,6 @@ cudaError_t read_kv4_status(int* status) noexcept {
   if (code != cudaSuccess) return code;
   const int zero = 0;
   return cudaMemcpyToSymbol(kvb::g_kvb_status, &zero, sizeof(int));
-}
-
-cudaError_t read_kv4_wait_failure(long long* record6) noexcept {
-  cudaError_t code = cudaMemcpyFromSymbol(record6, kvb::g_kvb_first_failure, 6 * sizeof(long long));
-  if (code != cudaSuccess) return code;
-  const long long zeros[6] = {0, 0, 0, 0, 0, 0};
-  return cudaMemcpyToSymbol(kvb::g_kvb_first_failure, zeros, sizeof(zeros));
 }
 
 }  // namespace detail

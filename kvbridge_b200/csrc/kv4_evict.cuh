@@ -47,7 +47,8 @@ struct SelectSmem {
 // weights share few exponents, and the counters of a byte were a queue.) Then
 // one ordered pass: a token is kept if its key is above the threshold, or
 // equal to it and among the first `want` of those. Bound by the chain of those
-// steps, not by bytes (4 a token).
+// steps, not by bytes (4 a token): 16 sequences of 1.5K to 16K tokens on 8
+// heads 23 us, one of 128K on 2 heads 27 us in clusters of eight.
 __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectParams p) {
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ __align__(16) SelectSmem sm;
@@ -200,9 +201,12 @@ constexpr int kCompactThreads = 256;
 constexpr uint32_t kCompactTile = 64;            // kept tokens a CTA
 constexpr uint32_t kCompactStage = 32768 + 1024; // bytes of source V pages held at once, and gaps
 
-// One CTA per (64 kept tokens, KV head, sequence). Bound by HBM (and, for V,
-// by whole source pages: a kept token's V bytes lie in every 32-byte sector
-// row of its page). K rows and params go straight across. V pages come in
+// One CTA per (64 kept tokens, KV head, sequence). A kept token's V bytes lie
+// in every sector row of its page, so that V costs whole source pages: 143 MB
+// read where 16 sequences of up to 16K tokens on 8 heads keep 2,048 (38 MB),
+// 56 us. Bound by
+// the latency of its steps in a row (token list, table, pages, picking, stores)
+// at five CTAs an SM, whose waits do not overlap enough to fill the HBM. K rows and params go straight across. V pages come in
 // whole (16-byte loads) into shared memory, the kept tokens' bytes are picked
 // into a tile of the new layout, and the tile is stored in 16-byte runs. Slots
 // after the kept ones are not written.

@@ -692,3 +692,77 @@ def test_decode_with_eviction(cuda_device):
             p = np.exp(s - s.max())
             want = p @ v / p.sum()
             assert np.allclose(out[0, 0, h * group + gq].double().cpu().numpy(), want, rtol=2 ** -7, atol=2e-3)
+
+
+def test_bounded_cache_refusals():
+    from kvbridge_b200 import kv4_decode
+
+    with pytest.raises(ValueError, match="budget"):
+        kv4_decode.BoundedCache(1, 1, 64, 16, 100, 100, 0, 0, "cpu")
+    with pytest.raises(ValueError, match="observe"):
+        kv4_decode.decode(prompt=3, observe=4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [
+    dict(batch=3, prompt=700, steps=40, budget=200, slack=16, page_tokens=16, dim=64, q_heads=4, kv_heads=2),
+    dict(batch=1, prompt=65, steps=70, budget=100, slack=1, page_tokens=32, dim=256, q_heads=6, kv_heads=1, observe=1),
+    dict(batch=2, prompt=500, steps=20, budget=300, slack=300, page_tokens=64, q_heads=16, dtype=torch.float32),
+])
+def test_bounded_decode(cuda_device, kw):
+    """The serving loop: how often it evicts, and its last output. Values are
+    sums of normal numbers' 4-bit images with weights that add up to 1, so below
+    6: bf16 rounds them to 6 * 2^-8, the 16-bit digits of P add 2^-15 of that."""
+    from kvbridge_b200 import kv4_decode
+
+    result = kv4_decode.decode(**kw, device=cuda_device)
+    held, evictions, cap = kw["prompt"], 0, kw["budget"] + kw["slack"]
+    for _ in range(kw["steps"]):
+        if held >= cap:
+            held, evictions = kw["budget"], evictions + 1
+        held += 1
+    assert (result["longest"], result["evictions"]) == (held, evictions)
+    assert result["error"] < (2e-5 if kw.get("dtype") is torch.float32 else 6 * 2 ** -8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_append_codes_at_ties(cuda_device, dtype, dim):
+    """Rows whose quotients lie at or next to half integers: codes are those of
+    the rounded division, bit for bit."""
+    g = torch.Generator().manual_seed(81)
+    n, heads, page = 96, 2, 16
+    half = torch.randint(0, 31, (n, heads, dim), generator=g).float() / 2  # 0, 0.5, .. 15
+    half[..., 0], half[..., 1] = 0.0, 15.0
+    x = half * torch.exp2(torch.randint(-20, 12, (n, heads, 1), generator=g).float())
+    x = x * torch.where(torch.rand((n, heads, 1), generator=g) < 0.5, 1.0, 1.0 + 1.0 / 3)
+    x = (x + torch.randn((n, heads, 1), generator=g) * (x.amax(-1, keepdim=True) / 8)).to(dtype)
+    pool = kvb.Kv4Pool.empty(n // page, heads, page, dim, device=cuda_device)
+    slots = torch.randperm(n, generator=g)
+    kvb.append_kv4(pool, kvb.Kv4Rows(x.to(cuda_device), x.flip(0).contiguous().to(cuda_device), slots.to(cuda_device)))
+    code, want = util.quantize(x.float())
+    k = pool.k.cpu().transpose(1, 2).reshape(n, heads, dim // 2)[slots]
+    assert torch.equal(k, util.pack(code))
+    params = pool.k_params.cpu().transpose(1, 2).reshape(n, heads, 2)[slots]
+    assert torch.equal(params, want)
+    v = pool.v.cpu().permute(0, 3, 1, 2).reshape(n, heads, dim // 2)[slots]
+    assert torch.equal(v.flip(0), util.pack(code))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads,group,dim", [(1, 8, 128), (1, 4, 256), (2, 1, 64)])
+def test_attention_many_partials_a_row(cuda_device, kv_heads, group, dim):
+    """Few long segments: as many partials a row as there can be."""
+    cache = util.make_cache([9001, 33000], kv_heads, dim, 64, seed=91)
+    rule = util.make_query(cache, util.Rule(rows=1, group=group, dtype=torch.float32), seed=92)
+    util.check_attention(cache, rule, cuda_device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rule", [dict(), dict(window=70), dict(window=40, prefix=[3] * 40, softcap=20.0)])
+def test_attention_more_sequences_than_lanes(cuda_device, rule):
+    lens = [(37 * b) % 301 for b in range(40)]
+    cache = util.make_cache(lens, 2, 64, 16, seed=95)
+    rule = util.make_query(cache, util.Rule(rows=2, group=3, **rule), seed=96)
+    util.check_attention(cache, rule, cuda_device)
