@@ -116,10 +116,12 @@ kvb::Kv4RowsParams rows_params(const Kv4Pool& pool, const Kv4Rows& rows) {
                             vector};
 }
 
-// Tokens a CTA: 16 where 64 would leave SMs without one (64 tokens appended and
-// loaded 6.9 us for 10.3, 1,024 tokens 18 us for 32); else 64, but 32 to append rows of dim 128, whose loads are then one batch a lane (65,536 bf16
-// tokens on 8 heads 114 us for 129; fp32 111 for 113; dims 64 and 256 the other
-// way round, 70 us for 85 and 235 for 294; to load, 64 is better at any dim).
+// Tokens a CTA: 16 where 64 would give an SM less than two CTAs (64 tokens
+// appended and loaded 6.9 us for 10.3, 1,024 tokens 18 us for 32); else 64, but
+// 32 to append rows of dim 128, whose loads are then one batch a lane (65,536
+// bf16 tokens on 8 heads 114 us for 129; fp32 111 for 113; dims 64 and 256 the
+// other way round, 70 us for 85 and 235 for 294; to load, 64 is better at any
+// dim, at 128 69 us for 85).
 bool small_tiles(const Kv4Pool& pool, const Kv4Rows& rows) {
   return uint64_t((rows.tokens + 63) / 64) * pool.kv_heads < uint64_t(2 * detail::device_sms());
 }

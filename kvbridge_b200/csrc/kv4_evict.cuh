@@ -48,7 +48,7 @@ struct SelectSmem {
 // one ordered pass: a token is kept if its key is above the threshold, or
 // equal to it and among the first `want` of those. Bound by the chain of those
 // steps, not by bytes (4 a token): 16 sequences of 1.5K to 16K tokens on 8
-// heads 23 us, one of 128K on 2 heads 27 us in clusters of eight.
+// heads 23 us, one of 128K on 2 heads about 28 us in clusters of eight.
 __global__ void __launch_bounds__(kSelectThreads) select_tokens_kernel(SelectParams p) {
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ __align__(16) SelectSmem sm;
