@@ -198,18 +198,21 @@ struct CompactParams {
 };
 
 constexpr int kCompactThreads = 256;
-constexpr uint32_t kCompactTile = 64;            // kept tokens a CTA
-constexpr uint32_t kCompactStage = 32768 + 1024; // bytes of source V pages held at once, and gaps
+constexpr uint32_t kCompactTile = 64;  // kept tokens a CTA
+// Bytes of source V pages held at once, and gaps: two of the largest pages. Eight
+// CTAs fit an SM (twice the bytes and five CTAs: 16 sequences of up to 16K tokens
+// selected and moved in 82 us, with this in 75; half of it is no faster).
+constexpr uint32_t kCompactStage = 16384 + 512;
 
 // One CTA per (64 kept tokens, KV head, sequence). A kept token's V bytes lie
 // in every sector row of its page, so that V costs whole source pages: 143 MB
-// read where 16 sequences of up to 16K tokens on 8 heads keep 2,048 (38 MB),
-// 56 us. Bound by
-// the latency of its steps in a row (token list, table, pages, picking, stores)
-// at five CTAs an SM, whose waits do not overlap enough to fill the HBM. K rows and params go straight across. V pages come in
-// whole (16-byte loads) into shared memory, the kept tokens' bytes are picked
-// into a tile of the new layout, and the tile is stored in 16-byte runs. Slots
-// after the kept ones are not written.
+// read where 16 sequences of up to 16K tokens on 8 heads keep 2,048 (38 MB), 49
+// us. Bound by the latency of its steps in a row (token list, table, pages,
+// picking, stores) at eight CTAs an SM, whose waits do not overlap enough to
+// fill the HBM. K rows and params go straight across. V pages come in whole
+// (16-byte copies) into shared memory, the kept tokens' bytes are picked into a
+// tile of the new layout, and the tile is stored in 16-byte runs. Slots after
+// the kept ones are not written.
 template <int D>
 __global__ void __launch_bounds__(kCompactThreads) compact_kv4_kernel(const CompactParams p) {
   __shared__ __align__(16) uint8_t stage[kCompactStage];
