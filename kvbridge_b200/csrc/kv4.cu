@@ -232,11 +232,10 @@ struct Kv4Kernel {
 // CTAs of 128 threads an SM, i.e. the register cap: 128 registers at four,
 // 168 at three, 255 at two. (Dim 128, 8 columns: three CTAs 83 us for 16x16K
 // tokens, four 94 us with 160 bytes of spills; 4 columns: 1x64K 26.6 us at
-// three, 28.0 us at four.)
+// three, 28.0 us at four. Weights of 32 sequences of 1K to 32K tokens, 8
+// columns: three 82 us, with cap and bias 115 us; four, which spill, 81 and 117
+// us; 1x64K, 4 columns, 13.1 against 13.4 us.)
 constexpr int attend_ctas(int dim) { return dim == 256 ? 2 : dim == 64 ? 4 : 3; }
-// (32 sequences of 1K to 32K tokens, 8 columns of dim 128: four 81 us, three 84
-// us, two 92 us.)
-constexpr int weigh_ctas(int dim) { return dim == 256 ? 2 : 4; }
 
 template <int D, int C, int PD, int RULES>
 Kv4Kernel attend_kernel() {
@@ -246,7 +245,7 @@ Kv4Kernel attend_kernel() {
 
 template <int D, int C, int RULES>
 Kv4Kernel weigh_kernel() {
-  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, weigh_ctas(D), RULES>),
+  return {reinterpret_cast<const void*>(&kvb::weigh_kv4_kernel<D, C, attend_ctas(D), RULES>),
           kvb::Kv4Smem<D, false>::kBytes};
 }
 

@@ -1226,7 +1226,7 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps, HELD == 8 ? 2 : 1) merge_
 // groups needs every group's digits in registers, or atomics, whose order
 // changes the sums.) Reads half of what attention does and a float a token,
 // writes the float. Bound by the instructions of the scores: 32 sequences of
-// 1K to 32K tokens, eight columns, take 81 us, 4.3 TB/s; 5,000 tokens 6.2 us,
+// 1K to 32K tokens, eight columns, take 82 us, 4.2 TB/s; 5,000 tokens 5.6 us,
 // a kernel's latency.
 
 template <int D, int C, int MINB, int RULES>
