@@ -576,6 +576,7 @@ __device__ void kv4_make_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
         qf.a[1][i][2 * odd + 1] = 0u;
       }
     }
+  int digits[kv4_q_tiles(C)][2];  // digit sums of rows grp and grp + 8
 #pragma unroll
   for (int m = 0; m < kv4_q_tiles(C); ++m)
 #pragma unroll
@@ -588,17 +589,18 @@ __device__ void kv4_make_query(const Kv4AttendParams& p, uint32_t b, uint32_t h,
       }
       s += __shfl_xor_sync(0xffffffffu, s, 1);
       s += __shfl_xor_sync(0xffffffffu, s, 2);
+      digits[m][r] = s;
       qf.start[m][r] = -8 * s;
     }
-  // sum of n, from the digit sums; exact: |n| <= 2^22, 256 of them.
-  int total = qf.start[0][0] + 256 * qf.start[0][1];
+  // sum of n, exact: 256 values of at most 2^22, so at most 2^30 (and -8 times
+  // that would not fit).
+  int total = digits[0][0] + 256 * digits[0][1];
   if constexpr (C == 8) {
-    total += 65536 * qf.start[1][0];
+    total += 65536 * digits[1][0];
   } else {
     const int other = __shfl_xor_sync(0xffffffffu, total, 16);  // the upper lane has digit 2
     total = grp >= 4 ? 65536 * total + other : total + 65536 * other;
   }
-  total /= -8;
   // Scores in log2 units, or in natural ones where a cap or a bias comes after.
   const float unit = RULES == kRulesAll ? p.rule.scale : p.rule.scale * kLog2e;
   const float dot = amax <= 3.402823466e38f ? down * unit : __int_as_float(0x7fffffff);

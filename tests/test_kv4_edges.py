@@ -1,0 +1,98 @@
+"""The 4-bit cache where its arithmetic and its checks can go wrong: queries
+whose values share a sign, at bounds of the digits that the kernels hold."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kvbridge_b200 as kvb
+
+import kv4_testutil as util
+from kv4_testutil import EPS, ROUND, SMALLEST, Rule, make_cache
+
+
+def bounds(cache, rule, want):
+    """What the kernels' formats allow around util.expected (causal by index):
+
+    * scores: queries are fixed point with a unit of at most 2^-21 of the row's
+      largest value, for every type: half of it, scale * max|q| * sum|k| * 2^-22;
+      the fp32 fold of scale_t * (q . code) and lo * sum q a few 2^-24 of scale *
+      sum|q| * max|k|, the score's own roundings 8 * 2^-24 of it.
+    * sums of n probabilities in fp32, a quarter of the tokens a lane: n / 4 + 16
+      roundings; exp 2^-21.
+    * probability times V scale: half a unit, 2^-16 (fp32 outputs 2^-23) of the
+      largest of its 64 tokens, times a code's distance from 8.
+    * the result's own rounding.
+
+    Returns the bounds of out, lse and weights."""
+    scale, group = cache.dim ** -0.5, rule.group
+    out, lse = np.zeros_like(want.out), np.zeros_like(want.lse)
+    weights = [np.zeros_like(w) for w in want.weights]
+    grain = 2.0 ** (-23 if rule.dtype == torch.float32 else -16)
+    for b, n in enumerate(cache.lens):
+        sums = (n / 4 + 16) * EPS + 2.0 ** -21
+        for h in range(cache.heads):
+            k, v = cache.dense("k", b, h), cache.dense("v", b, h)
+            t = np.arange(n)
+            par = cache.v_params.numpy()[cache.table[b].numpy()[t // cache.page], h, t % cache.page].astype(np.float64)
+            for r in range(rule.rows):
+                see = t <= n - rule.rows + r
+                if not see.any():
+                    continue
+                for head in range(h * group, (h + 1) * group):
+                    q = rule.q[b, r, head].double().numpy()
+                    x = scale * (k[see] @ q)
+                    score = scale * np.abs(q).max() * np.abs(k[see]).sum(-1).max() * 2.0 ** -22
+                    score += 16 * EPS * scale * np.abs(q).sum() * np.abs(k[see]).max() + 8 * EPS * np.abs(x).max()
+                    p = np.exp(x - want.lse[b, r, head])
+                    lse[b, r, head] = score + sums + 4 * EPS * abs(want.lse[b, r, head])
+                    weights[b][h, see] += p * (2 * score + sums + 2 * lse[b, r, head])
+                    held = np.zeros(n)
+                    held[see] = p * par[see, 0]
+                    tiles = sum(8 * grain * held[i:i + 64].max() * see[i:i + 64].sum() for i in range(0, n, 64))
+                    parts = (p[:, None] * (np.abs(v[see]) + 16 * par[see, :1])).sum(0)
+                    own = want.out[b, r, head]
+                    out[b, r, head] = ((2 * score + 2 * sums) * parts + tiles
+                                       + ROUND[rule.dtype] * np.abs(own) + SMALLEST[rule.dtype])
+    return out, lse, weights
+
+
+def signed_queries(shape, dtype, seed):
+    """One kind of query values a sequence, most with a mean far from zero."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(shape, generator=g)
+    q[0], q[1], q[2], q[3], q[4] = 1.0, -1.0, 1.5, 1.99, -1.99
+    q[5] = torch.rand(shape[1:], generator=g)
+    q[6] += 1
+    q[7] += 3
+    q[8] = -0.25 - 0.5 * torch.rand(shape[1:], generator=g)
+    return q.to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 32)])
+@pytest.mark.parametrize("rows,group", [(1, 1), (1, 4), (1, 8), (3, 4)])
+def test_queries_with_a_mean(cuda_device, dtype, dim, page, rows, group):
+    """Output, log-sum-exp and weights: a query's sum multiplies every token's offset."""
+    lens = [130, 64, 70, 200, 65, 129, 128, 90, 193, 150]
+    cache = make_cache(lens, 2, dim, page, seed=5)
+    rule = Rule(rows=rows, group=group, dtype=dtype)
+    rule.q = signed_queries((len(lens), rows, 2 * group, dim), dtype, 6)
+    want = util.expected(cache, rule)
+    out_tol, lse_tol, weight_tol = bounds(cache, rule, want)
+    pool, query = cache.to(cuda_device), util.device_query(cache, rule, cuda_device)
+    out, lse = util.attend(cache, rule, cuda_device, pool=pool, query=query)
+    for b in range(len(lens)):
+        assert np.all(np.abs(lse[b] - want.lse[b]) <= lse_tol[b]), (b, np.abs(lse[b] - want.lse[b]).max(), lse_tol[b].max())
+        assert np.all(np.abs(out[b] - want.out[b]) <= out_tol[b]), (b, np.abs(out[b] - want.out[b]).max(), out_tol[b].max())
+    weights = torch.zeros((len(lens), 2, max(lens)), device=cuda_device)
+    kvb.accumulate_weights_kv4(pool, query, torch.from_numpy(want.lse).float().to(cuda_device), weights)
+    got = weights.cpu().double().numpy()
+    for b, n in enumerate(lens):
+        off = np.abs(got[b, :, :n] - want.weights[b])
+        # (sums over the columns add a rounding each)
+        assert np.all(off <= weight_tol[b] + rows * group * EPS * want.weights[b]), (b, off.max())
