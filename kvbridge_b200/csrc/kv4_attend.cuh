@@ -353,16 +353,20 @@ struct Kv4Feeder {
     addr = smem_addr(slots);
   }
 
+  // The block-table entry of the lane's 16-token group of stage `at`.
+  __device__ __forceinline__ uint32_t entry_of(const Kv4AttendParams& p, uint32_t at) const {
+    const uint32_t j = uint32_t(int32_t(at) - cur.base);
+    const uint32_t stage = RULES && j >= cur.head ? j + cur.skip : j;
+    return (stage * kStageTokens + 16 * (threadIdx.x & 3)) >> p.log2_page;
+  }
+
   // Starts the lookup of the pages of stage `next`; kNoUnit where there is none.
   __device__ __forceinline__ void lookup(const Kv4AttendParams& p) {
     phys = kNoUnit;
     if (next < count) {
       while (int32_t(next) >= cur.base + int32_t(cur.stages)) kv4_next_segment<RULES>(p, segs, cur);
-      const uint32_t j = uint32_t(int32_t(next) - cur.base);
-      const uint32_t stage = RULES && j >= cur.head ? j + cur.skip : j;
-      const uint32_t t = stage * kStageTokens + 16 * (threadIdx.x & 3);
       head = p.col_groups == 1 ? cur.seg : cur.seg / p.col_groups;
-      const uint32_t page = t >> p.log2_page;  // all of it: V's quarters are not tokens
+      const uint32_t page = entry_of(p, next);  // all of it: V's quarters are not tokens
       if ((page << p.log2_page) < cur.len) phys = kv4_load(p.table + size_t(cur.b) * p.table_stride + page);
       ++next;
     }
@@ -413,7 +417,8 @@ struct Kv4Feeder {
   template <bool OF_V>
   __device__ __forceinline__ void copy(const Kv4AttendParams& p) {
     const bool ok = phys < p.pool.pages;
-    if (!OF_V && !ok && phys != kNoUnit) atomicMax(&g_kvb_status, kKv4BadPage);
+    // A bad id, which may have kNoUnit's value; not a group past the sequence's end.
+    if (!OF_V && !ok && (entry_of(p, next - 1) << p.log2_page) < cur.len) atomicMax(&g_kvb_status, kKv4BadPage);
     if (p.log2_page == 6) {
       if (ok) copy_page<OF_V>(p);
     } else {

@@ -96,3 +96,31 @@ def test_queries_with_a_mean(cuda_device, dtype, dim, page, rows, group):
         off = np.abs(got[b, :, :n] - want.weights[b])
         # (sums over the columns add a rounding each)
         assert np.all(off <= weight_tol[b] + rows * group * EPS * want.weights[b]), (b, off.max())
+
+
+NO_PAGE = -1  # what an unassigned entry of an int32 block table usually holds
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("rule", [Rule(), Rule(group=8), Rule(window=150), Rule(slopes=True)], ids=str)
+@pytest.mark.parametrize("bad", [NO_PAGE, 1 << 20, -7])
+def test_every_bad_page_id_is_reported(cuda_device, page, rule, bad):
+    """Any id that is not in the pool, -1 among them, inside a sequence; none beyond its end."""
+    cache = make_cache([90, 250, 40], 1, 128, page, seed=41)
+    rule = util.make_query(cache, rule, 42)
+    for b, n in enumerate(cache.lens):
+        cache.table[b, -(-n // page):] = bad
+    # A window of 150 starts at token 100: the 64 tokens before its first stage are not looked at.
+    for at, status in ((None, 0), (64, 4), (249, 4), (150, 4), (0, 0 if rule.window else 4)):
+        table = cache.table.clone()
+        if at is not None:
+            cache.table[1, at // page] = bad
+        pool, query = cache.to(cuda_device), util.device_query(cache, rule, cuda_device)
+        cache.table = table
+        kvb.read_device_status()
+        util.attend(cache, rule, cuda_device, pool=pool, query=query)
+        assert kvb.read_device_status() == status, at
+        lse = torch.zeros(query.lse_shape, device=cuda_device)
+        kvb.accumulate_weights_kv4(pool, query, lse, torch.zeros((3, 1, 250), device=cuda_device))
+        assert kvb.read_device_status() == status, at
