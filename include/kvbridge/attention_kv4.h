@@ -33,7 +33,8 @@
 // CUDA failures. Every buffer is a device pointer that the caller owns; the
 // library allocates nothing. Slots, page ids and lengths are read on the
 // device: an invalid one is skipped (a length clamped) and reported through
-// read_device_status (4 page id, 5 length, 6 slot, 8 kept token).
+// read_device_status (4 page id, 5 length, 6 slot, 8 kept token). No query row
+// sees the tokens of a page id that is not in the pool, and their weights stay.
 #include <cuda_runtime.h>
 #include <cstddef>
 #include <cstdint>

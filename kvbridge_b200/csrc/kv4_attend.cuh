@@ -321,6 +321,9 @@ __device__ __forceinline__ uint32_t kv4_start(const Kv4AttendParams& p, uint32_t
 // these gaps a quarter-warp's reads of four token groups or several pages hit
 // different banks. V false: K alone.
 constexpr uint32_t kKv4ParamPitch = 144;
+// {scale, lo} in the slots of 16 tokens whose page is not in the pool: no row
+// has a negative scale. Attention's K is NaN instead, which no maximum takes.
+constexpr float kKv4Absent = -1.0f;
 template <int D, bool V>
 struct Kv4Smem {
   static constexpr uint32_t kCodes = kStageTokens * D / 2;
@@ -414,11 +417,24 @@ struct Kv4Feeder {
                                                     (2 * lane & in_page)));
   }
 
+  // The lane's group of the stage is absent: two of its tokens a lane.
+  template <bool OF_V>
+  __device__ __forceinline__ void mark_absent() {
+    using S = Kv4Smem<D, V>;
+    const uint32_t lane = threadIdx.x & 31;
+    const float scale = V && !OF_V ? __int_as_float(0x7fffffff) : kKv4Absent;
+    *reinterpret_cast<float4*>(slots + (OF_V ? S::kOffVp : S::kOffKp) + (lane & 3) * kKv4ParamPitch + (lane >> 2) * 16) =
+        make_float4(scale, 0.f, scale, 0.f);
+  }
+
   template <bool OF_V>
   __device__ __forceinline__ void copy(const Kv4AttendParams& p) {
     const bool ok = phys < p.pool.pages;
     // A bad id, which may have kNoUnit's value; not a group past the sequence's end.
-    if (!OF_V && !ok && (entry_of(p, next - 1) << p.log2_page) < cur.len) atomicMax(&g_kvb_status, kKv4BadPage);
+    if (!ok && (entry_of(p, next - 1) << p.log2_page) < cur.len) {
+      if (!OF_V) atomicMax(&g_kvb_status, kKv4BadPage);
+      mark_absent<OF_V>();
+    }
     if (p.log2_page == 6) {
       if (ok) copy_page<OF_V>(p);
     } else {
@@ -826,7 +842,15 @@ __device__ __forceinline__ void kv4_softmax(const uint8_t* vparams, uint32_t see
   const float sub = m == -INFINITY ? 0.f : m;
   const float alpha = m == st.m ? 1.f : kv4_exp<RULES>(st.m, sub);
   st.m = m;
-  if (__any_sync(0xffffffffu, alpha != 1.f)) {
+  const float4* par = reinterpret_cast<const float4*>(vparams + kv4_params_at<C>());
+  // Of a page that is not in the pool: the scores are NaN (or -inf), and the
+  // maximum has passed over them.
+  const bool absent = par[0].x == kKv4Absent;
+  if (__any_sync(0xffffffffu, alpha != 1.f || absent)) {
+    if (absent) {
+#pragma unroll
+      for (int u = 0; u < kTokens; ++u) sc[u] = -INFINITY;
+    }
     st.l *= alpha;
     st.lo *= alpha;
 #pragma unroll
@@ -834,7 +858,6 @@ __device__ __forceinline__ void kv4_softmax(const uint8_t* vparams, uint32_t see
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.o[j][e] *= alpha;
   }
-  const float4* par = reinterpret_cast<const float4*>(vparams + kv4_params_at<C>());
 #pragma unroll
   for (int u = 0; u < kTokens; u += 2) {
     const float4 f = par[kv4_token(C, u) / 2];
@@ -854,7 +877,8 @@ __device__ __forceinline__ void kv4_softmax(const uint8_t* vparams, uint32_t see
   big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
   // Power of two (a little less, so that nothing rounds up to the next one)
   // that puts the tile's largest below 2^16 or 2^23: the fixed-point values
-  // are the low bytes of sc * up + 2^23.
+  // are the low bytes of sc * up + 2^23. (All tokens absent: big is -0 and the
+  // digits are 0, whatever the scales.)
   constexpr uint32_t kTop = PD == 2 ? 269 : 276;
   constexpr float kLess = 1.0f - 1.0f / 16384.0f;
   const uint32_t ex = max(__float_as_uint(big) >> 23, kTop - 253u);
@@ -1287,12 +1311,13 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
       kv4_dots<D, C>(feed.slots, qf, w);
       uint32_t seen = kv4_scores<C, RULES>(p, feed.slots + S::kOffKp, tb, cur.len, prefix,
                                   kv4_all_visible<RULES>(p, tb, cur.len, prefix), qf.sum, qf.slope, qf.pos, pos, w);
+      const bool absent = reinterpret_cast<const float*>(feed.slots + S::kOffKp + kv4_params_at<C>())[0] == kKv4Absent;
       __syncwarp();  // every lane has read K
       if (done + 1 < count) {
         feed.template copy<false>(p);
         feed.lookup(p);
       }
-      if (lse == INFINITY) seen = 0;
+      if (lse == INFINITY || absent) seen = 0;
 #pragma unroll
       for (int u = 0; u < kTokens; ++u) w[u] = seen >> u & 1u ? kv4_exp<RULES>(w[u], lse) : 0.f;
       // Sum over the columns (lanes grp % C), halving the tokens held at each

@@ -2,7 +2,7 @@
 whose values share a sign, at bounds of the digits that the kernels hold."""
 from __future__ import annotations
 
-import math
+from dataclasses import replace
 
 import numpy as np
 import pytest
@@ -124,3 +124,85 @@ def test_every_bad_page_id_is_reported(cuda_device, page, rule, bad):
         lse = torch.zeros(query.lse_shape, device=cuda_device)
         kvb.accumulate_weights_kv4(pool, query, lse, torch.zeros((3, 1, 250), device=cuda_device))
         assert kvb.read_device_status() == status, at
+
+
+def without(cache, rule, dropped):
+    """The cache and rule that stand for this call with the `dropped` (sequence,
+    first token, end) hidden: positions that say what the indices did, beyond
+    every row for the hidden tokens."""
+    hidden = replace(cache)
+    hidden.positions = torch.zeros(cache.k_params.shape[:-1], dtype=torch.int32)
+    for b, n in enumerate(cache.lens):
+        for h in range(cache.heads):
+            at = torch.from_numpy(cache.token_positions(b, h)).int()
+            for b2, first, end in dropped:
+                if b2 == b:
+                    at[first:end] = 1 << 30
+            t = torch.arange(n)
+            hidden.positions[cache.table[b].long()[t // cache.page], h, t % cache.page] = at
+    rule = replace(rule)
+    if rule.q_positions is None:
+        rule.q_positions = torch.tensor([[n - rule.rows + r for r in range(rule.rows)] for n in cache.lens], dtype=torch.int32)
+    return hidden, rule
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,page", [(128, 16), (64, 32), (256, 64), (128, 64)])
+@pytest.mark.parametrize("rule,positions", [
+    (Rule(), False), (Rule(group=8, dtype=torch.float32), False), (Rule(rows=3, group=3, window=150), False),
+    (Rule(window=90, prefix=[20, 70, 0, 300, 100]), False), (Rule(group=5, prefix=[0, 250, 400, 9, 1000]), False),
+    (Rule(softcap=20.0, slopes=True, rows=2), False), (Rule(rows=2), True), (Rule(group=8, slopes=True, window=300), True),
+], ids=str)
+@pytest.mark.parametrize("bound", [None, 4000])
+def test_tokens_of_a_bad_page_are_not_seen(cuda_device, dim, page, rule, positions, bound):
+    """First, inner, last and all pages of a sequence: attention, log-sum-exp
+    and weights are those without the page's tokens, whatever a warp read before."""
+    lens = [100, 333, 600, 64, 1500]
+    cache = make_cache(lens, 2, dim, page, seed=51, positions=positions)
+    rule = util.make_query(cache, rule, 52)
+    drop = [(0, 0), (1, 64 // page), (1, 333 // page), (2, 128 // page), (2, 128 // page + 1), (4, 3), (4, 1000 // page)]
+    drop += [(3, j) for j in range(64 // page)]  # the whole sequence
+    hidden, plain = without(cache, rule, [(b, j * page, (j + 1) * page) for b, j in drop])
+    want = util.expected(hidden, plain)
+    table = cache.table.clone()
+    for i, (b, j) in enumerate(drop):
+        table[b, j] = (NO_PAGE, 1 << 20, cache.k.shape[0])[i % 3]
+    good, cache.table = cache.table, table
+    pool, query = cache.to(cuda_device), util.device_query(cache, rule, cuda_device, max_tokens=bound)
+    cache.table = good
+    kvb.read_device_status()
+    out, lse = util.attend(cache, rule, cuda_device, pool=pool, query=query)
+    assert kvb.read_device_status() == 4
+    empty = np.isneginf(want.lse)
+    assert np.all(empty[3]) and np.array_equal(empty, np.isneginf(lse)) and np.all(out[empty] == 0)
+    assert np.all(np.abs(lse[~empty] - want.lse[~empty]) <= want.lse_tol[~empty])
+    assert np.all(np.abs(out - want.out) <= want.out_tol)
+    start = torch.rand((len(lens), 2, 4000))
+    weights = start.to(cuda_device)
+    kvb.accumulate_weights_kv4(pool, query, torch.from_numpy(want.lse).float().to(cuda_device), weights)
+    assert kvb.read_device_status() == 4
+    got, start = weights.cpu().double().numpy(), start.double().numpy()
+    for b, n in enumerate(lens):
+        full = start[b, :, :n] + want.weights[b]
+        assert np.all(np.abs(got[b, :, :n] - full) <= want.weight_tol[b] + 4 * EPS * full)
+    for b, j in drop:
+        assert np.array_equal(got[b, :, j * page:(j + 1) * page], start[b, :, j * page:(j + 1) * page])
+
+
+@pytest.mark.gpu
+def test_short_sequences_with_bad_pages(cuda_device):
+    """Calls of one warp a segment: each of 40 sequences lacks another page."""
+    lens = [1 + (i * 29) % 128 for i in range(40)]
+    cache = make_cache(lens, 2, 128, 16, seed=53)
+    rule = util.make_query(cache, Rule(rows=2, group=2), 54)
+    drop = [(b, (b * 5) % -(-n // 16)) for b, n in enumerate(lens)]
+    hidden, plain = without(cache, rule, [(b, 16 * j, 16 * j + 16) for b, j in drop])
+    want = util.expected(hidden, plain)
+    for b, j in drop:
+        cache.table[b, j] = NO_PAGE
+    out, lse = util.attend(cache, rule, cuda_device)
+    assert kvb.read_device_status() == 4
+    empty = np.isneginf(want.lse)
+    assert np.array_equal(empty, np.isneginf(lse)) and np.all(out[empty] == 0)
+    assert np.all(np.abs(lse[~empty] - want.lse[~empty]) <= want.lse_tol[~empty])
+    assert np.all(np.abs(out - want.out) <= want.out_tol)
