@@ -98,7 +98,7 @@ struct Kv4Query {
   const uint32_t* block_table;  // uint32[batch * table_stride]
   const int32_t* q_positions;   // int32[batch * rows], optional; required iff the pool has positions
   const float* slopes;          // float[q_heads], optional
-  const uint32_t* prefix_lens;  // uint32[batch], optional
+  const uint32_t* prefix_lens;  // uint32[batch], optional; 2^31 and more: 0, and reported as a length
 };
 const char* kv4_query_error(const Kv4Pool&, const Kv4Query&) noexcept;
 

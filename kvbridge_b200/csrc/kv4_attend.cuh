@@ -122,9 +122,9 @@ __device__ __forceinline__ void kv4_load_sequence(const Kv4AttendParams& p, Kv4C
     // The first row's window starts at len - rows - window + 1.
     const uint64_t reach = uint64_t(p.rows) + p.rule.window - 1;
     const uint32_t from = reach < c.len ? uint32_t(c.len - reach) / kStageTokens : 0u;
-    uint32_t fix = 0;
-    if (p.rule.prefix != nullptr) fix = min(HINT ? __ldcg(p.rule.prefix + c.b) : kv4_load(p.rule.prefix + c.b), c.len);
-    c.head = (fix + kStageTokens - 1) / kStageTokens;
+    int32_t fix = 0;
+    if (p.rule.prefix != nullptr) fix = int32_t(HINT ? __ldcg(p.rule.prefix + c.b) : kv4_load(p.rule.prefix + c.b));
+    c.head = (uint32_t(max(0, min(fix, int32_t(c.len)))) + kStageTokens - 1) / kStageTokens;
     if (c.head < from) {
       c.skip = from - c.head;
       c.stages -= c.skip;
@@ -743,11 +743,11 @@ __device__ __forceinline__ float kv4_exp(float x, float y) {
 // within the last row's window. A warp-uniform test that spares most stages
 // the masks. first, last: the rows' positions.
 template <int RULES>
-__device__ __forceinline__ bool kv4_all_visible(const Kv4AttendParams& p, uint32_t tb, uint32_t len, uint32_t prefix) {
+__device__ __forceinline__ bool kv4_all_visible(const Kv4AttendParams& p, uint32_t tb, uint32_t len, int32_t prefix) {
   const int32_t first = int32_t(len) - int32_t(p.rows), end = int32_t(tb + kStageTokens);
   if (RULES == kRulesNone) return end <= first + 1;
   if (RULES == kRulesAll && p.rule.q_pos != nullptr) return false;
-  if (uint32_t(end) <= min(prefix, len)) return true;
+  if (end <= min(prefix, int32_t(len))) return true;
   return end <= first + 1 && (p.rule.window == 0 || uint32_t(int32_t(len) - 1 - int32_t(tb)) < p.rule.window);
 }
 
@@ -757,7 +757,7 @@ __device__ __forceinline__ bool kv4_all_visible(const Kv4AttendParams& p, uint32
 // their indices.
 template <int C, int RULES>
 __device__ __forceinline__ uint32_t kv4_scores(const Kv4AttendParams& p, const uint8_t* params, uint32_t tb,
-                                               uint32_t len, uint32_t prefix, bool all, float sum, float slope,
+                                               uint32_t len, int32_t prefix, bool all, float sum, float slope,
                                                int32_t pq, const int32_t* pos, float (&sc)[kv4_tokens(C)]) {
   constexpr int kTokens = kv4_tokens(C);
   const uint32_t at = kv4_first_token<C>();
@@ -1060,7 +1060,7 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
     const uint32_t h = cur.seg / p.col_groups;
     Kv4Query<D, C> qf;
     kv4_make_query<D, C, RULES>(p, cur.b, h, cur.seg % p.col_groups, cur.len, raw, qf);
-    const uint32_t prefix = RULES && p.rule.prefix != nullptr ? kv4_load(p.rule.prefix + cur.b) : 0u;
+    const int32_t prefix = RULES && p.rule.prefix != nullptr ? int32_t(kv4_load(p.rule.prefix + cur.b)) : 0;
     Kv4State<D> st;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
@@ -1095,6 +1095,7 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) attend_kv4_kernel(const Kv4
       }
     }
 
+    if (RULES && prefix < 0 && lane == 0) atomicMax(&g_kvb_status, kKv4LenClamped);
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
     st.lo += __shfl_xor_sync(0xffffffffu, st.lo, 1);
@@ -1295,7 +1296,7 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
                             col % p.group);
       if (x != -INFINITY) lse = RULES == kRulesAll ? x : x * kLog2e;
     }
-    const uint32_t prefix = RULES && p.rule.prefix != nullptr ? kv4_load(p.rule.prefix + cur.b) : 0u;
+    const int32_t prefix = RULES && p.rule.prefix != nullptr ? int32_t(kv4_load(p.rule.prefix + cur.b)) : 0;
     float* weights = p.weights + (int64_t(cur.b) * p.pool.kv_heads + cur.seg) * p.weight_stride;
     for (; done < end; ++done) {
       const uint32_t j = uint32_t(int32_t(done) - cur.base);
@@ -1337,6 +1338,7 @@ __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4A
       if (t0 < cur.len) weights[t0] = old0 + w[0];
       if (t0 + 1 < cur.len) weights[t0 + 1] = old1 + w[1];
     }
+    if (RULES && prefix < 0 && lane == 0) atomicMax(&g_kvb_status, kKv4LenClamped);
     if (done < count) kv4_next_segment<RULES>(p, segs, cur);
   }
 }

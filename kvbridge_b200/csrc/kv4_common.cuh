@@ -54,11 +54,12 @@ __device__ __forceinline__ int32_t kv4_query_position(const Kv4Rule& rule, uint3
 }
 
 // Positions of tokens are not negative; a query row's may be (more rows than
-// tokens), and pq - pk is only formed where pk <= pq.
+// tokens), and pq - pk is only formed where pk <= pq. A prefix of 2^31 or more
+// is a negative int32, below which nothing lies.
 __device__ __forceinline__ bool kv4_visible(int32_t pk, int32_t pq, uint32_t window,
-                                            uint32_t prefix) {
+                                            int32_t prefix) {
   const bool past = pk <= pq && (window == 0 || uint32_t(pq - pk) < window);
-  return past || uint32_t(pk) < prefix;
+  return past || pk < prefix;
 }
 
 __device__ __forceinline__ uint32_t kv4_len(const uint32_t* seq_lens, uint32_t b,

@@ -172,7 +172,7 @@ class Kv4Query:
     softcap * tanh(x / softcap) if ``softcap``, then minus slopes[head] * |pq -
     pk| if ``slopes`` (float32 [q_heads]). A token is visible if pk <= pq and,
     with a ``window``, pq - pk < window, or if pk < prefix_lens[b] (int32
-    [batch]). pq is ``q_positions`` int32 [batch, rows], or seq_len - rows + r."""
+    [batch]; a negative one counts as 0 and is reported as a length). pq is ``q_positions`` int32 [batch, rows], or seq_len - rows + r."""
 
     def __init__(self, q, seq_lens, block_table, max_tokens: int, kv_heads: int, scale: float, softcap: float = 0.0,
                  slopes=None, window: int = 0, prefix_lens=None, q_positions=None):

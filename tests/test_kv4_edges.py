@@ -206,3 +206,33 @@ def test_short_sequences_with_bad_pages(cuda_device):
     assert np.array_equal(empty, np.isneginf(lse)) and np.all(out[empty] == 0)
     assert np.all(np.abs(lse[~empty] - want.lse[~empty]) <= want.lse_tol[~empty])
     assert np.all(np.abs(out - want.out) <= want.out_tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rule", [Rule(rows=4), Rule(window=60, group=8), Rule(window=60, rows=3, softcap=30.0)], ids=str)
+@pytest.mark.parametrize("positions", [False, True])
+@pytest.mark.parametrize("batch", [3, 34])
+def test_negative_prefixes_are_none(cuda_device, rule, positions, batch):
+    """A negative int32 prefix shows nothing more and is reported; the others hold."""
+    lens = [(180 + 77 * b) % 400 for b in range(batch)]
+    cache = make_cache(lens, 1, 64, 16, seed=61, positions=positions)
+    rule = util.make_query(cache, replace(rule, prefix=[(-1, 70, -(1 << 31))[b % 3] for b in range(batch)]), 62)
+    valid = replace(rule, prefix=[max(x, 0) for x in rule.prefix])
+    want = util.expected(cache, valid)
+    pool, query = cache.to(cuda_device), util.device_query(cache, rule, cuda_device)
+    kvb.read_device_status()
+    out, lse = util.attend(cache, rule, cuda_device, pool=pool, query=query)
+    assert kvb.read_device_status() == 5
+    empty = np.isneginf(want.lse)
+    assert np.array_equal(empty, np.isneginf(lse))
+    assert np.all(np.abs(lse[~empty] - want.lse[~empty]) <= want.lse_tol[~empty])
+    assert np.all(np.abs(out - want.out) <= want.out_tol)
+    weights = torch.zeros((batch, 1, max(lens)), device=cuda_device)
+    kvb.accumulate_weights_kv4(pool, query, torch.from_numpy(want.lse).float().to(cuda_device), weights)
+    assert kvb.read_device_status() == 5
+    got = weights.cpu().double().numpy()
+    for b, n in enumerate(lens):
+        assert np.all(np.abs(got[b, :, :n] - want.weights[b]) <= want.weight_tol[b] + 4 * EPS * want.weights[b])
+    check = util.device_query(cache, valid, cuda_device)
+    util.attend(cache, valid, cuda_device, pool=pool, query=check)
+    assert kvb.read_device_status() == 0
