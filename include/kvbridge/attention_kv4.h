@@ -133,13 +133,13 @@ struct Kv4Eviction {
 const char* kv4_eviction_error(const Kv4Eviction&) noexcept;
 // keep: int32[batch * kv_heads * budget], the kept tokens of each (b, h) in
 // ascending order, then zeros; kept_lens: uint32[batch] = min(seq_lens[b],
-// budget). Works for any cache that keeps weights.
+// budget), not in the place of seq_lens. Works for any cache that keeps weights.
 void select_tokens(const Kv4Eviction&, int32_t* keep, uint32_t* kept_lens, cudaStream_t);
 // Copies the kept tokens (codes, parameters, positions) of every sequence
 // and KV head in order to the pages new_table[b * new_stride + j] of the
 // same pool, which no block table of the call may use, and their weights to
 // new_weights (optional; `budget` values a row, zeros after the kept ones,
-// rows new_weight_stride apart). A kept token beyond its sequence or beyond
+// rows new_weight_stride apart, none in the place of the old ones). A kept token beyond its sequence or beyond
 // the block table's row is skipped and reported. The old pages are only read, so sequences
 // may share them; the caller frees them afterwards.
 void compact_kv4(const Kv4Pool&, const Kv4Eviction&, const uint32_t* block_table,

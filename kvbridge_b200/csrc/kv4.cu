@@ -455,6 +455,21 @@ void check_eviction(const Kv4Eviction& e) {
     throw std::invalid_argument("eviction seq_lens and weights must be 4-byte aligned");
 }
 
+// Whether some of `rows` rows of `a` (a_width floats each, a_stride apart) share
+// a float with some of `b`'s.
+bool rows_overlap(const float* a, int64_t a_stride, int64_t a_width, const float* b, int64_t b_stride, int64_t b_width,
+                  int64_t rows) {
+  const int64_t from = (int64_t(reinterpret_cast<uintptr_t>(b)) - int64_t(reinterpret_cast<uintptr_t>(a))) / int64_t(sizeof(float));
+  if (a_width == 0 || b_width == 0 || from >= (rows - 1) * a_stride + a_width || -from >= (rows - 1) * b_stride + b_width)
+    return false;
+  for (int64_t j = 0; j < rows; ++j) {
+    const int64_t start = from + j * b_stride;  // from a's first float
+    const int64_t i = start < a_width ? 0 : (start - a_width) / a_stride + 1;  // the first row of a that ends after it
+    if (i < rows && i * a_stride < start + b_width) return true;
+  }
+  return false;
+}
+
 }  // namespace
 
 void select_tokens(const Kv4Eviction& e, int32_t* keep, uint32_t* kept_lens, cudaStream_t stream) {
@@ -462,6 +477,9 @@ void select_tokens(const Kv4Eviction& e, int32_t* keep, uint32_t* kept_lens, cud
   if (!keep || !kept_lens) throw std::invalid_argument("keep and kept_lens must be non-null");
   if (!aligned_to(keep, 4) || !aligned_to(kept_lens, 4))
     throw std::invalid_argument("keep and kept_lens must be 4-byte aligned");
+  // Every CTA of a sequence reads its length, one writes what is kept of it.
+  if (kept_lens < e.seq_lens + e.batch && e.seq_lens < kept_lens + e.batch)
+    throw std::invalid_argument("kept_lens must not overlap seq_lens");
   kvb::SelectParams prm{e.seq_lens, e.weights,    e.weight_stride, keep,    kept_lens, e.batch,
                         e.kv_heads, e.max_tokens, e.budget,        e.sinks, e.recent};
   // CTAs a segment: one for every 2,048 tokens, at most the eight of a
@@ -499,6 +517,10 @@ void compact_kv4(const Kv4Pool& pool, const Kv4Eviction& e, const uint32_t* bloc
     throw std::invalid_argument("budget exceeds the new block-table row capacity");
   if (new_weights != nullptr && new_weight_stride < int64_t(e.budget))
     throw std::invalid_argument("new_weight_stride must be at least budget");
+  // CTAs write the new rows while others read the old ones.
+  if (new_weights != nullptr && rows_overlap(e.weights, e.weight_stride, e.max_tokens, new_weights, new_weight_stride,
+                                             e.budget, int64_t(e.batch) * e.kv_heads))
+    throw std::invalid_argument("new_weights must not overlap weights");
   kvb::CompactParams prm{view(pool),   e.seq_lens,   e.weights,   e.weight_stride,   block_table,
                          keep,         new_table,    new_weights, new_weight_stride, e.batch,
                          e.max_tokens, e.budget,     table_stride, new_stride,       pool.page_tokens,

@@ -284,7 +284,7 @@ class EvictPlan:
 
 def select_tokens(plan: EvictPlan, keep, kept_lens, stream=None) -> None:
     """``keep`` int32 [batch, kv_heads, budget]: the kept tokens, ascending, then
-    zeros; ``kept_lens`` int32 [batch]."""
+    zeros; ``kept_lens`` int32 [batch], a tensor apart from ``seq_lens``."""
     check(
         _lib.load().kvb_select_tokens(
             plan._ref, _tensor("keep", keep, torch.int32, plan._keep_shape, plan.device),
@@ -296,7 +296,8 @@ def select_tokens(plan: EvictPlan, keep, kept_lens, stream=None) -> None:
 def compact_kv4(pool: Kv4Pool, plan: EvictPlan, keep, new_table, new_weights=None, stream=None) -> None:
     """Copy the kept tokens in order to the pages of ``new_table`` int32 [batch,
     pages] (pages that the plan's block table does not use) and their weights to
-    ``new_weights`` float32 [batch, kv_heads, >= budget] (the first budget of each)."""
+    ``new_weights`` float32 [batch, kv_heads, >= budget] (the first budget of each),
+    a tensor apart from the plan's."""
     if pool.device != plan.device:
         raise ValueError("the plan's device differs from the pool's")
     if new_table.dim() != 2 or new_table.shape[0] != plan.batch:

@@ -2,6 +2,7 @@
 whose values share a sign, at bounds of the digits that the kernels hold."""
 from __future__ import annotations
 
+import ctypes
 from dataclasses import replace
 
 import numpy as np
@@ -9,6 +10,7 @@ import pytest
 import torch
 
 import kvbridge_b200 as kvb
+from kvbridge_b200 import _lib
 
 import kv4_testutil as util
 from kv4_testutil import EPS, ROUND, SMALLEST, Rule, make_cache
@@ -236,3 +238,50 @@ def test_negative_prefixes_are_none(cuda_device, rule, positions, batch):
     check = util.device_query(cache, valid, cuda_device)
     util.attend(cache, valid, cuda_device, pool=pool, query=check)
     assert kvb.read_device_status() == 0
+
+
+def test_eviction_in_place_is_refused(kvb_lib):
+    """Lengths and weights are read by CTAs that run beside the one that writes
+    their successors, so these may not share memory. No call here gets to a launch."""
+    base = 0x10000000  # never dereferenced
+    pool = _lib.KvbKv4Pool(3, 64, 16, 100, *[base] * 4, None)
+    plan = _lib.KvbKv4Eviction(2, 3, 200, 96, 4, 16, base, base, 256)
+
+    def select(kept_lens):
+        return kvb_lib.kvb_select_tokens(ctypes.byref(plan), base + 4096, kept_lens, None), _lib.last_error()
+
+    def compact(new_weights, stride):
+        return kvb_lib.kvb_compact_kv4(ctypes.byref(pool), ctypes.byref(plan), base, 16, base, base, 8, new_weights, stride,
+                                       None), _lib.last_error()
+
+    for at in (-4, 0, 4):
+        assert select(base + at) == (_lib.KVB_EINVAL, "kept_lens must not overlap seq_lens")
+    row = 4 * 256
+    overlapping = [(base, 256), (base + 4 * 199, 256), (base - 4 * 95, 96), (base + 4 * 200, 257), (base + 4 * 161, 256),
+                   (base + 5 * row + 4 * 199, 96), (base - 5 * row, 256), (base - 4 * 480 - 4 * 95, 96)]
+    for at, stride in overlapping:
+        assert compact(at, stride) == (_lib.KVB_EINVAL, "new_weights must not overlap weights"), (at - base, stride)
+
+
+@pytest.mark.gpu
+def test_compaction_into_the_same_rows_beside_the_weights(cuda_device):
+    """Rows that hold the old weights and then the new ones share no float: allowed."""
+    lens, heads, budget = [150, 200], 3, 96
+    cache = make_cache(lens, heads, 64, 16, seed=71, spare=12)
+    pool, device = cache.to(cuda_device), cuda_device
+    both = torch.rand((2, heads, 400), device=device)
+    before = both.clone()
+    free = [p for p in range(pool.pages) if p not in cache.table[0, :10].tolist() + cache.table[1, :13].tolist()]
+    new_table = torch.tensor(free[:12], dtype=torch.int32, device=device)
+    table, seq_lens = cache.table.to(device), torch.tensor(lens, dtype=torch.int32, device=device)
+    keep = torch.empty((2, heads, budget), dtype=torch.int32, device=device)
+    kept = torch.empty(2, dtype=torch.int32, device=device)
+    plan = _lib.KvbKv4Eviction(2, heads, 200, budget, 4, 16, seq_lens.data_ptr(), both.data_ptr(), 400)
+    lib = _lib.load()
+    torch.cuda.synchronize()
+    _lib.check(lib.kvb_select_tokens(ctypes.byref(plan), keep.data_ptr(), kept.data_ptr(), None))
+    _lib.check(lib.kvb_compact_kv4(pool._ref, ctypes.byref(plan), table.data_ptr(), table.shape[1], keep.data_ptr(),
+                                   new_table.data_ptr(), 6, both.data_ptr() + 4 * 200, 400, None))
+    torch.cuda.synchronize()
+    assert torch.equal(both[..., :200], before[..., :200]) and torch.equal(both[..., 296:], before[..., 296:])
+    assert torch.equal(both[..., 200:296], before.gather(-1, keep.long()))
