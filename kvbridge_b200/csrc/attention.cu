@@ -1095,11 +1095,14 @@ void append_kv(const AppendShape& s, const AppendInput& in, cudaStream_t stream)
 
 cudaError_t read_device_status(int* status) {
   if (status == nullptr) return cudaErrorInvalidValue;
+  // Cleared only where it holds something: a copy the less, and a code that
+  // arrives between the two copies is kept for the next call.
   int value = 0;
   cudaError_t code = cudaMemcpyFromSymbol(&value, kvb::g_kvb_status, sizeof(int));
   if (code != cudaSuccess) return code;
+  *status = value;
   const int zero = 0;
-  code = cudaMemcpyToSymbol(kvb::g_kvb_status, &zero, sizeof(int));
+  if (value != 0) code = cudaMemcpyToSymbol(kvb::g_kvb_status, &zero, sizeof(int));
   if (code != cudaSuccess) return code;
   int kv4 = 0;
   code = detail::read_kv4_status(&kv4);

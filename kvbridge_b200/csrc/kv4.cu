@@ -1,5 +1,6 @@
 // Launchers of the 4-bit cache operators (include/kvbridge/attention_kv4.h).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <limits>
 #include <map>
@@ -22,7 +23,16 @@ namespace {
 
 using detail::aligned_to;
 using detail::cuda_ok;
-using detail::launch_kernel_pdl;
+
+// Whether this process has launched a kernel of this module (or captured one):
+// until then reading the status leaves the module unloaded.
+std::atomic<bool> g_launched{false};
+
+void launch_kernel_pdl(const void* fn, dim3 grid, dim3 block, uint32_t smem, cudaStream_t stream, void** args,
+                       const char* what) {
+  g_launched.store(true, std::memory_order_relaxed);
+  detail::launch_kernel_pdl(fn, grid, block, smem, stream, args, what);
+}
 
 constexpr uint32_t kMaxColumns = 128;  // query rows x heads of a KV head
 
@@ -495,6 +505,7 @@ void select_tokens(const Kv4Eviction& e, int32_t* keep, uint32_t* kept_lens, cud
   const Kv4Kernel k{reinterpret_cast<const void*>(&kvb::select_tokens_kernel), kvb::kSelectKeys * uint32_t(sizeof(uint32_t))};
   resident_ctas(k, kvb::kSelectThreads);
   void* args[] = {&prm};
+  g_launched.store(true, std::memory_order_relaxed);
   detail::launch_kernel_cluster(k.fn, dim3(e.batch * e.kv_heads * ctas), dim3(kvb::kSelectThreads), ctas, smem, stream, args,
                                 "token selection launch");
 }
@@ -538,8 +549,10 @@ void compact_kv4(const Kv4Pool& pool, const Kv4Eviction& e, const uint32_t* bloc
 namespace detail {
 
 cudaError_t read_kv4_status(int* status) noexcept {
-  cudaError_t code = cudaMemcpyFromSymbol(status, kvb::g_kvb_status, sizeof(int));
-  if (code != cudaSuccess) return code;
+  *status = 0;
+  if (!g_launched.load(std::memory_order_relaxed)) return cudaSuccess;
+  const cudaError_t code = cudaMemcpyFromSymbol(status, kvb::g_kvb_status, sizeof(int));
+  if (code != cudaSuccess || *status == 0) return code;
   const int zero = 0;
   return cudaMemcpyToSymbol(kvb::g_kvb_status, &zero, sizeof(int));
 }

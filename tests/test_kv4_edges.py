@@ -3,7 +3,11 @@ whose values share a sign, at bounds of the digits that the kernels hold."""
 from __future__ import annotations
 
 import ctypes
+import json
+import subprocess
+import sys
 from dataclasses import replace
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -285,3 +289,41 @@ def test_compaction_into_the_same_rows_beside_the_weights(cuda_device):
     torch.cuda.synchronize()
     assert torch.equal(both[..., :200], before[..., :200]) and torch.equal(both[..., 296:], before[..., 296:])
     assert torch.equal(both[..., 200:296], before.gather(-1, keep.long()))
+
+
+COUNT_COPIES = """
+import json, warnings
+import torch
+from torch.profiler import ProfilerActivity, profile
+import kvbridge_b200 as kvb
+
+def copies():
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        with profile(activities=[ProfilerActivity.CUDA]) as p:
+            status = kvb.read_device_status()
+            torch.cuda.synchronize()
+    count = {e.key: e.count for e in p.key_averages()}
+    return [status, count.get("cudaMemcpyFromSymbol", 0), count.get("cudaMemcpyToSymbol", 0)]
+
+torch.zeros(1, device="cuda")
+copies()
+result = [copies()]
+pool = kvb.Kv4Pool.empty(2, 1, 16, 64)
+x = torch.zeros((1, 1, 64), device="cuda")
+for slot in (3, 32):
+    kvb.append_kv4(pool, kvb.Kv4Rows(x, x, torch.tensor([slot], device="cuda")))
+    result.append(copies())
+result.append(copies())
+print(json.dumps(result))
+"""
+
+
+@pytest.mark.gpu
+def test_reading_the_status_costs_no_more_than_its_words(cuda_device):
+    """[status, copies from the device, copies to it]: one word where the 4-bit
+    kernels have not run, two where they have, and a reset only of a code."""
+    root = Path(__file__).resolve().parents[1]
+    run = subprocess.run([sys.executable, "-c", COUNT_COPIES], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
+    assert json.loads(run.stdout.splitlines()[-1]) == [[0, 1, 0], [0, 2, 0], [6, 2, 1], [0, 2, 0]]
