@@ -709,7 +709,7 @@ __device__ __forceinline__ void kv4_dots(const uint8_t* codes, const Kv4Query<D,
 // is all of most stages, else 1 - 2 / (e^2y + 1), which cancels near 0.
 template <int N>
 __device__ __forceinline__ void kv4_cap(float cap, float (&x)[N]) {
-  const float inv = 1.0f / cap;
+  const float inv = fminf(1.0f / cap, 3.402823466e38f);  // (a denormal cap's is infinite: 0 * inf)
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(x[i]));  // (a NaN takes either way)

@@ -327,3 +327,16 @@ def test_reading_the_status_costs_no_more_than_its_words(cuda_device):
     run = subprocess.run([sys.executable, "-c", COUNT_COPIES], cwd=root, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr
     assert json.loads(run.stdout.splitlines()[-1]) == [[0, 1, 0], [0, 2, 0], [6, 2, 1], [0, 2, 0]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("softcap", [1e-45, 1e-39, 1e-30, 1e30, 3e38])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_caps_at_the_ends_of_the_range(cuda_device, softcap, dtype):
+    """Caps whose reciprocal overflows or vanishes, with queries that score 0 too."""
+    cache = make_cache([70, 300], 2, 128, 64, seed=81)
+    rule = util.make_query(cache, Rule(softcap=softcap, rows=2, dtype=dtype), 82)
+    rule.q[0, 1] = 0
+    rule.q[1, :, ::3] = 0
+    out, lse = util.check_attention(cache, rule, cuda_device)
+    assert np.all(np.isfinite(lse)) and np.all(np.isfinite(out))
