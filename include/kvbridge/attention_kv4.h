@@ -139,9 +139,11 @@ void select_tokens(const Kv4Eviction&, int32_t* keep, uint32_t* kept_lens, cudaS
 // and KV head in order to the pages new_table[b * new_stride + j] of the
 // same pool, which no block table of the call may use, and their weights to
 // new_weights (optional; `budget` values a row, zeros after the kept ones,
-// rows new_weight_stride apart, none in the place of the old ones). A kept token beyond its sequence or beyond
-// the block table's row is skipped and reported. The old pages are only read, so sequences
-// may share them; the caller frees them afterwards.
+// rows new_weight_stride apart, none in the place of the old ones). A kept
+// token beyond its sequence, beyond the block table's row or on a page that is
+// not in the pool is reported, and its new slot holds a row of NaN (position
+// 0). The old pages are only read, so sequences may share them; the caller
+// frees them afterwards.
 void compact_kv4(const Kv4Pool&, const Kv4Eviction&, const uint32_t* block_table,
                  uint32_t table_stride, const int32_t* keep, const uint32_t* new_table,
                  uint32_t new_stride, float* new_weights, int64_t new_weight_stride, cudaStream_t);

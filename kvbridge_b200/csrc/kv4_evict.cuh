@@ -306,8 +306,16 @@ __global__ void __launch_bounds__(kCompactThreads) compact_kv4_kernel(const Comp
   for (uint32_t i = tid; i < kCompactTile * kChunks; i += kCompactThreads) {
     const uint32_t t = i / kChunks, c = i % kChunks;
     const uint64_t from = src_at[t], unit = dst_unit[t / 16];
-    if (from == kNowhere || unit == kNowhere) continue;
+    if (unit == kNowhere || first + t >= kept) continue;
     const uint64_t to = unit * P + ((first + t) & (P - 1));
+    if (from == kNowhere) {  // a row that is not a number, for whatever the slot holds
+      if (c < 2) {
+        const float nan = __int_as_float(0x7fffffff);
+        (c == 0 ? p.pool.kp : p.pool.vp)[to] = make_float2(nan, nan);
+        if (c == 0 && p.pool.pos != nullptr) p.pool.pos[to] = 0;
+      }
+      continue;
+    }
     reinterpret_cast<uint4*>(p.pool.k)[to * kChunks + c] = kv4_stream(reinterpret_cast<const uint4*>(p.pool.k) + from * kChunks + c);
     if (c == 0) p.pool.kp[to] = p.pool.kp[from];
     if (c == 1) p.pool.vp[to] = p.pool.vp[from];

@@ -340,3 +340,45 @@ def test_caps_at_the_ends_of_the_range(cuda_device, softcap, dtype):
     rule.q[1, :, ::3] = 0
     out, lse = util.check_attention(cache, rule, cuda_device)
     assert np.all(np.isfinite(lse)) and np.all(np.isfinite(out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (256, 64)])
+@pytest.mark.parametrize("positions", [False, True])
+def test_skipped_kept_tokens_leave_nan(cuda_device, dim, page, positions):
+    """The new slot of a kept token that cannot be moved holds NaN and position 0,
+    not what the page held before; the others are moved."""
+    budget, heads = 150, 2
+    cache = make_cache([400], heads, dim, page, seed=91, spare=2 * -(-budget // page), positions=positions)
+    pool = cache.to(cuda_device)
+    used = cache.table[0, :-(-400 // page)].tolist()
+    new = [p for p in range(pool.pages) if p not in used][:-(-budget // page)]
+    table = cache.table.clone()
+    table[0, 2 * 64 // page] = NO_PAGE  # tokens from 128 on
+    lens, kept = (torch.tensor([n], dtype=torch.int32, device=cuda_device) for n in (400, 0))
+    weights = torch.rand((1, heads, 400), device=cuda_device)
+    plan = kvb.EvictPlan(weights, lens, table.to(cuda_device), budget=budget, sinks=4, recent=20)
+    keep = torch.empty((1, heads, budget), dtype=torch.int32, device=cuda_device)
+    kvb.select_tokens(plan, keep, kept)
+    keep[0, 0, 70], keep[0, 1, 3] = 400, -1  # beyond the sequence, and no token
+    for name in ("k_params", "v_params"):
+        getattr(pool, name)[torch.tensor(new, device=cuda_device)] = 0.5
+    kvb.read_device_status()
+    kvb.compact_kv4(pool, plan, keep, torch.tensor([new], dtype=torch.int32, device=cuda_device))
+    assert kvb.read_device_status() == 8
+    at = torch.arange(budget)
+    pages, slots = torch.tensor(new)[at // page], at % page
+    for h in range(heads):
+        t = keep[0, h].cpu().long()
+        gone = (t < 0) | (t >= 400) | (t // page == 2 * 64 // page)
+        assert bool(gone.any()) and not bool(gone.all())
+        source = table[0].long()[t.clamp(0, 399) // page], h, t.clamp(0, 399) % page
+        for name in ("k_params", "v_params"):
+            got = getattr(pool, name).cpu()[pages, h, slots]
+            assert torch.isnan(got[gone]).all()
+            assert torch.equal(got[~gone], getattr(cache, name)[source][~gone])
+        if positions:
+            want = torch.where(gone, 0, cache.positions[source])
+            assert torch.equal(pool.positions.cpu()[pages, h, slots], want)
+    last = budget % page  # nothing is written past the kept tokens
+    assert torch.all(pool.k_params[new[-1], :, last:] == 0.5) and torch.all(pool.v_params[new[-1], :, last:] == 0.5)
