@@ -183,6 +183,7 @@ class Kv4Query:
         if q.dtype not in TYPES:
             raise ValueError(f"q must be float32, float16 or bfloat16, not {q.dtype}")
         batch, rows, q_heads, dim = q.shape
+        _device("block_table", block_table, self.device)
         if block_table.dim() != 2:
             raise ValueError("block_table must have shape [batch, width]")
         if kv_heads < 1 or q_heads % kv_heads:
@@ -239,6 +240,7 @@ def accumulate_weights_kv4(pool: Kv4Pool, query: Kv4Query, lse, weights, stream=
     weight each token gets from the query rows, given their ``lse``."""
     _match_query(pool, query)
     batch = query.shape[0]
+    _device("weights", weights, pool.device)
     if weights.dim() != 3 or weights.shape[:2] != (batch, pool.kv_heads):
         raise ValueError("weights must have shape [batch, kv_heads, >= max_tokens]")
     check(
@@ -300,6 +302,9 @@ def compact_kv4(pool: Kv4Pool, plan: EvictPlan, keep, new_table, new_weights=Non
     a tensor apart from the plan's."""
     if pool.device != plan.device:
         raise ValueError("the plan's device differs from the pool's")
+    _device("new_table", new_table, pool.device)
+    if new_weights is not None:
+        _device("new_weights", new_weights, pool.device)
     if new_table.dim() != 2 or new_table.shape[0] != plan.batch:
         raise ValueError("new_table must have shape [batch, pages]")
     if new_weights is not None and (new_weights.dim() != 3 or new_weights.shape[:2] != (plan.batch, plan.kv_heads)):

@@ -382,3 +382,27 @@ def test_skipped_kept_tokens_leave_nan(cuda_device, dim, page, positions):
             assert torch.equal(pool.positions.cpu()[pages, h, slots], want)
     last = budget % page  # nothing is written past the kept tokens
     assert torch.all(pool.k_params[new[-1], :, last:] == 0.5) and torch.all(pool.v_params[new[-1], :, last:] == 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wrong", [None, [[0, 1]], torch.zeros((2, 3), dtype=torch.int32)], ids=["none", "list", "host"])
+def test_what_is_no_cuda_tensor_raises_value_errors(cuda_device, wrong):
+    cache = make_cache([70], 1, 64, 16, seed=95)
+    rule = util.make_query(cache, Rule(group=1), 96)
+    pool, query = cache.to(cuda_device), util.device_query(cache, rule, cuda_device)
+    lens = torch.tensor([70], dtype=torch.int32, device=cuda_device)
+    lse, table = torch.zeros(query.lse_shape, device=cuda_device), cache.table.to(cuda_device)
+    plan = kvb.EvictPlan(torch.rand((1, 1, 70), device=cuda_device), lens, table, budget=16)
+    keep = torch.zeros((1, 1, 16), dtype=torch.int32, device=cuda_device)
+    for call in (
+        lambda: kvb.Kv4Query(rule.q.to(cuda_device), lens, wrong, 70, 1, 0.1),
+        lambda: kvb.Kv4Query(rule.q.to(cuda_device), wrong, table, 70, 1, 0.1),
+        lambda: kvb.EvictPlan(plan.weights, lens, wrong, budget=16),
+        lambda: kvb.accumulate_weights_kv4(pool, query, lse, wrong),
+        lambda: kvb.accumulate_weights_kv4(pool, query, wrong, plan.weights),
+        lambda: kvb.compact_kv4(pool, plan, keep, wrong),
+        lambda: kvb.compact_kv4(pool, plan, keep, table, [0.0]),
+        lambda: kvb.launch_attention_kv4(pool, query, wrong, torch.empty_like(query.q)),
+    ):
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            call()
