@@ -406,3 +406,48 @@ def test_what_is_no_cuda_tensor_raises_value_errors(cuda_device, wrong):
     ):
         with pytest.raises(ValueError, match="CUDA tensor"):
             call()
+
+
+def spread(x, offset, extra):
+    """x [tokens, ..] as a view whose tokens lie `extra` elements further apart, from `offset` on."""
+    row = x[0].numel()
+    flat = torch.zeros(offset + len(x) * (row + extra), dtype=x.dtype, device=x.device)
+    return flat.as_strided(x.shape, (row + extra,) + x[0].stride(), offset).copy_(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("offset,extra", [(1, 0), (0, 1), (3, 5), (8, 4)])
+def test_rows_queries_and_outputs_off_16_bytes(cuda_device, dtype, offset, extra):
+    """Elements' own alignment is enough for rows, queries and outputs, and strides may be odd."""
+    cache = make_cache([130, 70, 300], 2, 128, 32, seed=101)
+    rule = util.make_query(cache, Rule(rows=2, group=4, dtype=dtype), 102)
+    want = util.expected(cache, rule)
+    pool, plain = cache.to(cuda_device), util.device_query(cache, rule, cuda_device)
+    q = spread(rule.q.to(cuda_device).flatten(0, 1), offset, extra)  # batch and row strides
+    q = q.as_strided(rule.q.shape, (2 * q.stride(0),) + q.stride(), offset)
+    query = kvb.Kv4Query(q, *plain._kept[:2], max_tokens=300, kv_heads=2, scale=128 ** -0.5)
+    space = torch.empty(kvb.attention_kv4_workspace_bytes(pool, query), dtype=torch.uint8, device=cuda_device)
+    out, same = torch.full((q.numel() + 16,), np.nan, dtype=dtype, device=cuda_device), torch.empty_like(plain.q)
+    kvb.launch_attention_kv4(pool, query, space, out[offset:offset + q.numel()].view(q.shape))
+    kvb.launch_attention_kv4(pool, plain, space, same)
+    assert torch.equal(out[offset:offset + q.numel()].view(q.shape), same)
+    assert torch.isnan(out[:offset]).all() and torch.isnan(out[offset + q.numel():]).all()
+    assert np.all(np.abs(same.double().cpu().numpy() - want.out) <= want.out_tol)
+
+    g = torch.Generator().manual_seed(103)
+    k, v = (torch.randn((100, 2, 128), generator=g).to(dtype).to(cuda_device) for _ in range(2))
+    slots = (torch.arange(100) + 7).to(cuda_device)
+    pools = [kvb.Kv4Pool.empty(4, 2, 32, 128, device=cuda_device) for _ in range(2)]
+    for p in pools:
+        for x in (p.k, p.v, p.k_params, p.v_params):
+            x.zero_()
+    kvb.append_kv4(pools[0], kvb.Kv4Rows(k, v, slots))
+    kvb.append_kv4(pools[1], kvb.Kv4Rows(spread(k, offset, extra), spread(v, 2 * offset, extra), slots))
+    for name in ("k", "v", "k_params", "v_params"):
+        assert torch.equal(getattr(pools[0], name), getattr(pools[1], name))
+    dense = [torch.empty_like(k) for _ in range(2)]
+    kvb.load_kv4(pools[0], kvb.Kv4Rows(*dense, slots))
+    apart = [spread(torch.zeros_like(k), offset, extra), spread(torch.zeros_like(v), offset, extra)]
+    kvb.load_kv4(pools[0], kvb.Kv4Rows(*apart, slots))
+    assert torch.equal(dense[0], apart[0]) and torch.equal(dense[1], apart[1])
