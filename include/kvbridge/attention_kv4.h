@@ -28,6 +28,12 @@
 // 2 * (dim / 2 + 8) bytes a token and KV head: 144 at dim 128, where the
 // int8 layout takes 264.
 //
+// Arithmetic. Sums, softmax statistics, the log-sum-exp and the weights are
+// fp32. Two values are held in fixed point: a query element to 2^-22 of its row's
+// largest (in fp32 rows too), and the product of a probability and a V scale to
+// 2^-16 (fp32 outputs 2^-23) of the largest of 64 tokens. Both stay far below
+// what the 4-bit codes leave open, half a step of every value.
+//
 // Entry points throw std::invalid_argument before anything is enqueued for
 // bad metadata or null or misaligned buffers, and std::runtime_error for
 // CUDA failures. Every buffer is a device pointer that the caller owns; the

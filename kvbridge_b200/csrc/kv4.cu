@@ -243,8 +243,9 @@ struct Kv4Kernel {
 // 168 at three, 255 at two. (Dim 128, 8 columns: three CTAs 83 us for 16x16K
 // tokens, four 94 us with 160 bytes of spills; 4 columns: 1x64K 26.6 us at
 // three, 28.0 us at four. Weights of 32 sequences of 1K to 32K tokens, 8
-// columns: three 82 us, with cap and bias 115 us; four, which spill, 81 and 117
-// us; 1x64K, 4 columns, 13.1 against 13.4 us.)
+// columns: three (48 to 80 bytes of spills) 82 us, with cap and bias 115 us; four
+// (64 to 128 bytes) 81 and 117 us; 1x64K, 4 columns, which spill at four alone,
+// 13.1 against 13.4 us.)
 constexpr int attend_ctas(int dim) { return dim == 256 ? 2 : dim == 64 ? 4 : 3; }
 
 template <int D, int C, int PD, int RULES>

@@ -40,19 +40,25 @@
 //          and c + 12 those of the other's, zeros for the rest; each lane
 //          sums its own share of the output. PD = 3: digit 2 in the same rows
 //          of a second tile.
-// PD = 2 holds P to 2^-16 of the tile's largest, below the rounding of 16-bit
-// outputs; fp32 outputs take 3. The lse is fp32 always, hence three q digits.
+// PD = 2 holds P * v_scale to 2^-16 of the tile's largest: a token's part of the
+// output is off by at most 8 * 2^-16 of that, where its codes stand for values
+// known to half of their step only (2^-1 of P * v_scale). One f16 sequence of
+// 64K tokens ends 2.15e-4 from 64 bits, the exact result rounded to f16 2.12e-4;
+// bf16 shows no difference. fp32 outputs take 3. Queries are held to 2^-22 of
+// their row's largest, fp32 ones too, by the same argument against the keys'
+// codes; the lse is fp32 always, hence three q digits for every type.
 //
 // Bound: 144 bytes a cached token and KV head at dim 128, and 4 * dim flops a
 // token and query row. With four query columns a KV head the copies bound it:
-// 32 sequences of 1K to 32K tokens (612 MB) take 105 us, 5.8 TB/s. With eight,
+// 32 sequences of 1K to 32K tokens (612 MB) take 106 us, 5.8 TB/s. With eight,
 // or at dim 256 with digits for several rows, the instructions between the
 // copies do (issue slots half used at twelve warps an SM, the rest waits for
 // the warp's own chain of products and shuffles): 64 x 16K tokens with 16-token
-// pages 248 us, 4.9 TB/s; eight rows of 24 heads of dim 256 over 32K tokens 60
-// us, 0.1 PFLOP/s. Short calls are bound by latency: one sequence of 4,096
-// tokens takes 10.7 us, of which the two kernels' starts and the merge are
-// about 7.
+// pages 249 us, 4.9 TB/s; eight rows of 24 heads of dim 256 over 32K tokens 60
+// to 64 us, 0.1 PFLOP/s. Explicit positions mask every stage and are loaded
+// within it: 16 x 16K tokens with 4 columns 75 us so, 59 us by index. Short calls
+// are bound by latency: one sequence of 4,096 tokens takes 11.0 us, of which the
+// two kernels' starts and the merge are about 7.
 #include "kv4_common.cuh"
 #include "kvb_schedule.h"
 
@@ -1258,8 +1264,10 @@ __global__ void __launch_bounds__(32 * kKv4MergeWarps, HELD == 8 ? 2 : 1) merge_
 // groups needs every group's digits in registers, or atomics, whose order
 // changes the sums.) Reads half of what attention does and a float a token,
 // writes the float. Bound by the instructions of the scores: 32 sequences of
-// 1K to 32K tokens, eight columns, take 82 us, 4.2 TB/s; 5,000 tokens 5.6 us,
-// a kernel's latency.
+// 1K to 32K tokens, eight columns, take 82 us, 4.2 TB/s; 5,000 tokens 5.5 to 6.2
+// us, a kernel's latency. K and the weights are read again for every eight
+// columns: 16 x 4,096 tokens take 15 us with 8, 28 with 16, 80 with 48 and 208
+// with 128.
 
 template <int D, int C, int MINB, int RULES>
 __global__ void __launch_bounds__(kKv4Threads, MINB) weigh_kv4_kernel(const Kv4AttendParams p, uint32_t group) {
