@@ -33,8 +33,8 @@ scales of every attended token and KV head: 2,112 B/token at 8 x 128) per
 call / time per call; ms_per_step is the time per call.
 
 `--impl reference` times the reference's own CPU implementation (its FP64
-oracle compiled from its sources into oracle/_ref; the C restatement in
-oracle/ when that build is absent) on the host cores, rank 0 only.
+oracle compiled from its sources into oracle/_ref) on the host cores, rank 0
+only; without that build it prints an `unavailable` line.
 """
 from __future__ import annotations
 
@@ -251,14 +251,18 @@ def run_reference_arm(args):
     rank = int(os.environ.get("RANK", "0"))
     if rank != 0:
         return 0
+    import oracle
+
+    if not oracle.RefOracle.available():
+        # The C restatement in oracle/ is this repository's code, not the reference.
+        print(json.dumps({"impl": "reference",
+                          "unavailable": "oracle/_ref is not built: the reference's sources are not here"}), flush=True)
+        return 0
     threads = os.cpu_count() or 1
     steps, warmup = args.steps, args.warmup
     # Each step is a bounded sample: the full 32-head computation over a
     # contiguous token range sized so that warmup + steps take ~90 s.
     full = sample_case(65536, "cpu")
-    import oracle
-
-    kind = "reference" if oracle.RefOracle.available() else "port"
     # Calibrate the per-token cost on 4,096 tokens.
     calib_tokens = 4096
     cal = sample_case(65536, "cpu")
@@ -297,11 +301,9 @@ def run_reference_arm(args):
             "value": round(value, 4),
             "unit": "GB/s",
             "cores": threads,
-            "kind": kind,
+            "kind": "reference",
             "sample": f"each step: the last {tokens} of 65,536 tokens for all 32 q-heads "
-                      f"({threads} threads, "
-                      + ("the reference's FP64 CPU oracle built from its sources)" if kind == "reference"
-                         else "the C restatement of the reference's FP64 oracle)"),
+                      f"({threads} threads, the reference's FP64 CPU oracle built from its sources)",
         },
         "e2e": {"value": round(value, 4), "unit": "GB/s", "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0},
     }
